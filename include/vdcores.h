@@ -154,6 +154,85 @@ int vdc_step_workspace(const vdc_step* step, uint64_t* bytes);
  * overlap. */
 int vdc_launch_step(const vdc_step* step, uint64_t stream, uint64_t timeout_ns);
 
+/* ---- Operators for drafted tokens: they serve several sequences whose pages lie in one pool, and take their arguments as
+ * device memory described by a struct.  None of them synchronises, allocates or keeps anything between calls, so calls on
+ * different streams do not meet.  What they find wrong in device memory (a length, page, position or request outside what the
+ * struct says) is reported as VDC_ERR_RANGE through vdc_read_status; the row concerned is left out (its outputs are zero, a
+ * picked token -1).  Pointers are device addresses, multiples of 16 where not said otherwise; strides of tensors are in
+ * elements, those of pages in bytes.  No counterpart in the reference.
+ *
+ * A cache of one layer: page p and KV head h at k + p * k_page + h * k_head (v alike): VDC_KV_PAGE rows of VDC_HEAD_DIM values,
+ * row r's 16-byte pieces at index (piece XOR (r mod 8)).  kind 0: bf16, as the decode engines keep it.  kind 1: e4m3 codes; row r
+ * stands for code * scale with the fp32 scale number r at k_scale + p * ks_page + h * ks_head (v_scale alike).  Page strides are
+ * multiples of 16. */
+typedef struct {
+  uint64_t k, v, k_scale, v_scale;
+  int64_t k_page, k_head, v_page, v_head, ks_page, ks_head, vs_page, vs_head;
+  int32_t kind, n_kv, n_pages, reserved;
+} vdc_cache;
+
+/* New tokens on their way into attention: T per sequence, `group` query heads to a KV head.
+ *   q [B, T, n_kv, group, 128], k and v [B, T, n_kv, 128], out like q: bf16, strides multiples of 8; out may be q.
+ *   lengths int32 [B]: rows the sequence holds; token t goes to row lengths[b] + t, that is to row % 64 of page
+ *     pages[b * pages_b + row / 64] (int32, max_pages to a sequence)
+ *   counts int32 [B] (0: T each): the sequence's tokens; those behind them write no cache rows, and zeros to out
+ *   q_norm, k_norm bf16 [128] (0: none): x / sqrt(mean x^2 + eps) * w in front of the rotation
+ *   table fp32 [table_rows, rot]: cos of rot / 2 angles, then sin; rot a multiple of 16 up to 128, 0 for no rotation
+ *   positions int32 [B, T] (0: the token's row): the table's row
+ *   interleaved 0: value i turns with i + rot / 2; 1: 2i with 2i + 1
+ * The arithmetic is fp32, rounded once when a value is stored; an e4m3 row's scale is its largest magnitude / 448. */
+typedef struct {
+  vdc_cache cache;
+  int32_t B, T, group, rot, interleaved, table_rows, max_pages;
+  float eps;
+  int64_t q_b, q_t, q_kv, q_g, k_b, k_t, k_kv, v_b, v_t, v_kv, o_b, o_t, o_kv, o_g, pages_b, pos_b, pos_t;
+  uint64_t q, k, v, out, pages, lengths, counts, table, positions, q_norm, k_norm;
+} vdc_rope_append_args;
+int vdc_rope_append(const vdc_rope_append_args* args, uint64_t stream);
+
+/* Rows start[b] .. start[b] + n - 1 (start 0: from row 0) of every sequence to k_out and v_out [B, n, n_kv, 128] bf16, dense;
+ * rows at or behind lengths[b] become zeros. */
+typedef struct {
+  vdc_cache cache;
+  int32_t B, n, max_pages, reserved;
+  int64_t pages_b;
+  uint64_t pages, lengths, start, k_out, v_out;
+} vdc_read_cache_args;
+int vdc_read_cache(const vdc_read_cache_args* args, uint64_t stream);
+
+/* Attention of T drafted tokens per sequence whose cache rows are lengths[b] .. lengths[b] + T - 1: token i attends to every row
+ * in front of lengths[b] and to the drafted tokens j that its mask names: bit j % 64 of mask[b, i, j / 64] (int64, words to a
+ * token, strides mask_b and mask_t in words; 0: a chain, j <= i).  counts as above.  A token with nothing to attend to gets
+ * zeros; so do those behind counts[b].  q and out as above (out not q); scale multiplies the scores.
+ * A drafted token whose value row holds an infinity or NaN makes NaN what attends to it, and nothing else.
+ * work: vdc_tree_attention_workspace bytes, free to be anything before and after. */
+typedef struct {
+  vdc_cache cache;
+  int32_t B, T, group, max_pages, words;
+  float scale;
+  int64_t q_b, q_t, q_kv, q_g, o_b, o_t, o_kv, o_g, pages_b, mask_b, mask_t;
+  uint64_t q, out, pages, lengths, counts, mask, work;
+} vdc_tree_attention_args;
+int vdc_tree_attention_workspace(const vdc_tree_attention_args* args, uint64_t* bytes);
+int vdc_tree_attention(const vdc_tree_attention_args* args, uint64_t stream, uint64_t timeout_ns);
+
+/* Logits rows [rows, vocab] (type 0 fp32, 1 bf16, 2 f16; row strides in elements, pointers multiples of the element) to out
+ * (out_type the same or 0; may be the logits themselves).  Row r belongs to request q = requests[r] (0: r) of n:
+ *   history int32 [n, L] (row stride history_s): its first prompt_lens[q] (0: none) ids are the prompt, those up to history_lens[q]
+ *     (0: all L) were generated; path int32 [rows, path_n]: ids drafted in front of row r, counted as generated.  Ids outside
+ *     the vocabulary are ignored.
+ *   an id of either: l = l > 0 ? l / repetition[q] : l * repetition[q]; generated c times: l -= frequency[q] * c, and
+ *     l -= presence[q] where c > 0; then l += bias of bias_ids int32 [n, n_bias] (an id named twice: the sum in their order); then
+ *     -inf where bit id % 32 of allowed int32 [rows, (vocab + 31) / 32] is clear.  Each of them may be 0: not wanted.
+ * tokens int32 [rows] (0: not wanted): the lowest id of the largest adjusted logit in fp32, NaN left out; -1 where all are -inf. */
+typedef struct {
+  int32_t rows, vocab, type, out_type, n, L, path_n, n_bias;
+  int64_t logits_s, out_s, history_s, path_s, bias_s, allowed_s;
+  uint64_t logits, out, tokens, requests, history, prompt_lens, history_lens, path, repetition, frequency, presence, bias_ids, bias,
+      allowed;
+} vdc_adjust_logits_args;
+int vdc_adjust_logits(const vdc_adjust_logits_args* args, uint64_t stream);
+
 /* Synchronises `stream` and copies the device status block to *status; returns
  * its code.  Clears the block when `clear` is non-zero. */
 int vdc_read_status(uint64_t stream, vdc_status* status, int clear);

@@ -27,6 +27,18 @@ extern "C" cudaError_t vdc_wide_prepare();
 extern "C" void vdc_wide_choose(int rows, int M, int K, int wfmt, int sms, int whole, int* out);
 extern "C" int vdc_wide_grid(const vdc_stage* s, int sms, int* tiles);
 extern "C" cudaError_t vdc_wide_launch(const vdc_stage* s, int sms, vdc_status* status, uint64_t timeout_ns, cudaStream_t stream);
+extern "C" const char* vdc_rope_append_refuses(const vdc_rope_append_args* a);
+extern "C" cudaError_t vdc_rope_append_launch(const vdc_rope_append_args* a, vdc_status* status, cudaStream_t stream);
+extern "C" const char* vdc_read_cache_refuses(const vdc_read_cache_args* a);
+extern "C" cudaError_t vdc_read_cache_launch(const vdc_read_cache_args* a, vdc_status* status, cudaStream_t stream);
+extern "C" const char* vdc_adjust_logits_refuses(const vdc_adjust_logits_args* a);
+extern "C" cudaError_t vdc_adjust_logits_prepare();
+extern "C" cudaError_t vdc_adjust_logits_launch(const vdc_adjust_logits_args* a, vdc_status* status, cudaStream_t stream);
+extern "C" const char* vdc_tree_attention_refuses(const vdc_tree_attention_args* a, bool pointers);
+extern "C" long long vdc_tree_attention_bytes(const vdc_tree_attention_args* a);
+extern "C" cudaError_t vdc_tree_attention_prepare();
+extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* a, int sms, vdc_status* status, uint64_t timeout_ns,
+                                                 cudaStream_t stream);
 extern "C" void vdc_stage_slices(const vdc_stage* s, int max_ctas, int* launches, int* largest);
 
 namespace {
@@ -101,6 +113,8 @@ int vdc_init(void) {
   e = vdc_stage_prepare();
   if (e == cudaSuccess) e = vdc_wide_prepare();
   if (e == cudaSuccess) e = vdc_step_prepare();
+  if (e == cudaSuccess) e = vdc_adjust_logits_prepare();
+  if (e == cudaSuccess) e = vdc_tree_attention_prepare();
   if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(stage kernels)");
   vdc_status* st = nullptr;
   e = cudaMalloc(&st, sizeof(vdc_status));
@@ -298,6 +312,57 @@ int vdc_launch_step(const vdc_step* step, uint64_t stream, uint64_t timeout_ns) 
   return e == cudaSuccess ? VDC_OK : fail_cuda(e, "step launch");
 }
 
+// The operators for drafted tokens: what they refuse, then the launch.
+static int ready(vdc_status** status) {
+  int dev;
+  if (int r = current_device(&dev)) return r;
+  if (!g_status[dev]) return fail_arg("vdc_init was not called on this device");
+  *status = g_status[dev];
+  return VDC_OK;
+}
+
+int vdc_rope_append(const vdc_rope_append_args* args, uint64_t stream) {
+  if (const char* why = args ? vdc_rope_append_refuses(args) : "null argument") return fail_arg(why);
+  vdc_status* status;
+  if (int r = ready(&status)) return r;
+  cudaError_t e = vdc_rope_append_launch(args, status, reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? VDC_OK : fail_cuda(e, "rope_append launch");
+}
+
+int vdc_read_cache(const vdc_read_cache_args* args, uint64_t stream) {
+  if (const char* why = args ? vdc_read_cache_refuses(args) : "null argument") return fail_arg(why);
+  vdc_status* status;
+  if (int r = ready(&status)) return r;
+  cudaError_t e = vdc_read_cache_launch(args, status, reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? VDC_OK : fail_cuda(e, "read_cache launch");
+}
+
+int vdc_adjust_logits(const vdc_adjust_logits_args* args, uint64_t stream) {
+  if (const char* why = args ? vdc_adjust_logits_refuses(args) : "null argument") return fail_arg(why);
+  vdc_status* status;
+  if (int r = ready(&status)) return r;
+  cudaError_t e = vdc_adjust_logits_launch(args, status, reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? VDC_OK : fail_cuda(e, "adjust_logits launch");
+}
+
+int vdc_tree_attention_workspace(const vdc_tree_attention_args* args, uint64_t* bytes) {
+  if (!args || !bytes) return fail_arg("null argument");
+  if (const char* why = vdc_tree_attention_refuses(args, false)) return fail_arg(why);
+  *bytes = (uint64_t)vdc_tree_attention_bytes(args);
+  return VDC_OK;
+}
+
+int vdc_tree_attention(const vdc_tree_attention_args* args, uint64_t stream, uint64_t timeout_ns) {
+  if (const char* why = args ? vdc_tree_attention_refuses(args, true) : "null argument") return fail_arg(why);
+  vdc_status* status;
+  if (int r = ready(&status)) return r;
+  int dev;
+  if (int r = current_device(&dev)) return r;
+  cudaError_t e = vdc_tree_attention_launch(args, g_sm_count[dev], status, timeout_ns ? timeout_ns : 2000000000ull,
+                                            reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? VDC_OK : fail_cuda(e, "tree_attention launch");
+}
+
 int vdc_wide_tiles(int rows, int M, int K, int wfmt, int sms, int whole, int* out) {
   if (!out || rows < 128 || rows > VDC_WIDE_ROWS || rows % 128 || M < 16 || K < 64 || wfmt < 0 || wfmt > 2 || sms < 1)
     return fail_arg("wide tile: bad shape");
@@ -330,6 +395,12 @@ int vdc_read_status(uint64_t stream, vdc_status* status, int clear) {
       snprintf(buf, sizeof buf, "row %d: %s (%d)", h.pc, h.opcode == VDC_STAGE_EMBED || h.opcode == VDC_STAGE_WIDE_EMBED ||
                (h.opcode == VDC_STEP_KIND && h.role == 0) ? "token id outside the vocabulary"
                : "no number among its logits, no next token", h.aux);
+    else if (h.code == VDC_ERR_RANGE)
+      snprintf(buf, sizeof buf, "%s: %s %d: its %s (%d) is outside what the call was given",
+               h.opcode == VDC_ROPE_APPEND_KIND ? "rope_append" : h.opcode == VDC_READ_CACHE_KIND ? "read_cache"
+               : h.opcode == VDC_ADJUST_LOGITS_KIND ? "adjust_logits" : "tree_attention",
+               h.opcode == VDC_ADJUST_LOGITS_KIND ? "row" : "sequence", h.pc,
+               h.role == 0 ? "length" : h.role == 1 ? "page" : h.role == 2 ? "position" : "request", h.aux);
     else
       snprintf(buf, sizeof buf, "megakernel gave up: code=%d sm=%d role=%d pc=%d opcode=0x%x bar=%d aux=%d", h.code, h.sm,
                h.role, h.pc, h.opcode, h.bar, h.aux);
@@ -693,6 +764,12 @@ int vdc_launch_static(int num_sms, int insts_per_sm, const void* compute_insts, 
     if (h.code == VDC_ERR_TOKEN)
       snprintf(buf, sizeof buf, "row %d: %s (%d)", h.pc, h.opcode == VDC_STAGE_EMBED ? "token id outside the vocabulary"
                : "no number among its logits, no next token", h.aux);
+    else if (h.code == VDC_ERR_RANGE)
+      snprintf(buf, sizeof buf, "%s: %s %d: its %s (%d) is outside what the call was given",
+               h.opcode == VDC_ROPE_APPEND_KIND ? "rope_append" : h.opcode == VDC_READ_CACHE_KIND ? "read_cache"
+               : h.opcode == VDC_ADJUST_LOGITS_KIND ? "adjust_logits" : "tree_attention",
+               h.opcode == VDC_ADJUST_LOGITS_KIND ? "row" : "sequence", h.pc,
+               h.role == 0 ? "length" : h.role == 1 ? "page" : h.role == 2 ? "position" : "request", h.aux);
     else
       snprintf(buf, sizeof buf, "megakernel gave up: code=%d sm=%d role=%d pc=%d opcode=0x%x bar=%d aux=%d", h.code, h.sm,
                h.role, h.pc, h.opcode, h.bar, h.aux);

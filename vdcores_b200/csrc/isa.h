@@ -61,6 +61,10 @@
 #define VDC_STAGE_WIDE_NORM 12
 #define VDC_STAGE_WIDE_TAIL 13
 #define VDC_STEP_KIND 14          // what a step kernel's errors carry in the status block's opcode
+#define VDC_ROPE_APPEND_KIND 15   // the same for the operators of drafted tokens
+#define VDC_READ_CACHE_KIND 16
+#define VDC_TREE_ATTENTION_KIND 17
+#define VDC_ADJUST_LOGITS_KIND 18
 #define VDC_WIDE_ROWS 2048       // most rows of one pass
 #define VDC_WIDE_POS 0           // words of the block those stages read: first position, rows; page table at VDC_ST_PAGETABLE
 #define VDC_WIDE_N 1
@@ -312,6 +316,7 @@
 #define VDC_ERR_CUDA 3
 #define VDC_ERR_ARG 4
 #define VDC_ERR_TOKEN 5   // a row without a next token (no number among its logits), or a token id outside the vocabulary
+#define VDC_ERR_RANGE 6   // a length, page, position or request in device memory outside what the call was given
 
 typedef struct vdc_status {
   int32_t abort;    // non-zero once any wait gave up (every other wait then returns) or a token was refused

@@ -65,8 +65,8 @@ ST_POS, ST_NPAGES, ST_TOKEN, ST_STEP = _defs["ST_POS"], _defs["ST_NPAGES"], _def
 ST_NEWROW, ST_NKVH, ST_MAXPAGES, ST_ERR = _defs["ST_NEWROW"], _defs["ST_NKVH"], _defs["ST_MAXPAGES"], _defs["ST_ERR"]
 ST_PAGETABLE = _defs["ST_PAGETABLE"]
 
-OK, ERR_TIMEOUT, ERR_BAD_OPCODE, ERR_CUDA, ERR_ARG = (_defs[k] for k in
-                                                       ("OK", "ERR_TIMEOUT", "ERR_BAD_OPCODE", "ERR_CUDA", "ERR_ARG"))
+OK, ERR_TIMEOUT, ERR_BAD_OPCODE, ERR_CUDA, ERR_ARG, ERR_RANGE = (
+    _defs[k] for k in ("OK", "ERR_TIMEOUT", "ERR_BAD_OPCODE", "ERR_CUDA", "ERR_ARG", "ERR_RANGE"))
 
 _flagval = {"VDC_F_ALLOCATE": F_ALLOCATE, "VDC_F_WRITEBACK": F_WRITEBACK, "0": 0}
 OPCODES = {}

@@ -1,0 +1,392 @@
+"""Operators for serving with drafted tokens, over paged caches like the engines'.
+
+    cache = KVCache.empty(n_pages, n_kv_heads, "e4m3")            # or KVCache(eng.kpool[l], eng.vpool[l])
+    mask, depth = tree_mask(parents)                              # parents [B, T], -1: a root
+    q = rope_append(q, k, v, cache, pages, lengths, table, positions=lengths[:, None] + depth)
+    o = tree_attention(q, cache, pages, lengths, mask=mask)
+    logits, tokens = adjust_logits(logits, history=..., repetition=..., allowed=...)
+    k, v = read_cache(cache, pages, lengths, n)
+
+Every call runs one or two kernels on the current stream and returns without synchronising; tensors that it allocates belong to
+that stream, and nothing is kept between calls.  Wrong arguments raise ValueError before anything runs.  What only the device can
+see (a length, page, position or request that does not fit) leaves the row concerned out, and `check()` raises it.
+A pool holds the pages of several sequences; `pages` [B, max_pages] int32 names each sequence's, `lengths` [B] int32 the rows it
+holds.  Heads have 128 values and a page 64 rows, as everywhere in the framework.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import isa, runtime
+
+BF16, F8 = torch.bfloat16, torch.float8_e4m3fn
+D, PAGE = isa.HEAD_DIM, isa.KV_PAGE
+_FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _on_gpu(name, t, dtype, dims):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.dim() == dims):
+        raise ValueError(f"{name} must be a {dims}-dimensional {dtype} tensor on the GPU")
+
+
+def _stream(t):
+    dev = t.device.index
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _same_device(first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+def _vector(name, t, n, dtype=torch.int32):
+    """Address of [n] values, one behind the other."""
+    if t is None:
+        return 0
+    _on_gpu(name, t, dtype, 1)
+    _need(t.shape[0] == n and (n <= 1 or t.stride(0) == 1), f"{name} must have {n} values, one behind the other")
+    return t.data_ptr()
+
+
+def _heads(name, x, n_kv):
+    """(B, T, query heads to a KV head, strides of the four leading dimensions as [B, T, n_kv, group]) of rows [B, T, heads, 128]
+    or [B, T, n_kv, group, 128]."""
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == BF16 and x.dim() in (4, 5) and x.shape[-1] == D):
+        raise ValueError(f"{name} must be [B, T, heads, {D}] or [B, T, n_kv, group, {D}] bf16 on the GPU")
+    size, st = x.shape, x.stride()
+    _need(st[-1] == 1, f"{name}: the values of a head must lie one behind the other")
+    if len(size) == 5:
+        _need(size[2] == n_kv, f"{name} has {size[2]} KV heads, the cache {n_kv}")
+        g, st = size[3], st[:4]
+    else:
+        _need(size[2] % n_kv == 0 and size[2] > 0, f"{name}: {size[2]} heads are no multiple of the cache's {n_kv}")
+        g = size[2] // n_kv
+        st = (st[0], st[1], st[2] * g, st[2])
+    return size[0], size[1], g, st
+
+
+class KVCache:
+    """The pages of one layer: k and v [pages, n_kv_heads, 64, 128], bf16 ("bf16") or e4m3 codes ("e4m3", as float8_e4m3fn or
+    uint8) with fp32 scales [pages, n_kv_heads, 64]; a row's 16-byte pieces lie at index (piece XOR (row mod 8)).  The tensors stay
+    the caller's; pages and heads may have any strides that are multiples of 16 bytes, a page's rows lie one behind the other."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        for name, t in (("k", k), ("v", v)):
+            _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 and t.shape[2:] == (PAGE, D),
+                  f"{name} must be [pages, heads, {PAGE}, {D}] on the GPU")
+            _need(t.dtype in (BF16, F8, torch.uint8), f"{name} must be bf16, or e4m3 codes as float8_e4m3fn or uint8")
+            _need(t.stride(3) == 1 and t.stride(2) == D, f"{name}: the rows of a page must lie one behind the other")
+        _need(k.shape == v.shape and k.dtype == v.dtype, "k and v differ in shape or type")
+        self.kind = "bf16" if k.dtype == BF16 else "e4m3"
+        scales = (k_scale, v_scale)
+        if self.kind == "bf16":
+            _need(scales == (None, None), "a bf16 cache has no scales")
+            strides = (0, 0, 0, 0)
+        else:
+            for name, t in zip(("k_scale", "v_scale"), scales):
+                _on_gpu(name, t, torch.float32, 3)
+                _need(t.shape == k.shape[:3] and t.stride(2) == 1, f"{name} must be [pages, heads, {PAGE}], a page's scales one behind the other")
+            strides = tuple(4 * t.stride(i) for t in scales for i in (0, 1))
+        _same_device(k, v, k_scale, v_scale)
+        self.n_pages, self.n_kv_heads = k.shape[:2]
+        size = k.element_size()
+        ptrs = [t.data_ptr() if t is not None else 0 for t in (k, v, k_scale, v_scale)]
+        self._c = runtime.Cache(*ptrs, *(size * t.stride(i) for t in (k, v) for i in (0, 1)), *strides, int(self.kind == "e4m3"),
+                                self.n_kv_heads, self.n_pages)
+
+    @classmethod
+    def empty(cls, n_pages: int, n_kv_heads: int, kind: str = "bf16", device="cuda"):
+        """A cache of zeroed pages."""
+        _need(kind in ("bf16", "e4m3"), f"unknown kind {kind!r}")
+        shape = (n_pages, n_kv_heads, PAGE, D)
+        if kind == "bf16":
+            return cls(*(torch.zeros(shape, dtype=BF16, device=device) for _ in range(2)))
+        return cls(*(torch.zeros(shape, dtype=torch.uint8, device=device).view(F8) for _ in range(2)),
+                   *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _tables(cache, pages, lengths, counts=None):
+    """(B, max_pages, row stride and address of pages, addresses of lengths and counts)."""
+    _need(isinstance(cache, KVCache), "cache must be a KVCache")
+    _on_gpu("pages", pages, torch.int32, 2)
+    B, n = pages.shape
+    _need(n >= 1 and (n == 1 or pages.stride(1) == 1), "pages: a sequence's must lie one behind the other, at least one")
+    _same_device(cache.k, pages, lengths, counts)
+    _need(lengths is not None, "lengths are needed")
+    return B, n, pages.stride(0) if B > 1 else 0, pages.data_ptr(), _vector("lengths", lengths, B), _vector("counts", counts, B)
+
+
+def check():
+    """Waits for the current stream and raises what the operators (or an engine) found wrong on the device."""
+    runtime.init()
+    runtime.read_status(torch.cuda.current_stream().cuda_stream)
+
+
+def rope_table(n_positions: int, dim: int = D, theta: float = 10000.0, scaling: Optional[dict] = None, device="cuda") -> torch.Tensor:
+    """fp32 [n_positions, dim] for rope_append: cosines of dim / 2 angles, then sines.  `scaling` stretches for long contexts:
+      {"type": "linear", "factor": f}                     every frequency / f
+      {"type": "ntk", "factor": f}                        theta * f^(dim / (dim - 2)): the lowest frequency / f, the highest as it is
+      {"type": "llama3", "factor": f, "low_freq_factor": a, "high_freq_factor": b, "original_max_position": n}
+                                                          frequencies with under a turns in n positions / f, over b as they are,
+                                                          between them a blend that is linear in the turns
+      {"type": "yarn", "factor": f, "original_max_position": n, "beta_fast": 32, "beta_slow": 1}
+                                                          the same with a blend that is linear in the dimension between those with
+                                                          beta_slow and beta_fast turns, cosines and sines times 0.1 ln f + 1"""
+    _need(dim >= 0 and dim % 16 == 0 and dim <= D, f"the rotated part must be a multiple of 16 up to {D}")
+    _need(n_positions >= 1 and theta > 0, "positions and theta must be positive")
+    i = torch.arange(0, dim, 2, dtype=torch.float64)
+    scaling, mag = dict(scaling or {"type": "none"}), 1.0
+    kind, f = scaling.pop("type", None), float(scaling.pop("factor", 1.0))
+    known = {"none": (), "linear": (), "ntk": (), "llama3": ("low_freq_factor", "high_freq_factor", "original_max_position"),
+             "yarn": ("original_max_position", "beta_fast", "beta_slow")}
+    _need(kind in known, f"unknown scaling {kind!r}")
+    _need(set(scaling) <= set(known[kind]) and f >= 1.0, f"scaling {kind!r} takes factor >= 1 and {known[kind]}")
+    if kind == "ntk" and dim > 2:
+        theta = theta * f ** (dim / (dim - 2))
+    inv = theta ** (-i / max(1, dim))
+    if kind == "linear":
+        inv = inv / f
+    elif kind == "llama3":
+        lo, hi, n = (float(scaling[k]) for k in known[kind])
+        keep = ((n * inv / (2 * math.pi) - lo) / (hi - lo)).clamp(0, 1)
+        inv = inv * keep + inv / f * (1 - keep)
+    elif kind == "yarn":
+        n, fast, slow = float(scaling["original_max_position"]), float(scaling.get("beta_fast", 32)), float(scaling.get("beta_slow", 1))
+        at = lambda turns: dim * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(theta))    # noqa: E731
+        lo, hi = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), dim - 1)
+        keep = 1 - ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        inv = inv * keep + inv / f * (1 - keep)
+        mag = 0.1 * math.log(f) + 1.0
+    a = torch.arange(n_positions, dtype=torch.float64)[:, None] * inv
+    return (mag * torch.cat((a.cos(), a.sin()), 1)).float().to(device)
+
+
+def pack_mask(seen: torch.Tensor) -> torch.Tensor:
+    """[..., T, T] bool (token i attends to drafted token j) -> int64 [..., T, words] for tree_attention."""
+    T = seen.shape[-1]
+    words = max(1, -(-T // 64))
+    bits = torch.zeros(*seen.shape[:-1], words * 64, dtype=torch.int64, device=seen.device)
+    bits[..., :T] = seen.to(torch.int64)
+    return (bits.view(*seen.shape[:-1], words, 64) << torch.arange(64, device=seen.device)).sum(-1)
+
+
+def tree_mask(parents, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
+    """Mask (for tree_attention) and depths (int32) of trees: parents [T] or [B, T], each token's parent in front of it, -1 for a
+    root.  A token attends to its ancestors and itself."""
+    p = torch.as_tensor(parents).cpu().long()
+    _need(p.dim() in (1, 2) and p.shape[-1] >= 1, "parents must be [T] or [B, T]")
+    T = p.shape[-1]
+    _need(bool(((p >= -1) & (p < torch.arange(T))).all()), "a parent must be in front of its token, or -1")
+    q = p.view(-1, T)
+    seen, depth = torch.zeros(q.shape[0], T, T, dtype=torch.bool), torch.zeros(q.shape, dtype=torch.int32)
+    rows = torch.arange(q.shape[0])
+    for i in range(T):
+        par = q[:, i].clamp(min=0)
+        has = q[:, i] >= 0
+        seen[:, i] = seen[rows, par] & has[:, None]
+        seen[:, i, i] = True
+        depth[:, i] = torch.where(has, depth[rows, par] + 1, 0)
+    return pack_mask(seen).view(*p.shape, -1).to(device), depth.view(p.shape).to(device)
+
+
+def rope_append(q, k, v, cache: KVCache, pages, lengths, table=None, positions=None, counts=None, layout: str = "half", qk_norm=None,
+                eps: float = 1e-6, out=None) -> torch.Tensor:
+    """Rotates q [B, T, heads, 128] (or [B, T, n_kv, group, 128]) and k [B, T, n_kv, 128], and appends k and v to the cache: token t
+    of sequence b becomes row lengths[b] + t.  Returns the rotated queries (`out`, which may be q; by default a new tensor).
+
+    table: fp32 [n, dim] of rope_table, or an engine's `rope`; the first dim of a head's 128 values turn (None: nothing does)
+    positions: int32 [B, T], the table's rows (default: the tokens' rows; a drafted tree's are lengths + depth)
+    counts: int32 [B], the tokens of a sequence; those behind them append nothing and give zeros
+    layout: "half" pairs value i with i + dim / 2, "interleaved" 2i with 2i + 1
+    qk_norm: bf16 weights (q, k) of 128 values each (a pair, or one tensor of 256): RMS norm of every head in front of the rotation
+
+    bf16 rows, fp32 arithmetic, one rounding at the end.  An e4m3 cache gets e4m3(x / s) with s = the row's largest magnitude / 448;
+    a row with an infinity or NaN gets a scale that is one, and reads back as NaN."""
+    n_kv = cache.n_kv_heads
+    B, n_pages, pages_b, p_pages, p_lengths, p_counts = _tables(cache, pages, lengths, counts)
+    qB, T, group, qs = _heads("q", q, n_kv)
+    _need(qB == B, f"q has {qB} sequences, pages {B}")
+    kv = []
+    for name, x in (("k", k), ("v", v)):
+        _on_gpu(name, x, BF16, 4)
+        _need(x.shape == (B, T, n_kv, D) and x.stride(3) == 1, f"{name} must be [{B}, {T}, {n_kv}, {D}], a head's values one behind the other")
+        kv += x.stride()[:3]
+    if out is None:
+        out = torch.empty(q.shape, dtype=BF16, device=q.device)
+    else:
+        _need(isinstance(out, torch.Tensor) and out.shape == q.shape, "out must have the shape of q")
+    os = _heads("out", out, n_kv)[3]
+    rot = rows = p_table = p_pos = pos_b = pos_t = p_q = p_k = 0
+    if table is not None:
+        _on_gpu("table", table, torch.float32, 2)
+        rows, rot = table.shape
+        _need(table.is_contiguous(), "table must be contiguous")
+        p_table = table.data_ptr()
+    if positions is not None:
+        _on_gpu("positions", positions, torch.int32, 2)
+        _need(positions.shape == (B, T), f"positions must be [{B}, {T}]")
+        p_pos, (pos_b, pos_t) = positions.data_ptr(), positions.stride()
+    _need(layout in ("half", "interleaved"), f"unknown layout {layout!r}")
+    if qk_norm is not None:
+        if isinstance(qk_norm, torch.Tensor):
+            _need(qk_norm.dtype == BF16 and qk_norm.is_cuda and qk_norm.is_contiguous() and qk_norm.numel() == 2 * D,
+                  "qk_norm must be two bf16 vectors of 128 weights")
+            p_q = qk_norm.data_ptr()
+            p_k = p_q + 2 * D
+            _same_device(q, qk_norm)
+        else:
+            w_q, w_k = qk_norm
+            p_q, p_k = _vector("qk_norm[0]", w_q, D, BF16), _vector("qk_norm[1]", w_k, D, BF16)
+            _same_device(q, w_q, w_k)
+    _same_device(q, k, v, out, cache.k, table, positions)
+    if B == 0 or T == 0:
+        return out
+    runtime.rope_append(runtime.RopeAppend(cache._c, B, T, group, rot, layout == "interleaved", rows, n_pages, eps, *qs, *kv, *os,
+                                           pages_b, pos_b, pos_t, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p_pages,
+                                           p_lengths, p_counts, p_table, p_pos, p_q, p_k), _stream(q))
+    return out
+
+
+def read_cache(cache: KVCache, pages, lengths, n: int, start=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of rows start .. start + n - 1 (start: int32 [B], default 0) of every sequence as dense bf16 tensors
+    [B, n, n_kv, 128]; rows at or behind lengths[b] are zeros."""
+    B, n_pages, pages_b, p_pages, p_lengths, _ = _tables(cache, pages, lengths)
+    _need(n >= 0, "n must not be negative")
+    p_start = _vector("start", start, B)
+    _same_device(cache.k, start)
+    k, v = (torch.empty(B, n, cache.n_kv_heads, D, dtype=BF16, device=cache.k.device) for _ in range(2))
+    if B and n:
+        runtime.read_cache(runtime.ReadCache(cache._c, B, n, n_pages, 0, pages_b, p_pages, p_lengths, p_start, k.data_ptr(), v.data_ptr()),
+                           _stream(k))
+    return k, v
+
+
+def tree_attention(q, cache: KVCache, pages, lengths, mask=None, counts=None, scale: Optional[float] = None, out=None) -> torch.Tensor:
+    """Attention of T drafted tokens per sequence over its cache: q [B, T, heads, 128] (or [B, T, n_kv, group, 128]) as rope_append
+    returns it, their own rows at lengths[b] .. lengths[b] + T - 1 (appended before, `lengths` as they were then).  Token i attends to
+    all rows in front of lengths[b] and to the drafted tokens of its mask.
+
+    mask: int64 [B, T, words] (or [T, words] for all), from tree_mask or pack_mask; default a chain (every token attends to those in
+      front of it and itself), so that T = 1 is an ordinary decode step
+    counts: int32 [B], the drafted tokens of a sequence; rows behind them are neither attended to nor computed (zeros)
+    scale: default 1 / sqrt(128)
+    out: a tensor like q, not q itself; by default a new one
+
+    Scores, softmax and sums are fp32.  A token with nothing to attend to gets zeros."""
+    n_kv = cache.n_kv_heads
+    B, n_pages, pages_b, p_pages, p_lengths, p_counts = _tables(cache, pages, lengths, counts)
+    qB, T, group, qs = _heads("q", q, n_kv)
+    _need(qB == B, f"q has {qB} sequences, pages {B}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=BF16, device=q.device)
+    else:
+        _need(isinstance(out, torch.Tensor) and out.shape == q.shape, "out must have the shape of q")
+        _need(out.data_ptr() != q.data_ptr(), "out must not be q")
+    os = _heads("out", out, n_kv)[3]
+    words, p_mask, mask_b, mask_t = -(-T // 64), 0, 0, 0
+    if mask is not None:
+        _need(isinstance(mask, torch.Tensor) and mask.is_cuda and mask.dtype == torch.int64 and mask.dim() in (2, 3),
+              "mask must be [B, T, words] or [T, words] int64 on the GPU")
+        size, st = mask.shape, mask.stride()
+        _need(size[-2:] == (T, words) and (len(size) == 2 or size[0] == B), f"mask must be [{B}, {T}, {words}] or [{T}, {words}]")
+        _need(words == 1 or st[-1] == 1, "mask: a token's words must lie one behind the other")
+        p_mask, mask_t, mask_b = mask.data_ptr(), st[-2], st[0] if len(size) == 3 else 0
+    _same_device(q, cache.k, out, mask)
+    if B == 0 or T == 0:
+        return out
+    a = runtime.TreeAttention(cache._c, B, T, group, n_pages, words, D ** -0.5 if scale is None else scale, *qs, *os, pages_b, mask_b,
+                              mask_t, q.data_ptr(), out.data_ptr(), p_pages, p_lengths, p_counts, p_mask, 0)
+    nbytes = runtime.tree_attention_workspace(a)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    if nbytes:
+        a.work = work.data_ptr()
+    runtime.tree_attention(a, _stream(q))
+    return out
+
+
+def adjust_logits(logits, requests=None, history=None, prompt_lens=None, history_lens=None, path=None, repetition=None, frequency=None,
+                  presence=None, bias_ids=None, bias=None, allowed=None, out=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Penalties for repeated tokens, biases and grammar masks on logits [rows, vocab] (or [vocab]; fp32, bf16 or f16).  Returns the
+    adjusted logits (`out`, which may be the logits; by default a new tensor of their type; fp32 is always possible) and tokens int32
+    [rows]: the lowest id of each row's largest adjusted logit, -1 where none is left.
+
+    requests: int32 [rows], the request of each row (default: row r is request r); per request
+      history: int32 [n, L] ids, the first prompt_lens[n] of them the prompt (default none), those up to history_lens[n] (default all)
+        generated; repetition, frequency, presence: fp32 [n]
+      bias_ids: int32 [n, m], bias: fp32 [n, m], added to those ids
+    path: int32 [rows, p], ids drafted in front of the row's token, counted as generated
+    allowed: int32 [rows, (vocab + 31) / 32], bit id % 32 of word id / 32 set where an id may come next
+    Ids outside the vocabulary (-1, say) are ignored.
+
+    An id of history or path: l = l / repetition if l > 0 else l * repetition; generated c times: l -= frequency * c + presence; then
+    the bias, then -inf where it is not allowed.  fp32 arithmetic, rounded once; the tokens are chosen before that rounding."""
+    one = isinstance(logits, torch.Tensor) and logits.dim() == 1
+    if one:
+        logits, out = logits[None], out[None] if out is not None else None
+    _need(isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dtype in _FLOATS and logits.dim() == 2,
+          "logits must be [rows, vocab] fp32, bf16 or f16 on the GPU")
+    rows, vocab = logits.shape
+    _need(vocab >= 1 and (vocab == 1 or logits.stride(1) == 1), "a row's logits must lie one behind the other")
+    if out is None:
+        out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+    else:
+        _need(isinstance(out, torch.Tensor) and out.shape == logits.shape and out.dtype in (logits.dtype, torch.float32) and
+              (vocab == 1 or out.stride(1) == 1), "out must be like the logits, or fp32")
+    n = None
+
+    def table(name, t, dtype, dims, per_row=False):
+        """Address and row stride of a table of requests (or rows)."""
+        nonlocal n
+        if t is None:
+            return 0, 0
+        _on_gpu(name, t, dtype, dims)
+        if dims == 2:
+            _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: a row's values must lie one behind the other")
+        else:
+            _need(t.shape[0] <= 1 or t.stride(0) == 1, f"{name}: values must lie one behind the other")
+        if not per_row and n is None:
+            n = t.shape[0]
+        _need(t.shape[0] == (rows if per_row else n), f"{name} has {t.shape[0]} rows, not {rows if per_row else n}")
+        return t.data_ptr(), t.stride(0) if dims == 2 else 0
+
+    i32, f32 = torch.int32, torch.float32
+    p_hist, hist_s = table("history", history, i32, 2)
+    p_prompt, _ = table("prompt_lens", prompt_lens, i32, 1)
+    p_lens, _ = table("history_lens", history_lens, i32, 1)
+    p_rep, _ = table("repetition", repetition, f32, 1)
+    p_freq, _ = table("frequency", frequency, f32, 1)
+    p_pres, _ = table("presence", presence, f32, 1)
+    p_ids, bias_s = table("bias_ids", bias_ids, i32, 2)
+    p_bias, bias_s2 = table("bias", bias, f32, 2)
+    p_path, path_s = table("path", path, i32, 2, True)
+    p_allowed, allowed_s = table("allowed", allowed, i32, 2, True)
+    p_req, _ = table("requests", requests, i32, 1, True)
+    _need((bias_ids is None) == (bias is None), "bias and bias_ids go together")
+    if bias is not None:
+        _need(bias.shape == bias_ids.shape and (n == 1 or bias_s == bias_s2), "bias and bias_ids must have one shape and row stride")
+    _need(history is not None or (prompt_lens is None and history_lens is None), "lengths without a history")
+    if allowed is not None:
+        _need(allowed.shape[1] == (vocab + 31) // 32, f"allowed must have {(vocab + 31) // 32} words a row")
+    n = rows if n is None else n
+    _need(requests is not None or n == rows, f"{n} requests for {rows} rows: requests must say which row is whose")
+    _same_device(logits, out, history, prompt_lens, history_lens, path, repetition, frequency, presence, bias_ids, bias, allowed, requests)
+    tokens = torch.empty(rows, dtype=i32, device=logits.device)
+    if rows:
+        runtime.adjust_logits(runtime.AdjustLogits(
+            rows, vocab, _FLOATS[logits.dtype], _FLOATS[out.dtype], n, history.shape[1] if history is not None else 0,
+            path.shape[1] if path is not None else 0, bias.shape[1] if bias is not None else 0, logits.stride(0), out.stride(0), hist_s,
+            path_s, bias_s, allowed_s, logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), p_req, p_hist, p_prompt, p_lens, p_path, p_rep,
+            p_freq, p_pres, p_ids, p_bias, p_allowed), _stream(logits))
+    return (out[0] if one else out), tokens

@@ -51,6 +51,30 @@ class Step(ctypes.Structure):
                                                   "logits", "hidden_out", "taps", "route", "work")])
 
 
+def _struct(name, doc, *groups):
+    return type(name, (ctypes.Structure,), {"__doc__": doc, "_fields_": [(n, t) for t, names in groups for n in names.split()]})
+
+
+Cache = _struct("Cache", "A layer's paged cache (vdc_cache in include/vdcores.h, which documents the fields).",
+                (ctypes.c_uint64, "k v k_scale v_scale"),
+                (ctypes.c_int64, "k_page k_head v_page v_head ks_page ks_head vs_page vs_head"),
+                (ctypes.c_int32, "kind n_kv n_pages reserved"))
+RopeAppend = _struct("RopeAppend", "Arguments of vdc_rope_append.", (Cache, "cache"),
+                     (ctypes.c_int32, "B T group rot interleaved table_rows max_pages"), (ctypes.c_float, "eps"),
+                     (ctypes.c_int64, "q_b q_t q_kv q_g k_b k_t k_kv v_b v_t v_kv o_b o_t o_kv o_g pages_b pos_b pos_t"),
+                     (ctypes.c_uint64, "q k v out pages lengths counts table positions q_norm k_norm"))
+ReadCache = _struct("ReadCache", "Arguments of vdc_read_cache.", (Cache, "cache"), (ctypes.c_int32, "B n max_pages reserved"),
+                    (ctypes.c_int64, "pages_b"), (ctypes.c_uint64, "pages lengths start k_out v_out"))
+TreeAttention = _struct("TreeAttention", "Arguments of vdc_tree_attention.", (Cache, "cache"),
+                        (ctypes.c_int32, "B T group max_pages words"), (ctypes.c_float, "scale"),
+                        (ctypes.c_int64, "q_b q_t q_kv q_g o_b o_t o_kv o_g pages_b mask_b mask_t"),
+                        (ctypes.c_uint64, "q out pages lengths counts mask work"))
+AdjustLogits = _struct("AdjustLogits", "Arguments of vdc_adjust_logits.",
+                       (ctypes.c_int32, "rows vocab type out_type n L path_n n_bias"),
+                       (ctypes.c_int64, "logits_s out_s history_s path_s bias_s allowed_s"),
+                       (ctypes.c_uint64, "logits out tokens requests history prompt_lens history_lens path repetition frequency "
+                                         "presence bias_ids bias allowed"))
+
 _u64, _i32, _vp = ctypes.c_uint64, ctypes.c_int, ctypes.c_void_p
 _lib.vdc_version.restype = _i32
 _lib.vdc_init.restype = _i32
@@ -64,6 +88,11 @@ _lib.vdc_launch_stages_limited.argtypes = [ctypes.POINTER(Stage), _i32, _i32, _u
 _lib.vdc_count_stage_launches.argtypes = [ctypes.POINTER(Stage), _i32, _i32, ctypes.POINTER(_i32), ctypes.POINTER(_i32)]
 _lib.vdc_step_workspace.argtypes = [ctypes.POINTER(Step), ctypes.POINTER(_u64)]
 _lib.vdc_launch_step.argtypes = [ctypes.POINTER(Step), _u64, _u64]
+_lib.vdc_rope_append.argtypes = [ctypes.POINTER(RopeAppend), _u64]
+_lib.vdc_read_cache.argtypes = [ctypes.POINTER(ReadCache), _u64]
+_lib.vdc_tree_attention_workspace.argtypes = [ctypes.POINTER(TreeAttention), ctypes.POINTER(_u64)]
+_lib.vdc_tree_attention.argtypes = [ctypes.POINTER(TreeAttention), _u64, _u64]
+_lib.vdc_adjust_logits.argtypes = [ctypes.POINTER(AdjustLogits), _u64]
 _lib.vdc_wide_tiles.argtypes = [_i32] * 6 + [ctypes.POINTER(_i32)]
 _lib.vdc_read_status.argtypes = [_u64, ctypes.POINTER(Status), _i32]
 _lib.vdc_build_tma_desc.argtypes = [_vp, _vp, _i32, _i32, ctypes.POINTER(_u64), ctypes.POINTER(_u64),
@@ -96,6 +125,7 @@ EXPORTED_SYMBOLS = [
     "vdc_version", "vdc_init", "vdc_set_smem_size", "vdc_launch", "vdc_launch_async", "vdc_launch_async_full",
     "vdc_launch_static", "vdc_launch_stages", "vdc_launch_stages_limited",
     "vdc_count_stage_launches", "vdc_wide_tiles", "vdc_step_workspace", "vdc_launch_step",
+    "vdc_rope_append", "vdc_read_cache", "vdc_tree_attention_workspace", "vdc_tree_attention", "vdc_adjust_logits",
     "vdc_read_status",
     "vdc_build_tma_desc", "vdc_set_cache_policy", "vdc_enable_peer_access", "vdc_ipc_open", "vdc_ipc_close", "vdc_peer_alloc", "vdc_peer_free", "vdc_ipc_export", "vdc_opcode_count", "vdc_opcode_name", "vdc_opcode_value",
     "vdc_opcode_is_compute", "vdc_config", "vdc_family_specs", "vdc_last_error", "vdc_validate_streams",
@@ -228,6 +258,37 @@ def launch_step(step, stream=0, timeout_ns=0):
     """Enqueues one token of a model at batch 1; no synchronisation."""
     init()
     _check(_lib.vdc_launch_step(ctypes.byref(step), int(stream), int(timeout_ns)))
+
+
+def rope_append(args, stream=0):
+    """Enqueues one RopeAppend; no synchronisation."""
+    init()
+    _check(_lib.vdc_rope_append(ctypes.byref(args), int(stream)))
+
+
+def read_cache(args, stream=0):
+    """Enqueues one ReadCache; no synchronisation."""
+    init()
+    _check(_lib.vdc_read_cache(ctypes.byref(args), int(stream)))
+
+
+def tree_attention_workspace(args):
+    """Bytes of workspace that a TreeAttention needs; pointers are not looked at, needs no GPU."""
+    n = _u64()
+    _check(_lib.vdc_tree_attention_workspace(ctypes.byref(args), ctypes.byref(n)))
+    return int(n.value)
+
+
+def tree_attention(args, stream=0, timeout_ns=0):
+    """Enqueues one TreeAttention; no synchronisation."""
+    init()
+    _check(_lib.vdc_tree_attention(ctypes.byref(args), int(stream), int(timeout_ns)))
+
+
+def adjust_logits(args, stream=0):
+    """Enqueues one AdjustLogits; no synchronisation."""
+    init()
+    _check(_lib.vdc_adjust_logits(ctypes.byref(args), int(stream)))
 
 
 def wide_tiles(rows, M, K, wfmt, sms, whole=False):
