@@ -1,72 +1,800 @@
 // Attention of drafted tokens over a paged cache.  Shapes, masks and errors: include/vdcores.h.
 //
-// A warp per query row: running maximum and sum of the softmax over the sequence's rows, in fp32, four values of a head to a lane.
+// The mathematics: o_i = sum_j 2^(s_ij - m_i) v_j / sum_j 2^(s_ij - m_i) with s = q k^T scale log2(e), one pass over the keys with a
+// running reference m_i of each row.  m_i follows the row's maximum lazily: sums are only rescaled when a score exceeds it by
+// kSlack powers of two, which the formats of the weights and sums have room for.
+//
+// The work: a unit is 128 query rows (tokens x query heads) of one KV head of one sequence, the units' pages laid end to end are
+// shared out evenly to one CTA per SM, so that sequences of any mix of lengths load the SMs alike.  A CTA's part of a unit is a
+// piece; pieces that are not whole units leave sums and statistics in the workspace, and a second kernel joins them.
+//
+// A piece: the query rows lie in tensor memory, row i on lane i, as the first operand of S = Q K^T (64 keys of a page at a time,
+// K from shared memory as the pool's rows lie there: their piece order is the tensor cores' 128-byte swizzle).  Two groups of four
+// warps take the pages in turn: each reads its S, makes the weights P and puts them into tensor memory, first operand of
+// O += P V.  Each group sums its own O; the two meet at the end of the piece.
+//
+// Few rows (decoding, small trees) would leave most lanes idle: they are repeated over the lanes, each copy takes a part of every
+// page's keys (the other columns of its P stay zero), and the copies' sums meet like the groups'.
+//
+// e4m3 caches: a key's scale multiplies its scores.  A value's scale vs goes into its weight, P' = 2^(s + log2 vs - m), and the
+// sum of weights is that of P' / vs: one exponential, and no product per value.  Q becomes two e4m3 parts with a common power of two
+// per row, which are exact for bf16 values down to 2^-10 of the row's largest (below, 2^-18 of it), so K is used as it lies in
+// memory, in two passes of the 8-bit tensor cores.  V is widened to f16 (exact) by four more warps; P is f16 as well.
 #include "mk_stage.cuh"
 
 namespace vdc {
 namespace {
 
-constexpr int D = VDC_HEAD_DIM, PAGE = VDC_KV_PAGE, kWarps = 8;
+constexpr int D = VDC_HEAD_DIM, PAGE = VDC_KV_PAGE, kRows = 128;
+constexpr int kMathWarps = 8;                   // two groups of four
+constexpr float kLog2e = 1.4426950408889634f;
 
 template <bool kF8>
-__device__ __forceinline__ float4 stored4(uint64_t page, uint64_t scale, int row, int lane) {
-  if constexpr (kF8) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(page + row * D + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4);
-    const float s = reinterpret_cast<const float*>(scale)[row];
-    const float2 lo = e4m3x2_to_float2(w & 0xFFFFu), hi = e4m3x2_to_float2(w >> 16);
-    return make_float4(lo.x * s, lo.y * s, hi.x * s, hi.y * s);
-  } else {
-    const uint2 w = *reinterpret_cast<const uint2*>(page + row * 2 * D + (((lane >> 1) ^ (row & 7)) << 4) + (lane & 1) * 8);
-    return make_float4(bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y));
+struct Cfg {
+  static constexpr int kStages = kF8 ? 6 : 4;
+  static constexpr int kPageBytes = PAGE * D * (kF8 ? 1 : 2);
+  static constexpr int kStageBytes = 2 * kPageBytes;
+  static constexpr int kTx = kStageBytes + (kF8 ? 2 * PAGE * 4 : 0);
+  static constexpr int kWideWarps = kF8 ? 4 : 0;
+  static constexpr int kLoadWarp = kMathWarps + kWideWarps, kMmaWarp = kLoadWarp + 1;
+  static constexpr int kThreads = (kMmaWarp + 1) * 32;
+  static constexpr float kSlack = kF8 ? 4.f : 8.f;      // powers of two by which a score may exceed its row's reference
+  static constexpr float kLift = kF8 ? 11.f : 0.f;      // f16 weights are kept that much larger: 2^15 at most, 2^-25 of the largest with all bits
+};
+constexpr int kWideBufs = 4, kWideBytes = PAGE * D * 2;
+constexpr int kScratchRow = 36;                         // floats of a row's 32 sums on their way between warps
+constexpr int kScratch = kMathWarps * 32 * kScratchRow * 4;
+
+// columns of tensor memory
+constexpr int kColO = 0, kColS = 256, kColP = 384, kColQ = 448, kCols = 512;
+
+struct TreeShared {
+  uint64_t full[8], empty[8], q_full, s_full[2], s_empty[2], p_full[2], o_done[2], tail[2];
+  uint64_t v_full[kWideBufs], v_empty[kWideBufs], par_full[kWideBufs];
+  uint32_t tmem;
+  volatile int fail;
+  int first_b;
+  long long begin, end, first_base;
+  uint32_t poison[2][4][2];
+  float q_mul[kRows];
+  float2 stats[kMathWarps][32];       // of the rows on a warp's lanes: reference, sum of weights
+  float2 row[kRows];                  // of a row over all its copies: the same
+  alignas(16) float4 par[kWideBufs][PAGE];     // of a key of an e4m3 page: its scale, log2 of the value's, 1 / the value's
+  alignas(16) float scales[8][2][PAGE];
+};
+
+// Pages of sequence b (0 where there is nothing to compute, or something is wrong).
+__device__ __forceinline__ int seq_pages(const vdc_tree_attention_args& a, int b, int& ctx, int& live, bool* wrong = nullptr) {
+  ctx = __ldg(reinterpret_cast<const int*>(a.lengths) + b);
+  live = a.counts ? max(0, min(a.T, __ldg(reinterpret_cast<const int*>(a.counts) + b))) : a.T;
+  const int64_t keys = (int64_t)ctx + live;
+  const bool bad = ctx < 0 || keys > (int64_t)a.max_pages * PAGE;
+  if (wrong) *wrong = bad;
+  return bad || live == 0 ? 0 : (int)((keys + PAGE - 1) / PAGE);
+}
+
+__device__ __forceinline__ int tiles_of(const vdc_tree_attention_args& a) { return (a.T * a.group + kRows - 1) / kRows; }
+
+// A warp adds up the pages of all sequences.
+__device__ __forceinline__ long long all_pages(const vdc_tree_attention_args& a, int lane) {
+  long long n = 0;
+  int ctx, live;
+  for (int b = lane; b < a.B; b += 32) n += seq_pages(a, b, ctx, live);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
+  return n;
+}
+
+struct Piece {
+  int b, head, tile, p0, p1, np, ctx, live;
+  __device__ __forceinline__ int total() const { return ctx + live; }
+  __device__ __forceinline__ bool whole() const { return p0 == 0 && p1 == np; }
+};
+
+// The pieces of a CTA, in order; every role walks them by itself.
+struct Walk {
+  const vdc_tree_attention_args& a;
+  long long x, end, base;     // place among all units' pages, its end, where sequence b begins
+  int b;
+  __device__ __forceinline__ Walk(const vdc_tree_attention_args& a_, const TreeShared& sh)
+      : a(a_), x(sh.begin), end(sh.end), base(sh.first_base), b(sh.first_b) {}
+  __device__ __forceinline__ bool next(Piece& p) {
+    if (x >= end) return false;
+    const int tiles = tiles_of(a), units = a.cache.n_kv * tiles;
+    for (;; ++b) {
+      if (b >= a.B) return false;
+      p.np = seq_pages(a, b, p.ctx, p.live);
+      if (x < base + (long long)p.np * units) break;
+      base += (long long)p.np * units;
+    }
+    const int u = (int)((x - base) / p.np);
+    p.b = b;
+    p.head = u / tiles;
+    p.tile = u % tiles;
+    p.p0 = (int)((x - base) % p.np);
+    p.p1 = (int)min((long long)p.np, p.p0 + (end - x));
+    x += p.p1 - p.p0;
+    return true;
+  }
+};
+
+// ---- tensor cores
+// Shared-memory operand in rows of 128 bytes with the 128-byte swizzle (start 1024-byte aligned but for the step inside a row).
+// K-major: sbo from eight rows to the next.  MN-major: sbo from eight k to the next, lbo from 64 values to the next.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// fmt: both operands' (kind::f16: 0 f16, 1 bf16; kind::f8f6f4: 0 e4m3); fp32 sums, 128 lanes
+__host__ __device__ constexpr uint32_t idesc(int fmt, int n, bool b_mn) {
+  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f8_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(id), "r"(accumulate)
+      : "memory");
+}
+
+// Warp-wide loads of N consecutive 32-bit columns of this thread's lane; load and wait are one statement, so that nothing that
+// uses the registers can come between them.
+#define R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : R8(r, 0), R8(r, 8) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,"
+      "%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24), R8(r, 32), R8(r, 40), R8(r, 48), R8(r, 56) : "r"(taddr) : "memory");
+}
+#undef R8
+template <int N>
+__device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 8) {
+    const uint32_t v[8] = {r[i], r[i + 1], r[i + 2], r[i + 3], r[i + 4], r[i + 5], r[i + 6], r[i + 7]};
+    tmem_st8(taddr + i, v);
   }
 }
 
-template <bool kF8>
-__global__ void __launch_bounds__(kWarps * 32) tree_attention(const vdc_tree_attention_args a, vdc_status* status) {
-  const vdc_cache& c = a.cache;
-  const int lane = threadIdx.x & 31, rows = a.T * a.group;
-  const int r = blockIdx.x * kWarps + (threadIdx.x >> 5), head = blockIdx.y, b = blockIdx.z;
-  if (r >= rows) return;
-  const int t = r / a.group, g = r % a.group;
-  const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + b * a.q_b + t * a.q_t + head * a.q_kv + g * a.q_g;
-  __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.out) + b * a.o_b + t * a.o_t + head * a.o_kv + g * a.o_g;
-  const int* pages = reinterpret_cast<const int*>(a.pages) + b * a.pages_b;
-  const long long* mask = reinterpret_cast<const long long*>(a.mask) + b * a.mask_b + t * a.mask_t;
-  const int ctx = reinterpret_cast<const int*>(a.lengths)[b];
-  const int live = a.counts ? max(0, min(a.T, reinterpret_cast<const int*>(a.counts)[b])) : a.T;
-  int64_t keys = (int64_t)ctx + live;
-  if (ctx < 0 || keys > (int64_t)a.max_pages * PAGE) {
-    if (lane == 0) report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 0, b, ctx);
-    keys = 0;
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int x, int head, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(0), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// The math warps meet; true for all of them if one says so.  None of them waits for anything without a limit elsewhere, so all arrive.
+__device__ __forceinline__ bool math_any(bool x) {
+  int r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, 1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"((int)x), "n"(kMathWarps * 32) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void math_sync() { asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(kMathWarps * 32) : "memory"); }
+
+// Bit j: the row of token t attends to key page * 64 + j.
+__device__ __forceinline__ uint64_t seen_bits(const vdc_tree_attention_args& a, const Piece& p, int page, int t) {
+  auto word = [&](int w) -> uint64_t {
+    if (w >= a.words) return 0;
+    if (a.mask) return (uint64_t)__ldg(reinterpret_cast<const long long*>(a.mask) + p.b * a.mask_b + t * a.mask_t + w);
+    const int n = t + 1 - 64 * w;
+    return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+  };
+  const int off = page * PAGE - p.ctx;         // the drafted token of key 0, above -64
+  uint64_t m;
+  if (off < 0) m = word(0) << -off | ((1ull << -off) - 1);
+  else m = off & 63 ? word(off >> 6) >> (off & 63) | word((off >> 6) + 1) << (64 - (off & 63)) : word(off >> 6);
+  const int n = p.total() - page * PAGE;
+  return n < 64 ? m & ((1ull << n) - 1) : m;
+}
+
+// A record of a piece: sums [rows][128], then (reference, sum of weights) [rows]; a multiple of 16 bytes.
+__host__ __device__ __forceinline__ long long record_floats(const vdc_tree_attention_args& a) {
+  const int rows = a.T * a.group;
+  return ((long long)(rows < kRows ? rows : kRows) * (D + 2) + 3) & ~3ll;
+}
+
+__device__ __forceinline__ __nv_bfloat16* out_row(const vdc_tree_attention_args& a, int b, int head, int r) {
+  return reinterpret_cast<__nv_bfloat16*>(a.out) + b * a.o_b + (r / a.group) * a.o_t + head * a.o_kv + (r % a.group) * a.o_g;
+}
+
+template <bool kF8, int kReps>
+__global__ void __launch_bounds__(Cfg<kF8>::kThreads, 1)
+tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_constant__ CUtensorMap k_map,
+               const __grid_constant__ CUtensorMap v_map, vdc_status* status, uint64_t timeout_ns) {
+  using C = Cfg<kF8>;
+  constexpr int kKeys = PAGE / kReps, kLive = kRows / kReps;     // keys of a page that a copy takes, rows of a tile that may exist
+  extern __shared__ __align__(1024) uint8_t dyn[];
+  __shared__ TreeShared sh;
+  uint8_t* ring = dyn + (-(int)smem_u32(dyn) & 1023);
+  uint8_t* wide = ring + C::kStages * C::kStageBytes;            // widened V pages (e4m3)
+  float* scratch = reinterpret_cast<float*>(wide + (kF8 ? kWideBufs * kWideBytes : 0));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Waiter wait{&sh.fail, status, timeout_ns, VDC_TREE_ATTENTION_KIND};
+
+  if (warp == C::kMmaWarp) tmem_alloc(&sh.tmem, kCols);
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < C::kStages; ++i) {
+        mbar_init(&sh.full[i], 1);
+        mbar_init(&sh.empty[i], 1 + C::kWideWarps);
+      }
+      mbar_init(&sh.q_full, 4);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sh.s_full[i], 1);
+        mbar_init(&sh.s_empty[i], 4);
+        mbar_init(&sh.p_full[i], 4);
+        mbar_init(&sh.o_done[i], 1);
+        mbar_init(&sh.tail[i], 4);
+      }
+      for (int i = 0; i < kWideBufs; ++i) {
+        mbar_init(&sh.v_full[i], 4);
+        mbar_init(&sh.v_empty[i], 1);
+        mbar_init(&sh.par_full[i], 2);
+      }
+      sh.fail = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (lane < 16) reinterpret_cast<uint32_t*>(sh.poison)[lane] = 0;
+    // this CTA's share of all units' pages, and the sequence it begins in
+    const long long units = (long long)a.cache.n_kv * tiles_of(a), total = all_pages(a, lane) * units;
+    const long long ctas = min((long long)gridDim.x, max(total, 1ll)), me = min((long long)blockIdx.x, ctas);    // a page each at least
+    const long long begin = total * me / ctas, end = total * min(me + 1, ctas) / ctas;
+    long long base = 0;
+    int first = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      int ctx, live;
+      long long n = b0 + lane < a.B ? seq_pages(a, b0 + lane, ctx, live) * units : 0, sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long below = __shfl_up_sync(~0u, sum, o);
+        if (lane >= o) sum += below;
+      }
+      const unsigned past = __ballot_sync(~0u, base + sum > begin);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        base += __shfl_sync(~0u, sum - n, at);
+        first = b0 + at;
+        break;
+      }
+      base += __shfl_sync(~0u, sum, 31);
+    }
+    if (lane == 0) {
+      sh.begin = begin;
+      sh.end = end;
+      sh.first_base = base;
+      sh.first_b = first;
+    }
   }
-  if (t >= live) keys = 0;
-  float4 qv, acc = make_float4(0, 0, 0, 0);
-  {
-    const uint2 w = *reinterpret_cast<const uint2*>(q + lane * 4);
-    qv = make_float4(bf_lo(w.x) * a.scale, bf_hi(w.x) * a.scale, bf_lo(w.y) * a.scale, bf_hi(w.y) * a.scale);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int rows = a.T * a.group;
+  Walk walk(a, sh);
+  Piece p;
+
+  if (warp == C::kLoadWarp) {
+    // ---- pages into the ring
+    RingAt at{C::kStages};
+    bool ok = true;
+    int n = 0;
+    while (ok && walk.next(p)) {
+      const int* table = reinterpret_cast<const int*>(a.pages) + p.b * a.pages_b;
+      int ids = 0;
+      for (int i = p.p0; i < p.p1; ++i, ++n) {
+        if (((i - p.p0) & 31) == 0) {
+          ids = i + lane < p.p1 ? __ldg(table + i + lane) : 0;
+          if (ids < 0 || ids >= a.cache.n_pages) ids = 0;       // reported by the math warps, which leave the sequence out
+        }
+        const int page = __shfl_sync(~0u, ids, (i - p.p0) & 31);
+        if (n >= C::kStages && !wait.warp_wait(&sh.empty[at.st], at.parity ^ 1u, 0, i)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          uint8_t* k = ring + at.st * C::kStageBytes;
+          uint8_t* v = k + C::kPageBytes;
+          uint64_t* bar = &sh.full[at.st];
+          mbar_arrive_expect_tx(bar, C::kTx);
+          if constexpr (kF8) {
+            bulk_load_1d(k, reinterpret_cast<const void*>(a.cache.k + page * a.cache.k_page + p.head * a.cache.k_head), C::kPageBytes, bar);
+            bulk_load_1d(sh.scales[at.st][0], reinterpret_cast<const void*>(a.cache.k_scale + page * a.cache.ks_page + p.head * a.cache.ks_head), PAGE * 4, bar);
+            bulk_load_1d(sh.scales[at.st][1], reinterpret_cast<const void*>(a.cache.v_scale + page * a.cache.vs_page + p.head * a.cache.vs_head), PAGE * 4, bar);
+            bulk_load_1d(v, reinterpret_cast<const void*>(a.cache.v + page * a.cache.v_page + p.head * a.cache.v_head), C::kPageBytes, bar);
+          } else {
+            for (int h = 0; h < 2; ++h) tma_page(k + h * (C::kPageBytes / 2), &k_map, h * 64, p.head, page, bar);
+            for (int h = 0; h < 2; ++h) tma_page(v + h * (C::kPageBytes / 2), &v_map, h * 64, p.head, page, bar);
+          }
+        }
+        __syncwarp();
+        at.next();
+      }
+    }
+  } else if (warp == C::kMmaWarp) {
+    // ---- tensor cores: one thread issues; S of two pages ahead of O
+    if (lane == 0) {
+      constexpr uint32_t id_s = kF8 ? idesc(0, PAGE, false) : idesc(1, PAGE, false), id_o = kF8 ? idesc(0, D, true) : idesc(1, D, true);
+      const uint32_t base = smem_u32(ring), wide_base = smem_u32(wide);
+      RingAt s_at{C::kStages}, o_at{C::kStages};
+      int n_s[2] = {0, 0}, n_o[2] = {0, 0};      // pages of each group so far
+      int g_o = 0;
+      uint32_t piece = 0;
+      bool ok = true;
+      auto scores = [&](int i) {                 // of page i of the piece
+        const int w = i & 1;
+        if (!wait(&sh.full[s_at.st], s_at.parity, 1, i)) return false;
+        if (n_s[w] > 0 && !wait(&sh.s_empty[w], (n_s[w] - 1) & 1, 1, i)) return false;
+        tc_fence_after();
+        const uint32_t k = base + s_at.st * C::kStageBytes, d = tmem + kColS + w * PAGE;
+        if constexpr (kF8) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)            // the rows' upper parts, then their lower ones
+            umma_f8_ta(d, tmem + kColQ + j * 8, desc_sw128(k + (j & 3) * 32, 16, 1024), id_s, j > 0);
+          umma_commit(&sh.s_full[w]);
+          umma_commit(&sh.empty[s_at.st]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            umma_bf16_ta(d, tmem + kColQ + j * 8, desc_sw128(k + (j >> 2) * (C::kPageBytes / 2) + (j & 3) * 32, 16, 1024), id_s, j > 0);
+          umma_commit(&sh.s_full[w]);
+        }
+        ++n_s[w];
+        s_at.next();
+        return true;
+      };
+      while (ok && walk.next(p)) {
+        const int n = p.p1 - p.p0;
+        ok = wait(&sh.q_full, piece & 1, 1, -1);
+        ++piece;
+        if (ok) ok = scores(0);
+        if (ok && n > 1) ok = scores(1);
+        for (int i = 0; i < n && ok; ++i) {
+          const int w = i & 1;
+          ok = wait(&sh.p_full[w], n_o[w] & 1, 2, i);
+          if (kF8 && ok) ok = wait(&sh.v_full[g_o & 3], (g_o >> 2) & 1, 2, i);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t v = kF8 ? wide_base + (g_o & 3) * kWideBytes : base + o_at.st * C::kStageBytes + C::kPageBytes;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            umma_bf16_ta(tmem + kColO + w * D, tmem + kColP + w * 32 + j * 8, desc_sw128(v + j * 2048, kWideBytes / 2, 1024), id_o, i > 1 || j > 0);
+          umma_commit(&sh.o_done[w]);
+          umma_commit(kF8 ? &sh.v_empty[g_o & 3] : &sh.empty[o_at.st]);
+          ++n_o[w];
+          ++g_o;
+          o_at.next();
+          if (i + 2 < n) ok = scores(i + 2);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (kF8 && warp >= kMathWarps) {
+    // ---- e4m3 values to f16, scales to what the scores need
+    const int t = tid - kMathWarps * 32;
+    RingAt at{C::kStages};
+    int g = 0;
+    bool ok = true;
+    while (ok && walk.next(p)) {
+      for (int i = p.p0; i < p.p1; ++i, ++g) {
+        const int vb = g & 3;
+        ok = wait.warp_wait(&sh.full[at.st], at.parity, 3, i);
+        if (ok && g >= kWideBufs) ok = wait.warp_wait(&sh.v_empty[vb], ((g >> 2) - 1) & 1, 3, i);
+        if (!ok) break;
+        const int left = p.total() - i * PAGE, own = p.ctx - i * PAGE;    // rows that exist, rows in front of the drafted ones
+        if (t < PAGE) {
+          float ks = sh.scales[at.st][0][t], vs = sh.scales[at.st][1][t];
+          float lg = log2f(fmaxf(vs, 0x1p-100f)), inv = __fdividef(1.f, fmaxf(vs, 0x1p-100f));
+          if (!(vs < INFINITY)) lg = vs, inv = 0.f;             // no number: whoever attends to it gets none either
+          if (t >= left) ks = lg = inv = 0.f;
+          sh.par[vb][t] = make_float4(ks, lg, inv, 0.f);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.par_full[vb]);
+        }
+        const uint8_t* src = ring + at.st * C::kStageBytes + C::kPageBytes;
+        uint8_t* dst = wide + vb * kWideBytes;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = j * 16 + (t >> 3), piece = t & 7, sw = row & 7;
+          uint4 c = lds128(src + row * D + ((piece ^ sw) << 4));
+          if (row >= left) {
+            c = make_uint4(0, 0, 0, 0);
+          } else if (row >= own) {              // a drafted token's codes without a number: its scale says so
+            auto clean = [](uint32_t w) {
+              const uint32_t nan = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+              return w & ~((nan >> 7) * 0xFFu);
+            };
+            c = make_uint4(clean(c.x), clean(c.y), clean(c.z), clean(c.w));
+          }
+          uint32_t o[8];
+          const uint32_t in[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t h[2];
+            e4m3x4_to_half2(in[q], h);
+            o[2 * q] = h[0];
+            o[2 * q + 1] = h[1];
+          }
+          // sixteen values are two pieces of a half's row; lanes of the other half take them in the other order, for the banks' sake
+          uint8_t* to = dst + (piece >> 2) * (kWideBytes / 2) + row * 128;
+          const int lo = (((2 * piece) & 7) ^ sw) << 4, hi = (((2 * piece + 1) & 7) ^ sw) << 4;
+          const bool swap = piece >= 4;
+          const uint4 x = make_uint4(o[0], o[1], o[2], o[3]), y = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(to + (swap ? hi : lo)) = swap ? y : x;
+          *reinterpret_cast<uint4*>(to + (swap ? lo : hi)) = swap ? x : y;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sh.v_full[vb]);
+          mbar_arrive(&sh.empty[at.st]);
+        }
+        at.next();
+      }
+    }
+  } else {
+    // ---- scores to weights, sums to results
+    const int w = warp >> 2, quarter = warp & 3;                       // group, lanes of tensor memory
+    const uint32_t lanes = tmem + ((uint32_t)quarter << 21);
+    const int slot = quarter * 32 + lane, tile_row = slot % kLive, key0 = (slot / kLive) * kKeys;
+    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+    {
+      const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) tmem_st8(lanes + kColP + w * 32 + i, zero);
+      tmem_st_wait();
+    }
+    int c = 0, g = 0, tails = 0;      // pages of this group, of the CTA, and last pages of this group
+    uint32_t piece = 0;
+    while (walk.next(p)) {
+      const int r = p.tile * kRows + tile_row, t = r / a.group;
+      const bool live = r < rows && t < p.live;
+      const int n = p.p1 - p.p0;
+      bool failed = false;
+      if (w == 0) {
+        // the row into tensor memory
+        uint32_t q[64];
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + p.b * a.q_b + t * a.q_t +
+                                                          p.head * a.q_kv + (r % a.group) * a.q_g);
+        const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint4 v = live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+          q[4 * i] = v.x ^ sign; q[4 * i + 1] = v.y ^ sign; q[4 * i + 2] = v.z ^ sign; q[4 * i + 3] = v.w ^ sign;
+        }
+        if constexpr (!kF8) {
+          tmem_store(lanes + kColQ, q);
+        } else {
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) top = max(top, max(q[i] & 0x7FFFu, (q[i] >> 16) & 0x7FFFu));
+          const int e = (int)(top >> 7);                              // exponent of the largest
+          // a power of two that takes the largest to [128, 256); rows of (nearly) nothing as they are
+          const int up = e == 0xFF ? 0 : min(126, 134 - max(e, 1));
+          const float mul = exp2f((float)up);
+          uint32_t part[32];
+#pragma unroll
+          for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              uint32_t word = 0;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float2 f = make_float2(bf_lo(q[2 * i + j]) * mul, bf_hi(q[2 * i + j]) * mul);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+                if (pass == 0) {
+                  word |= hi << (16 * j);
+                } else {
+                  const float2 h = e4m3x2_to_float2(hi);
+                  word |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f.x - h.x, f.y - h.y), __NV_SATFINITE, __NV_E4M3) << (16 * j);
+                }
+              }
+              part[i] = word;
+            }
+            tmem_store(lanes + kColQ + pass * 32, part);
+          }
+          sh.q_mul[slot] = e == 0xFF ? NAN : exp2f((float)-up);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.q_full);
+      }
+      // the sequence's whole page table: a page outside the pool leaves the sequence out, in every piece alike
+      bool bad = false;
+      for (int i = tid; i < p.np; i += kMathWarps * 32) {
+        const int id = __ldg(reinterpret_cast<const int*>(a.pages) + p.b * a.pages_b + i);
+        if (id < 0 || id >= a.cache.n_pages) {
+          bad = true;
+          report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, p.b, id);
+        }
+      }
+      float row_scale = scale;
+      if constexpr (kF8) {
+        failed = !wait.warp_wait(&sh.q_full, piece & 1, 4, -1);
+        row_scale = scale * sh.q_mul[slot];
+      }
+      ++piece;
+
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < n && !failed; ++i, ++g) {
+        if ((i & 1) != w) continue;
+        const int page = p.p0 + i;
+        const bool tail = (page + 1) * PAGE > p.ctx;
+        uint64_t bits = ~0ull;
+        if (tail) bits = live ? seen_bits(a, p, page, t) : 0;
+        uint32_t raw[kKeys];
+        if (!wait.warp_wait(&sh.s_full[w], c & 1, 4, i)) {
+          failed = true;
+          break;
+        }
+        tc_fence_after();
+        tmem_load(lanes + kColS + w * PAGE + key0, raw);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.s_empty[w]);
+        float s[kKeys];
+        if constexpr (kF8) {
+          if (!wait.warp_wait(&sh.par_full[g & 3], (g >> 2) & 1, 4, i)) {
+            failed = true;
+            break;
+          }
+        }
+        uint64_t poison = 0;
+        if (tail && !kF8) {
+          // values behind the sequence's end become zeros (a weight of zero would not do: zero times NaN); so do drafted tokens'
+          // that are no numbers, whose readers get none by their scores
+          const int st = g % C::kStages;
+          if (!wait.warp_wait(&sh.full[st], (g / C::kStages) & 1, 4, i)) {
+            failed = true;
+            break;
+          }
+          const int row = (tid & 127) >> 1, key = page * PAGE + row;
+          uint4* v = reinterpret_cast<uint4*>(ring + st * C::kStageBytes + C::kPageBytes + (tid & 1) * (C::kPageBytes / 2) + row * 128);
+          bool none = key >= p.total();
+          if (!none && key >= p.ctx) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint4 x = v[j];
+              auto odd = [](uint32_t u) { return (u & 0x7F80u) == 0x7F80u || (u & 0x7F800000u) == 0x7F800000u; };
+              none |= odd(x.x) || odd(x.y) || odd(x.z) || odd(x.w);
+            }
+            if (none) atomicOr(&sh.poison[w][tails & 3][row >> 5], 1u << (row & 31));
+          }
+          none |= __shfl_xor_sync(~0u, none, 1);       // both halves of the row
+          if (none) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          if (quarter == 0 && lane < 2) sh.poison[w][(tails + 2) & 3][lane] = 0;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.tail[w]);
+          if (!wait.warp_wait(&sh.tail[w], tails & 1, 4, i)) {
+            failed = true;
+            break;
+          }
+          volatile uint32_t* po = sh.poison[w][tails & 3];
+          poison = (uint64_t)po[1] << 32 | po[0];
+          ++tails;
+        }
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) {
+          s[j] = __uint_as_float(raw[j]);
+          if constexpr (kF8) {
+            const float4 k = sh.par[g & 3][key0 + j];
+            s[j] = fmaf(s[j] * k.x, row_scale, k.y);
+          }
+        }
+        if (tail) {
+          bits >>= key0;
+          poison >>= key0;
+#pragma unroll
+          for (int j = 0; j < kKeys; ++j) {
+            if (!((bits >> j) & 1)) s[j] = -INFINITY;
+            else if (!kF8 && ((poison >> j) & 1)) s[j] = NAN;
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if constexpr (!kF8) top *= row_scale;
+        if (c > 0 && !wait.warp_wait(&sh.o_done[w], (c - 1) & 1, 4, i)) {
+          failed = true;
+          break;
+        }
+        tc_fence_after();
+        if (__any_sync(~0u, top > m + C::kSlack)) {
+          const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : exp2_ftz(m - m2);
+          l *= f;
+          m = m2;
+          if (i > 1) {
+#pragma unroll
+            for (int j = 0; j < D; j += 32) {
+              uint32_t o[32];
+              tmem_load(lanes + kColO + w * D + j, o);
+#pragma unroll
+              for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+              tmem_store(lanes + kColO + w * D + j, o);
+            }
+          }
+        }
+        const float ref = (m == -INFINITY ? 0.f : m) - C::kLift;
+        uint32_t pk[kKeys / 2];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kKeys; j += 2) {
+          const float p0 = kF8 ? exp2_ftz(s[j] - ref) : exp2_ftz(fmaf(s[j], row_scale, -ref));
+          const float p1 = kF8 ? exp2_ftz(s[j + 1] - ref) : exp2_ftz(fmaf(s[j + 1], row_scale, -ref));
+          if constexpr (kF8) {
+            sum[j & 3] = fmaf(p0, sh.par[g & 3][key0 + j].z, sum[j & 3]);
+            sum[(j + 1) & 3] = fmaf(p1, sh.par[g & 3][key0 + j + 1].z, sum[(j + 1) & 3]);
+            const __half2 h = __floats2half2_rn(p0, p1);
+            pk[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
+          } else {
+            sum[j & 3] += p0;
+            sum[(j + 1) & 3] += p1;
+            pk[j / 2] = pack_bf16x2(p0, p1);
+          }
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_store(lanes + kColP + w * 32 + key0 / 2, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[w]);
+        ++c;
+      }
+      const bool has = n > w;                  // this group had pages
+      if (!failed && has && !wait.warp_wait(&sh.o_done[w], (c - 1) & 1, 5, n)) failed = true;
+      sh.stats[warp][lane] = make_float2(m, l);
+      if (math_any(failed)) break;
+      bad = math_any(bad);
+      // ---- the row's copies meet: reference and sum of weights first, then 32 columns at a time
+      if (tid < kLive) {
+        float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2 * kReps; ++k) mm = fmaxf(mm, sh.stats[(k / kReps) * 4 + (k % kReps) * (4 / kReps) + (tid >> 5)][lane].x);
+#pragma unroll
+        for (int k = 0; k < 2 * kReps; ++k) {
+          const float2 st = sh.stats[(k / kReps) * 4 + (k % kReps) * (4 / kReps) + (tid >> 5)][lane];
+          // a copy that saw nothing has no weight; one without a number passes that on
+          ll += st.x == -INFINITY && st.y == 0.f ? 0.f : st.x == -INFINITY ? st.y : st.y * exp2_ftz(st.x - mm);
+        }
+        if (bad || !live) mm = -INFINITY, ll = 0.f;
+        sh.row[tid] = make_float2(mm, ll);
+      }
+      math_sync();
+      const float2 all = sh.row[tile_row];
+      const bool none = !has || all.y == 0.f || (m == -INFINITY && l == 0.f);
+      const float f = m == -INFINITY ? 1.f : exp2_ftz(m - all.x);
+      const bool whole = p.whole();
+      float* rec = reinterpret_cast<float*>(a.work) + (2 * blockIdx.x + (p.p1 == p.np ? 0 : 1)) * record_floats(a);
+      const int rec_rows = min(rows, kRows), tile_rows = min(rows - p.tile * kRows, kRows);
+      tc_fence_after();
+#pragma unroll 1
+      for (int col = 0; col < D; col += 32) {
+        uint32_t o[32];
+        if (has) tmem_load(lanes + kColO + w * D + col, o);
+        float* row = scratch + (warp * 32 + lane) * kScratchRow;
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<float4*>(row + j) = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                     : make_float4(__uint_as_float(o[j]) * f, __uint_as_float(o[j + 1]) * f,
+                                                                   __uint_as_float(o[j + 2]) * f, __uint_as_float(o[j + 3]) * f);
+        math_sync();
+#pragma unroll
+        for (int k = 0; k < kLive / 32; ++k) {
+          const int rr = (tid >> 3) + k * 32, c4 = (tid & 7) * 4;
+          if (rr < tile_rows) {
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < 2 * kReps; ++q) {
+              const int from = (q / kReps) * 4 + (q % kReps) * (4 / kReps) + (rr >> 5);
+              const float4 x = *reinterpret_cast<const float4*>(scratch + (from * 32 + (rr & 31)) * kScratchRow + c4);
+              sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+            }
+            if (whole) {
+              const float ll = sh.row[rr].y, inv = ll == 0.f ? 0.f : 1.f / ll;
+              *reinterpret_cast<uint2*>(out_row(a, p.b, p.head, p.tile * kRows + rr) + col + c4) =
+                  make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+            } else {
+              *reinterpret_cast<float4*>(rec + rr * D + col + c4) = sum;
+            }
+          }
+        }
+        math_sync();
+      }
+      if (!whole && tid < tile_rows) *reinterpret_cast<float2*>(rec + rec_rows * D + 2 * tid) = sh.row[tid];
+      tc_fence_before();
+    }
   }
+  // sequences without anything to attend with, or that do not fit their tables, get zeros
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    int ctx, live;
+    bool wrong;
+    if (seq_pages(a, b, ctx, live, &wrong)) continue;
+    if (wrong && tid == 0) report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 0, b, ctx);
+    const int heads = a.cache.n_kv, n = rows * heads * (D / 8);
+    for (int i = tid; i < n; i += C::kThreads)
+      *reinterpret_cast<uint4*>(out_row(a, b, (i / (D / 8)) % heads, i / (D / 8) / heads) + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  wait.drain();
+  if (warp == C::kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kCols);
+  }
+}
+
+// Joins the pieces of units that several CTAs shared: a warp per row, lane i the values 4i .. 4i + 3.  Pieces are taken in order,
+// so that the result does not depend on when they came.
+constexpr int kJoinWarps = 4;
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_constant__ vdc_tree_attention_args a, int ctas, vdc_status* status) {
+  grid_dep_wait();
+  const int lane = threadIdx.x & 31, rr = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
+  const int tiles = tiles_of(a), units = a.cache.n_kv * tiles, b = blockIdx.x / units, u = blockIdx.x % units;
+  const int rows = a.T * a.group, r = (u % tiles) * kRows + rr, rec_rows = min(rows, kRows);
+  int ctx, live;
+  const int np = seq_pages(a, b, ctx, live);
+  if (np == 0) return;
+  long long before = 0;
+  for (int i = lane; i < b; i += 32) {
+    int c2, l2;
+    before += seq_pages(a, i, c2, l2);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
+  const long long total = all_pages(a, lane) * units, first = before * units + (long long)u * np;
+  ctas = (int)min((long long)ctas, total);
+  const int c0 = (int)(((first + 1) * ctas - 1) / total), c1 = (int)(((first + np) * ctas - 1) / total);
+  if (c0 == c1 || r >= rows || rr >= kRows) return;
+  const long long rec = record_floats(a);
+  auto record = [&](int c) { return reinterpret_cast<const float*>(a.work) + (2ll * c + (c == c1 ? 0 : 1)) * rec; };
   float m = -INFINITY, l = 0.f;
-  for (int64_t at = 0; at < keys; ++at) {
-    const int p = pages[at / PAGE], row = (int)(at % PAGE);
-    if (p < 0 || p >= c.n_pages) {
-      if (lane == 0) report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, b, p);
-      m = -INFINITY, l = 0.f, acc = make_float4(0, 0, 0, 0);
-      break;
-    }
-    if (at >= ctx) {
-      const int j = (int)(at - ctx);
-      if (!(a.mask ? (mask[j >> 6] >> (j & 63)) & 1 : j <= t)) continue;
-    }
-    const float4 k = stored4<kF8>(c.k + p * c.k_page + head * c.k_head, c.k_scale + p * c.ks_page + head * c.ks_head, row, lane);
-    const float4 v = stored4<kF8>(c.v + p * c.v_page + head * c.v_head, c.v_scale + p * c.vs_page + head * c.vs_head, row, lane);
-    const float s = warp_sum(qv.x * k.x + qv.y * k.y + qv.z * k.z + qv.w * k.w);
-    const float m2 = fmaxf(m, s), f = expf(m - m2), e = expf(s - m2);
-    m = m2;
-    l = l * f + e;
-    acc = make_float4(acc.x * f + e * v.x, acc.y * f + e * v.y, acc.z * f + e * v.z, acc.w * f + e * v.w);
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, __ldg(record(c) + rec_rows * D + 2 * rr));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  for (int c = c0; c <= c1; ++c) {
+    const float* p = record(c);
+    const float2 st = *reinterpret_cast<const float2*>(p + rec_rows * D + 2 * rr);
+    const float4 x = *reinterpret_cast<const float4*>(p + rr * D + lane * 4);
+    const float f = st.x == -INFINITY ? 1.f : exp2_ftz(st.x - m);      // no reference: nothing, or no number
+    l += st.y * f;
+    sum.x += x.x * f; sum.y += x.y * f; sum.z += x.z * f; sum.w += x.w * f;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(o + lane * 4) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  *reinterpret_cast<uint2*>(out_row(a, b, u / tiles, r) + lane * 4) =
+      make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+}
+
+template <bool kF8>
+constexpr int dynamic_bytes() {
+  return 1024 + Cfg<kF8>::kStages * Cfg<kF8>::kStageBytes + (kF8 ? kWideBufs * kWideBytes : 0) + kScratch;
+}
+
+int ctas_of(const vdc_tree_attention_args* a, int sms) {
+  const long long rows = (long long)a->T * a->group, most = (long long)a->B * a->cache.n_kv * ((rows + kRows - 1) / kRows) * a->max_pages;
+  const int n = sms < VDC_MAX_SMS ? sms : VDC_MAX_SMS;
+  return (int)(most < n ? most : n);
 }
 
 }  // namespace
@@ -78,23 +806,70 @@ extern "C" const char* vdc_cache_refuses(const vdc_cache* c, int max_pages);
 
 extern "C" const char* vdc_tree_attention_refuses(const vdc_tree_attention_args* a, bool pointers) {
   auto al = [](uint64_t p, int n) { return p % n == 0; };
-  if (a->B < 1 || a->T < 1 || a->T > 4096 || a->group < 1 || a->group > 128 || a->B > 65535) return "tree_attention: tokens or heads out of range";
+  if (a->B < 1 || a->T < 1 || a->T > 4096 || a->group < 1 || a->group > 128 || a->max_pages < 1 || a->max_pages > 0x7FFFFFFF / VDC_KV_PAGE ||
+      a->cache.n_kv < 1 || (long long)a->B * a->cache.n_kv * ((a->T * a->group + kRows - 1) / kRows) > 0x7FFFFFFF)
+    return "tree_attention: tokens or heads out of range";
   if (a->words * 64 < a->T) return "tree_attention: the mask has fewer bits than there are tokens";
+  if (!(a->scale > -INFINITY && a->scale < INFINITY)) return "tree_attention: the scale is no number";
   if (!pointers) return nullptr;
   if (const char* why = vdc_cache_refuses(&a->cache, a->max_pages)) return why;
   if (!a->q || !a->out || !al(a->q | a->out, 16)) return "tree_attention: null or misaligned rows";
   if (!al(a->q_b | a->q_t | a->q_kv | a->q_g | a->o_b | a->o_t | a->o_kv | a->o_g, 8)) return "tree_attention: row strides must be multiples of 8";
   if (!a->pages || !a->lengths || !al(a->pages | a->lengths | a->counts, 4) || !al(a->mask, 8)) return "tree_attention: null or misaligned tables";
+  if (!a->work || !al(a->work, 16)) return "tree_attention: null or misaligned workspace";
   return nullptr;
 }
 
-extern "C" long long vdc_tree_attention_bytes(const vdc_tree_attention_args*) { return 0; }
+extern "C" long long vdc_tree_attention_bytes(const vdc_tree_attention_args* a) {
+  return 2ll * ctas_of(a, VDC_MAX_SMS) * record_floats(*a) * 4;
+}
 
-extern "C" cudaError_t vdc_tree_attention_prepare() { return cudaSuccess; }
+namespace {
+using Kernel = void (*)(const vdc_tree_attention_args, const CUtensorMap, const CUtensorMap, vdc_status*, uint64_t);
+const Kernel kKernels[2][3] = {{tree_attention<false, 1>, tree_attention<false, 2>, tree_attention<false, 4>},
+                               {tree_attention<true, 1>, tree_attention<true, 2>, tree_attention<true, 4>}};
+}  // namespace
 
-extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* a, int, vdc_status* status, uint64_t, cudaStream_t stream) {
-  const dim3 grid((a->T * a->group + kWarps - 1) / kWarps, a->cache.n_kv, a->B);
-  if (a->cache.kind) tree_attention<true><<<grid, kWarps * 32, 0, stream>>>(*a, status);
-  else tree_attention<false><<<grid, kWarps * 32, 0, stream>>>(*a, status);
-  return cudaGetLastError();
+extern "C" cudaError_t vdc_tree_attention_prepare() {
+  for (int f8 = 0; f8 < 2; ++f8)
+    for (int i = 0; i < 3; ++i)
+      if (cudaError_t e = cudaFuncSetAttribute((const void*)kKernels[f8][i], cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               f8 ? dynamic_bytes<true>() : dynamic_bytes<false>()))
+        return e;
+  return cudaSuccess;
+}
+
+extern "C" int vdc_build_tma_desc(void* out_desc, const void* base, int dtype, int rank, const uint64_t* shape, const uint64_t* strides_bytes,
+                                  const uint32_t* box_dim, const uint32_t* elem_strides, int swizzle_bytes, int interleave_bytes);
+
+extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* a, int sms, vdc_status* status, uint64_t timeout_ns,
+                                                 cudaStream_t stream) {
+  alignas(64) CUtensorMap maps[2] = {};
+  const vdc_cache& c = a->cache;
+  if (!c.kind) {
+    // a page of a head in two halves of 64 values, rows of 128 bytes
+    const uint64_t shape[4] = {VDC_HEAD_DIM, VDC_KV_PAGE, (uint64_t)c.n_kv, (uint64_t)c.n_pages};
+    const uint32_t box[4] = {64, VDC_KV_PAGE, 1, 1}, ones[4] = {1, 1, 1, 1};
+    auto step = [](int n, int64_t stride) { return n > 1 ? (uint64_t)stride : (uint64_t)Cfg<false>::kPageBytes; };
+    const uint64_t ks[3] = {2 * VDC_HEAD_DIM, step(c.n_kv, c.k_head), step(c.n_pages, c.k_page)};
+    const uint64_t vs[3] = {2 * VDC_HEAD_DIM, step(c.n_kv, c.v_head), step(c.n_pages, c.v_page)};
+    if (vdc_build_tma_desc(&maps[0], reinterpret_cast<const void*>(c.k), 2, 4, shape, ks, box, ones, 0, 0) != VDC_OK ||
+        vdc_build_tma_desc(&maps[1], reinterpret_cast<const void*>(c.v), 2, 4, shape, vs, box, ones, 0, 0) != VDC_OK)
+      return cudaErrorInvalidValue;
+  }
+  const int rows = a->T * a->group, reps = rows <= 32 ? 2 : rows <= 64 ? 1 : 0, ctas = ctas_of(a, sms);
+  const int units = a->B * c.n_kv * ((rows + kRows - 1) / kRows);
+  kKernels[c.kind][reps]<<<ctas, c.kind ? Cfg<true>::kThreads : Cfg<false>::kThreads,
+                           c.kind ? dynamic_bytes<true>() : dynamic_bytes<false>(), stream>>>(*a, maps[0], maps[1], status, timeout_ns);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)units, (unsigned)(((rows < kRows ? rows : kRows) + kJoinWarps - 1) / kJoinWarps));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, tree_join, *a, ctas, status);
 }
