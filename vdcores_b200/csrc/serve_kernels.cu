@@ -203,12 +203,21 @@ __global__ void __launch_bounds__(kReadThreads) read_cache(const vdc_read_cache_
 }
 
 // ------------------------------------------------------------------------- //
-// adjust_logits: a row is shared by the CTAs of a cluster, a contiguous part of the vocabulary each.  A CTA walks its part in
-// tiles: it counts the row's ids that fall into the tile in shared memory, one word a token (bit 31: in the prompt, below:
-// times generated), and adds up the tile's biases; then one pass over the logits.  The largest logits meet over the cluster.
+// adjust_logits: a row is shared by the CTAs of a cluster, a contiguous part of the vocabulary each, walked in tiles.  For a tile a
+// CTA counts the row's ids that fall into it in shared memory: a word a token with the times generated and, above them, a bit for
+// "biased" and one for "in the prompt".  Then one pass over the tile's logits, eight at a time: most have a word of zero and need
+// nothing.  The words have 16 bits where the ids cannot overflow 14 of them, otherwise 32 and half the tile.
+// The largest logits meet over the cluster.
 // ------------------------------------------------------------------------- //
-constexpr int kLogitThreads = 512, kLogitTile = 16384, kLogitMaxBias = 4096;
+constexpr int kLogitThreads = 512, kLogitCountBytes = 65536, kLogitMaxBias = 4096, kLogitShort = 0x3FFF;
 
+__device__ __forceinline__ float2 pair_of(uint32_t u, __nv_bfloat16) { return make_float2(bf_lo(u), bf_hi(u)); }
+__device__ __forceinline__ float2 pair_of(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+__device__ __forceinline__ uint32_t pair_to(float x, float y, __nv_bfloat16) { return pack_bf16x2(x, y); }
+__device__ __forceinline__ uint32_t pair_to(float x, float y, __half) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 template <class T> __device__ __forceinline__ float to_f32(T x);
 template <> __device__ __forceinline__ float to_f32(float x) { return x; }
 template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -217,6 +226,40 @@ template <class T> __device__ __forceinline__ T from_f32(float x);
 template <> __device__ __forceinline__ float from_f32(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
+
+// Eight logits as they lie in memory, at a multiple of 16 bytes.
+template <class T>
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t u[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(u[i]);
+    } else {
+      const uint32_t u[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = pair_of(u[i], T());
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
+  }
+};
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pair_to(x[0], x[1], T()), pair_to(x[2], x[3], T()), pair_to(x[4], x[5], T()), pair_to(x[6], x[7], T()));
+  }
+}
 
 // Largest first, and the lower id of two equal ones; NaN never.
 __device__ __forceinline__ void better(float& v, int& i, float v2, int i2) {
@@ -230,13 +273,16 @@ struct LogitShared {
   int cta_at;
 };
 
-template <class Tin, class Tout>
-__global__ void __launch_bounds__(kLogitThreads) adjust_logits(const vdc_adjust_logits_args a, int parts, vdc_status* status) {
-  extern __shared__ uint32_t count[];                     // a word a token of the tile, then (n_bias) a float a token
+template <class Tin, class Tout, class Count>
+__global__ void __launch_bounds__(kLogitThreads, 3) adjust_logits(const vdc_adjust_logits_args a, int parts, vdc_status* status) {
+  constexpr int kTile = kLogitCountBytes / (int)sizeof(Count);       // tokens
+  constexpr uint32_t kPrompt = 1u << (8 * sizeof(Count) - 1), kBiased = kPrompt >> 1;
+  extern __shared__ uint4 dyn[];                                     // the tile's words, then the row's biases: ids, values
   __shared__ LogitShared sh;
+  uint32_t* count = reinterpret_cast<uint32_t*>(dyn);
+  int* ids = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(dyn) + kLogitCountBytes);
+  float* add = reinterpret_cast<float*>(ids + a.n_bias);
   const int row = blockIdx.x / parts, part = blockIdx.x % parts, tid = threadIdx.x;
-  const int per = ((a.vocab + parts - 1) / parts + 7) & ~7;
-  const int v_begin = min(a.vocab, part * per), v_end = min(a.vocab, v_begin + per);
   const Tin* in = reinterpret_cast<const Tin*>(a.logits) + row * a.logits_s;
   Tout* out = reinterpret_cast<Tout*>(a.out) + row * a.out_s;
   int req = row;
@@ -254,66 +300,120 @@ __global__ void __launch_bounds__(kLogitThreads) adjust_logits(const vdc_adjust_
   }
   const int n_path = seen_matters && a.path ? a.path_n : 0;
   const int* path = reinterpret_cast<const int*>(a.path) + row * a.path_s;
-  const bool counted = n_hist + n_path > 0;
   const int n_bias = known && a.bias_ids ? a.n_bias : 0;
-  const int* bias_ids = reinterpret_cast<const int*>(a.bias_ids) + (known ? req * a.bias_s : 0);
-  const float* bias = reinterpret_cast<const float*>(a.bias) + (known ? req * a.bias_s : 0);
-  float* add = reinterpret_cast<float*>(count + kLogitTile);
+  const bool counted = n_hist + n_path + n_bias > 0;
+  for (int i = tid; i < n_bias; i += kLogitThreads) {
+    ids[i] = __ldg(reinterpret_cast<const int*>(a.bias_ids) + req * a.bias_s + i);
+    add[i] = __ldg(reinterpret_cast<const float*>(a.bias) + req * a.bias_s + i);
+  }
   const uint32_t* allowed = a.allowed ? reinterpret_cast<const uint32_t*>(a.allowed) + row * a.allowed_s : nullptr;
+
+  // Groups of eight tokens start where a load of eight logits may: group g holds tokens 8 g - lead .. 8 g - lead + 7, of which the
+  // first and the last group have some only.
+  const int lead = (int)(((uintptr_t)in & 15) / sizeof(Tin)), n_groups = (a.vocab + lead + 7) / 8;
+  const int per = (n_groups + parts - 1) / parts, g_begin = min(n_groups, part * per), g_end = min(n_groups, g_begin + per);
+  const bool wide_out = (((uintptr_t)(out - lead)) & 15) == 0;
+  auto whole = [&](int g) { return 8 * g >= lead && 8 * g + 8 - lead <= a.vocab; };
 
   float best = -INFINITY;
   int best_at = 0x7FFFFFFF;
-  for (int v0 = v_begin; v0 < v_end; v0 += kLogitTile) {
-    const int n = min(kLogitTile, v_end - v0);
-    if (counted || n_bias) {
+  for (int g0 = g_begin; g0 < g_end; g0 += kTile / 8) {
+    const int g1 = min(g_end, g0 + kTile / 8), first = 8 * g0 - lead;       // the tile's first token
+    if (counted) {
       __syncthreads();
-      for (int i = tid; i < n; i += kLogitThreads) {
-        count[i] = 0;
-        if (n_bias) add[i] = 0.f;
-      }
+      for (int i = tid; i < (g1 - g0) * (int)sizeof(Count) / 2; i += kLogitThreads) dyn[i] = make_uint4(0, 0, 0, 0);
       __syncthreads();
+      const unsigned n = (unsigned)(g1 - g0) * 8;
+      auto mark = [&](unsigned k, uint32_t bit, bool once) {
+        if (k >= n) return;
+        uint32_t* word = sizeof(Count) == 4 ? count + k : count + (k >> 1);
+        bit <<= sizeof(Count) == 4 ? 0 : 16 * (k & 1);
+        if (once) atomicOr(word, bit);
+        else atomicAdd(word, bit);
+      };
+#pragma unroll 4
       for (int i = tid; i < n_hist; i += kLogitThreads) {
-        const unsigned k = (unsigned)(__ldg(hist + i) - v0);
-        if (k < (unsigned)n) {
-          if (i < n_prompt) atomicOr(&count[k], 0x80000000u);
-          else atomicAdd(&count[k], 1u);
-        }
+        const unsigned k = (unsigned)(__ldg(hist + i) - first);
+        mark(k, i < n_prompt ? kPrompt : 1u, i < n_prompt);
       }
-      for (int i = tid; i < n_path; i += kLogitThreads) {
-        const unsigned k = (unsigned)(__ldg(path + i) - v0);
-        if (k < (unsigned)n) atomicAdd(&count[k], 1u);
-      }
-      // an id's first mention adds up all of its biases, in their order
-      for (int i = tid; i < n_bias; i += kLogitThreads) {
-        const int id = __ldg(bias_ids + i);
-        const unsigned k = (unsigned)(id - v0);
-        if (k >= (unsigned)n) continue;
-        bool first = true;
-        for (int j = 0; j < i && first; ++j) first = __ldg(bias_ids + j) != id;
-        if (!first) continue;
-        float sum = 0.f;
-        for (int j = i; j < n_bias; ++j)
-          if (__ldg(bias_ids + j) == id) sum += __ldg(bias + j);
-        add[k] = sum;
-      }
+      for (int i = tid; i < n_path; i += kLogitThreads) mark((unsigned)(__ldg(path + i) - first), 1u, false);
+      for (int i = tid; i < n_bias; i += kLogitThreads) mark((unsigned)(ids[i] - first), kBiased, true);
       __syncthreads();
     }
-    for (int i = tid; i < n; i += kLogitThreads) {
-      const int v = v0 + i;
-      float x = to_f32(in[v]);
-      if (counted) {
-        const uint32_t w = count[i];
-        if (w) {
-          const uint32_t times = w & 0x7FFFFFFFu;
-          if (a.repetition) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-          x = __fsub_rn(x, __fmul_rn(freq, (float)times));
-          if (times) x = __fsub_rn(x, pres);
+    Eight<Tin> next;
+    int g = g0 + tid;
+    if (g < g1 && whole(g)) next.load(in + (8 * g - lead));
+    for (; g < g1; g += kLogitThreads) {
+      const int v = 8 * g - lead;
+      const bool full = whole(g);
+      float x[8];
+      uint32_t exist = 0xFF;
+      if (full) {
+        next.get(x);
+      } else {
+        exist = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool is = v + j >= 0 && v + j < a.vocab;
+          x[j] = is ? to_f32(in[v + j]) : -INFINITY;
+          exist |= (uint32_t)is << j;
         }
       }
-      if (n_bias) x = __fadd_rn(x, add[i]);
-      if (allowed && !((__ldg(allowed + (v >> 5)) >> (v & 31)) & 1)) x = -INFINITY;
-      out[v] = from_f32<Tout>(x);
-      better(best, best_at, x, v);
+      const int g2 = g + kLogitThreads;
+      if (g2 < g1 && whole(g2)) next.load(in + (8 * g2 - lead));
+      if (counted) {
+        uint32_t w[8];
+        uint32_t any;
+        if constexpr (sizeof(Count) == 2) {
+          const uint4 c = dyn[g - g0];
+          any = c.x | c.y | c.z | c.w;
+          w[0] = c.x & 0xFFFF; w[1] = c.x >> 16; w[2] = c.y & 0xFFFF; w[3] = c.y >> 16;
+          w[4] = c.z & 0xFFFF; w[5] = c.z >> 16; w[6] = c.w & 0xFFFF; w[7] = c.w >> 16;
+        } else {
+          const uint4 c = dyn[2 * (g - g0)], d = dyn[2 * (g - g0) + 1];
+          any = c.x | c.y | c.z | c.w | d.x | d.y | d.z | d.w;
+          w[0] = c.x; w[1] = c.y; w[2] = c.z; w[3] = c.w; w[4] = d.x; w[5] = d.y; w[6] = d.z; w[7] = d.w;
+        }
+        if (any) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (w[j] & ~kBiased) {
+              const uint32_t times = w[j] & (kBiased - 1);
+              if (a.repetition) x[j] = x[j] > 0.f ? __fdiv_rn(x[j], rep) : __fmul_rn(x[j], rep);
+              x[j] = __fsub_rn(x[j], __fmul_rn(freq, (float)times));
+              if (times) x[j] = __fsub_rn(x[j], pres);
+            }
+            if (w[j] & kBiased) {
+              float sum = 0.f;
+              for (int i = 0; i < n_bias; ++i)
+                if (ids[i] == v + j) sum += add[i];
+              x[j] = __fadd_rn(x[j], sum);
+            }
+          }
+        }
+      }
+      if (allowed) {
+        const int v1 = max(v, 0), word = v1 >> 5;
+        const uint32_t lo = __ldg(allowed + word), hi = (v1 & 31) > 24 && 32 * (word + 1) < a.vocab ? __ldg(allowed + word + 1) : 0u;
+        const uint32_t bits = __funnelshift_r(lo, hi, v1 & 31) << (v1 - v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (!((bits >> j) & 1)) x[j] = -INFINITY;
+      }
+      const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      if (top > best) {
+        best = top;
+#pragma unroll
+        for (int j = 7; j >= 0; --j)
+          if (x[j] == top) best_at = v + j;
+      }
+      if (full && wide_out) {
+        store8(out + v, x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if ((exist >> j) & 1) out[v + j] = from_f32<Tout>(x[j]);
+      }
     }
   }
   if (!a.tokens) return;      // the same for every CTA of a cluster
@@ -412,15 +512,19 @@ extern "C" const char* vdc_adjust_logits_refuses(const vdc_adjust_logits_args* a
   return nullptr;
 }
 
-constexpr int kLogitSmem = kLogitTile * 4, kLogitSmemBias = 2 * kLogitTile * 4;
+constexpr int kLogitSmem = kLogitCountBytes + kLogitMaxBias * 8;
+
 template <class Tin, class Tout>
 static cudaError_t launch_logits(const vdc_adjust_logits_args* a, vdc_status* status, cudaStream_t stream) {
-  int parts = 1;
-  while (parts < 8 && (int64_t)a->rows * parts < 2 * VDC_MAX_SMS && a->vocab > parts * 2048) parts *= 2;
+  const bool is_short = (int64_t)a->L + a->path_n <= kLogitShort;
+  // a tile to a CTA; where that leaves SMs idle, more CTAs, of 2048 tokens at least
+  int parts = (a->vocab + 8 + kLogitCountBytes / 2 - 1) / (kLogitCountBytes / 2);
+  if (parts > 8) parts = 8;
+  while (parts < 8 && (int64_t)a->rows * parts < 2 * VDC_MAX_SMS && a->vocab > parts * 2048) ++parts;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a->rows * parts));
   cfg.blockDim = dim3(kLogitThreads);
-  cfg.dynamicSmemBytes = a->n_bias ? kLogitSmemBias : kLogitSmem;
+  cfg.dynamicSmemBytes = kLogitCountBytes + a->n_bias * 8;
   cfg.stream = stream;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
@@ -428,7 +532,8 @@ static cudaError_t launch_logits(const vdc_adjust_logits_args* a, vdc_status* st
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, adjust_logits<Tin, Tout>, *a, parts, status);
+  return is_short ? cudaLaunchKernelEx(&cfg, adjust_logits<Tin, Tout, uint16_t>, *a, parts, status)
+                  : cudaLaunchKernelEx(&cfg, adjust_logits<Tin, Tout, uint32_t>, *a, parts, status);
 }
 
 extern "C" cudaError_t vdc_adjust_logits_launch(const vdc_adjust_logits_args* a, vdc_status* status, cudaStream_t stream) {
@@ -438,11 +543,18 @@ extern "C" cudaError_t vdc_adjust_logits_launch(const vdc_adjust_logits_args* a,
   return a->out_type ? launch_logits<__half, __half>(a, status, stream) : launch_logits<__half, float>(a, status, stream);
 }
 
-extern "C" cudaError_t vdc_adjust_logits_prepare() {
-  const void* all[] = {(const void*)adjust_logits<float, float>, (const void*)adjust_logits<__nv_bfloat16, __nv_bfloat16>,
-                       (const void*)adjust_logits<__nv_bfloat16, float>, (const void*)adjust_logits<__half, __half>,
-                       (const void*)adjust_logits<__half, float>};
-  for (const void* f : all)
-    if (cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kLogitSmemBias)) return e;
+template <class Tin, class Tout>
+static cudaError_t prepare_logits() {
+  const void* both[] = {(const void*)adjust_logits<Tin, Tout, uint16_t>, (const void*)adjust_logits<Tin, Tout, uint32_t>};
+  for (const void* f : both)
+    if (cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kLogitSmem)) return e;
   return cudaSuccess;
+}
+extern "C" cudaError_t vdc_adjust_logits_prepare() {
+  cudaError_t e = prepare_logits<float, float>();
+  if (e == cudaSuccess) e = prepare_logits<__nv_bfloat16, __nv_bfloat16>();
+  if (e == cudaSuccess) e = prepare_logits<__nv_bfloat16, float>();
+  if (e == cudaSuccess) e = prepare_logits<__half, __half>();
+  if (e == cudaSuccess) e = prepare_logits<__half, float>();
+  return e;
 }

@@ -36,14 +36,18 @@ struct Cfg {
   static constexpr int kStageBytes = 2 * kPageBytes;
   static constexpr int kTx = kStageBytes + (kF8 ? 2 * PAGE * 4 : 0);
   static constexpr int kWideWarps = kF8 ? 4 : 0;
-  static constexpr int kLoadWarp = kMathWarps + kWideWarps, kMmaWarp = kLoadWarp + 1;
-  static constexpr int kThreads = (kMmaWarp + 1) * 32;
+  static constexpr int kLoadWarp = kMathWarps + kWideWarps, kScoreWarp = kLoadWarp + 1, kSumWarp = kLoadWarp + 2, kParWarp = kLoadWarp + 3;
+  static constexpr int kThreads = kF8 ? 512 : 384;        // whole groups of four warps
+  // registers of a thread: at launch, then of the math warps and of the others (512 * 128 = 256 * 168 + 256 * 88, 384 * 168 =
+  // 256 * 208 + 128 * 88)
+  static constexpr int kMathRegs = kF8 ? 168 : 208, kOtherRegs = 88;
   static constexpr float kSlack = kF8 ? 4.f : 8.f;      // powers of two by which a score may exceed its row's reference
   static constexpr float kLift = kF8 ? 11.f : 0.f;      // f16 weights are kept that much larger: 2^15 at most, 2^-25 of the largest with all bits
 };
 constexpr int kWideBufs = 4, kWideBytes = PAGE * D * 2;
 constexpr int kScratchRow = 36;                         // floats of a row's 32 sums on their way between warps
 constexpr int kScratch = kMathWarps * 32 * kScratchRow * 4;
+constexpr int kQRow = 68;                               // words of a query row on its way to tensor memory: 256 bytes, apart for the banks' sake
 
 // columns of tensor memory
 constexpr int kColO = 0, kColS = 256, kColP = 384, kColQ = 448, kCols = 512;
@@ -59,7 +63,7 @@ struct TreeShared {
   float q_mul[kRows];
   float2 stats[kMathWarps][32];       // of the rows on a warp's lanes: reference, sum of weights
   float2 row[kRows];                  // of a row over all its copies: the same
-  alignas(16) float4 par[kWideBufs][PAGE];     // of a key of an e4m3 page: its scale, log2 of the value's, 1 / the value's
+  alignas(16) float par[kWideBufs][3][PAGE];   // of the keys of an e4m3 page: scale, log2 of the value's, 1 / the value's
   alignas(16) float scales[8][2][PAGE];
 };
 
@@ -135,6 +139,60 @@ __device__ __forceinline__ void umma_f8_ta(uint32_t d_tmem, uint32_t a_tmem, uin
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(id), "r"(accumulate)
       : "memory");
+}
+
+template <int kRegs, bool kMore>
+__device__ __forceinline__ void set_registers() {
+  if constexpr (kMore) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+// True for one lane of a whole warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// Bounded wait on an mbarrier: 1 when its phase is over, 0 when another role has failed or the wait took longer than the limit.  The
+// loop is in the statement, and callers look at the answers of a page's waits once, together: a branch of one warp costs some 20
+// cycles, and a completed wait 56 like this, 131 with a vote and a branch of its own.  After a wait that was given up what the page
+// computes is nothing, but all of its accesses stay where they are.
+__device__ __forceinline__ uint32_t spin(uint64_t* bar, uint32_t parity, const Waiter& wait) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u64 first, now;\n\t.reg .u32 f;\n\t"
+      "mov.u32 %0, 1;\n\t"
+      "mov.u64 first, 0;\n\t"
+      "again_%=:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra done_%=;\n\t"
+      "ld.volatile.shared.u32 f, [%3];\n\t"
+      "setp.ne.u32 q, f, 0;\n\t"
+      "@q bra fail_%=;\n\t"
+      "mov.u64 now, %%globaltimer;\n\t"
+      "setp.eq.u64 q, first, 0;\n\t"
+      "@q mov.u64 first, now;\n\t"
+      "sub.u64 now, now, first;\n\t"
+      "setp.le.u64 q, now, %4;\n\t"
+      "@q bra again_%=;\n\t"
+      "fail_%=:\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "done_%=:\n\t}"
+      : "=&r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<int*>(wait.fail))), "l"(wait.timeout_ns)
+      : "memory");
+  return ok;
+}
+// Whether all lanes' waits of a page ended well; if not, the status block and the other roles hear of it.
+__device__ __forceinline__ bool all_well(uint32_t ok, const Waiter& wait, int role, int at) {
+  if (__all_sync(~0u, ok)) return true;
+  if ((threadIdx.x & 31) == 0 && !*wait.fail) {
+    report(wait.status, VDC_ERR_TIMEOUT, wait.kind, role, at, 0);
+    *wait.fail = 1;
+  }
+  __syncwarp();
+  return false;
 }
 
 // Warp-wide loads of N consecutive 32-bit columns of this thread's lane; load and wait are one statement, so that nothing that
@@ -224,15 +282,15 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
   uint8_t* ring = dyn + (-(int)smem_u32(dyn) & 1023);
   uint8_t* wide = ring + C::kStages * C::kStageBytes;            // widened V pages (e4m3)
   float* scratch = reinterpret_cast<float*>(wide + (kF8 ? kWideBufs * kWideBytes : 0));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
   const Waiter wait{&sh.fail, status, timeout_ns, VDC_TREE_ATTENTION_KIND};
 
-  if (warp == C::kMmaWarp) tmem_alloc(&sh.tmem, kCols);
+  if (warp == C::kScoreWarp) tmem_alloc(&sh.tmem, kCols);
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < C::kStages; ++i) {
         mbar_init(&sh.full[i], 1);
-        mbar_init(&sh.empty[i], 1 + C::kWideWarps);
+        mbar_init(&sh.empty[i], kF8 ? 1 + C::kWideWarps + 1 : 1);
       }
       mbar_init(&sh.q_full, 4);
       for (int i = 0; i < 2; ++i) {
@@ -245,7 +303,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       for (int i = 0; i < kWideBufs; ++i) {
         mbar_init(&sh.v_full[i], 4);
         mbar_init(&sh.v_empty[i], 1);
-        mbar_init(&sh.par_full[i], 2);
+        mbar_init(&sh.par_full[i], 1);
       }
       sh.fail = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -286,9 +344,11 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   const int rows = a.T * a.group;
-  Walk walk(a, sh);
-  Piece p;
 
+  if (warp >= kMathWarps) {
+    set_registers<C::kOtherRegs, false>();
+    Walk walk(a, sh);
+    Piece p;
   if (warp == C::kLoadWarp) {
     // ---- pages into the ring
     RingAt at{C::kStages};
@@ -303,7 +363,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
           if (ids < 0 || ids >= a.cache.n_pages) ids = 0;       // reported by the math warps, which leave the sequence out
         }
         const int page = __shfl_sync(~0u, ids, (i - p.p0) & 31);
-        if (n >= C::kStages && !wait.warp_wait(&sh.empty[at.st], at.parity ^ 1u, 0, i)) {
+        if (n >= C::kStages && !all_well(spin(&sh.empty[at.st], at.parity ^ 1u, wait), wait, 0, i)) {
           ok = false;
           break;
         }
@@ -326,129 +386,179 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         at.next();
       }
     }
-  } else if (warp == C::kMmaWarp) {
-    // ---- tensor cores: one thread issues; S of two pages ahead of O
-    if (lane == 0) {
-      constexpr uint32_t id_s = kF8 ? idesc(0, PAGE, false) : idesc(1, PAGE, false), id_o = kF8 ? idesc(0, D, true) : idesc(1, D, true);
-      const uint32_t base = smem_u32(ring), wide_base = smem_u32(wide);
-      RingAt s_at{C::kStages}, o_at{C::kStages};
-      int n_s[2] = {0, 0}, n_o[2] = {0, 0};      // pages of each group so far
-      int g_o = 0;
-      uint32_t piece = 0;
-      bool ok = true;
-      auto scores = [&](int i) {                 // of page i of the piece
-        const int w = i & 1;
-        if (!wait(&sh.full[s_at.st], s_at.parity, 1, i)) return false;
-        if (n_s[w] > 0 && !wait(&sh.s_empty[w], (n_s[w] - 1) & 1, 1, i)) return false;
-        tc_fence_after();
-        const uint32_t k = base + s_at.st * C::kStageBytes, d = tmem + kColS + w * PAGE;
-        if constexpr (kF8) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)            // the rows' upper parts, then their lower ones
-            umma_f8_ta(d, tmem + kColQ + j * 8, desc_sw128(k + (j & 3) * 32, 16, 1024), id_s, j > 0);
-          umma_commit(&sh.s_full[w]);
-          umma_commit(&sh.empty[s_at.st]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            umma_bf16_ta(d, tmem + kColQ + j * 8, desc_sw128(k + (j >> 2) * (C::kPageBytes / 2) + (j & 3) * 32, 16, 1024), id_s, j > 0);
-          umma_commit(&sh.s_full[w]);
-        }
-        ++n_s[w];
-        s_at.next();
-        return true;
-      };
-      while (ok && walk.next(p)) {
-        const int n = p.p1 - p.p0;
-        ok = wait(&sh.q_full, piece & 1, 1, -1);
-        ++piece;
-        if (ok) ok = scores(0);
-        if (ok && n > 1) ok = scores(1);
-        for (int i = 0; i < n && ok; ++i) {
-          const int w = i & 1;
-          ok = wait(&sh.p_full[w], n_o[w] & 1, 2, i);
-          if (kF8 && ok) ok = wait(&sh.v_full[g_o & 3], (g_o >> 2) & 1, 2, i);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t v = kF8 ? wide_base + (g_o & 3) * kWideBytes : base + o_at.st * C::kStageBytes + C::kPageBytes;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            umma_bf16_ta(tmem + kColO + w * D, tmem + kColP + w * 32 + j * 8, desc_sw128(v + j * 2048, kWideBytes / 2, 1024), id_o, i > 1 || j > 0);
-          umma_commit(&sh.o_done[w]);
-          umma_commit(kF8 ? &sh.v_empty[g_o & 3] : &sh.empty[o_at.st]);
-          ++n_o[w];
-          ++g_o;
-          o_at.next();
-          if (i + 2 < n) ok = scores(i + 2);
-        }
-      }
-    }
-    __syncwarp();
-  } else if (kF8 && warp >= kMathWarps) {
-    // ---- e4m3 values to f16, scales to what the scores need
-    const int t = tid - kMathWarps * 32;
+  } else if (warp == C::kScoreWarp) {
+    // ---- S = Q K^T, as soon as the group has taken its last S.  The whole warp walks and waits, an elected lane issues:
+    // descriptors are then the same for the warp as far as the compiler knows, and stay in uniform registers (issued from a branch
+    // of lane 0 an MMA took about 120 cycles)
+    constexpr uint32_t id = kF8 ? idesc(0, PAGE, false) : idesc(1, PAGE, false);
+    const uint32_t tm = __shfl_sync(~0u, tmem, 0);
+    const uint64_t k_desc = desc_sw128(smem_u32(ring), 16, 1024);
     RingAt at{C::kStages};
-    int g = 0;
+    uint32_t piece = 0, n0 = 0, n1 = 0;        // pages of each group so far
     bool ok = true;
     while (ok && walk.next(p)) {
-      for (int i = p.p0; i < p.p1; ++i, ++g) {
-        const int vb = g & 3;
-        ok = wait.warp_wait(&sh.full[at.st], at.parity, 3, i);
-        if (ok && g >= kWideBufs) ok = wait.warp_wait(&sh.v_empty[vb], ((g >> 2) - 1) & 1, 3, i);
+      uint32_t good = spin(&sh.q_full, piece++ & 1, wait);
+      for (int i = 0; i < p.p1 - p.p0; ++i) {
+        const int w = i & 1;
+        const uint32_t before = w ? n1 : n0;
+        good &= spin(&sh.s_empty[w], (before & 1) ^ 1, wait) & spin(&sh.full[at.st], at.parity, wait);
+        ok = all_well(good, wait, 1, i);
         if (!ok) break;
-        const int left = p.total() - i * PAGE, own = p.ctx - i * PAGE;    // rows that exist, rows in front of the drafted ones
-        if (t < PAGE) {
-          float ks = sh.scales[at.st][0][t], vs = sh.scales[at.st][1][t];
-          float lg = log2f(fmaxf(vs, 0x1p-100f)), inv = __fdividef(1.f, fmaxf(vs, 0x1p-100f));
-          if (!(vs < INFINITY)) lg = vs, inv = 0.f;             // no number: whoever attends to it gets none either
-          if (t >= left) ks = lg = inv = 0.f;
-          sh.par[vb][t] = make_float4(ks, lg, inv, 0.f);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.par_full[vb]);
-        }
-        const uint8_t* src = ring + at.st * C::kStageBytes + C::kPageBytes;
-        uint8_t* dst = wide + vb * kWideBytes;
+        tc_fence_after();
+        const uint64_t k = k_desc + at.st * (C::kStageBytes >> 4);
+        const uint32_t d = tm + kColS + w * PAGE;
+        if (elect_one()) {
+          if constexpr (kF8) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = j * 16 + (t >> 3), piece = t & 7, sw = row & 7;
-          uint4 c = lds128(src + row * D + ((piece ^ sw) << 4));
-          if (row >= left) {
-            c = make_uint4(0, 0, 0, 0);
-          } else if (row >= own) {              // a drafted token's codes without a number: its scale says so
-            auto clean = [](uint32_t w) {
-              const uint32_t nan = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-              return w & ~((nan >> 7) * 0xFFu);
-            };
-            c = make_uint4(clean(c.x), clean(c.y), clean(c.z), clean(c.w));
-          }
-          uint32_t o[8];
-          const uint32_t in[4] = {c.x, c.y, c.z, c.w};
+            for (int j = 0; j < 8; ++j)        // the rows' upper parts, then their lower ones
+              umma_f8_ta(d, tm + kColQ + j * 8, k + (j & 3) * 2, id, j > 0);
+            umma_commit(&sh.s_full[w]);
+            umma_commit(&sh.empty[at.st]);
+          } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t h[2];
-            e4m3x4_to_half2(in[q], h);
-            o[2 * q] = h[0];
-            o[2 * q + 1] = h[1];
+            for (int j = 0; j < 8; ++j)
+              umma_bf16_ta(d, tm + kColQ + j * 8, k + (j >> 2) * (C::kPageBytes / 32) + (j & 3) * 2, id, j > 0);
+            umma_commit(&sh.s_full[w]);
           }
-          // sixteen values are two pieces of a half's row; lanes of the other half take them in the other order, for the banks' sake
-          uint8_t* to = dst + (piece >> 2) * (kWideBytes / 2) + row * 128;
-          const int lo = (((2 * piece) & 7) ^ sw) << 4, hi = (((2 * piece + 1) & 7) ^ sw) << 4;
-          const bool swap = piece >= 4;
-          const uint4 x = make_uint4(o[0], o[1], o[2], o[3]), y = make_uint4(o[4], o[5], o[6], o[7]);
-          *reinterpret_cast<uint4*>(to + (swap ? hi : lo)) = swap ? y : x;
-          *reinterpret_cast<uint4*>(to + (swap ? lo : hi)) = swap ? x : y;
         }
-        fence_proxy_async_smem();
+        __syncwarp();
+        n0 += 1 - w;
+        n1 += w;
+        at.next();
+      }
+    }
+  } else if (warp == C::kSumWarp) {
+    // ---- O += P V
+    constexpr uint32_t id = kF8 ? idesc(0, D, true) : idesc(1, D, true);
+    const uint32_t tm = __shfl_sync(~0u, tmem, 0);
+    const uint64_t v_desc = desc_sw128(kF8 ? smem_u32(wide) : smem_u32(ring) + C::kPageBytes, kWideBytes / 2, 1024);
+    RingAt at{C::kStages};
+    uint32_t n0 = 0, n1 = 0, g = 0;
+    bool ok = true;
+    while (ok && walk.next(p)) {
+      for (int i = 0; i < p.p1 - p.p0 && ok; ++i) {
+        const int w = i & 1;
+        uint32_t good = kF8 ? spin(&sh.v_full[g & 3], (g >> 2) & 1, wait) : 1u;
+        good &= spin(&sh.p_full[w], (w ? n1 : n0) & 1, wait);
+        ok = all_well(good, wait, 2, i);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t v = v_desc + (kF8 ? (g & 3) * (kWideBytes >> 4) : at.st * (C::kStageBytes >> 4));
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            umma_bf16_ta(tm + kColO + w * D, tm + kColP + w * 32 + j * 8, v + j * 128, id, i > 1 || j > 0);
+          umma_commit(&sh.o_done[w]);
+          umma_commit(kF8 ? &sh.v_empty[g & 3] : &sh.empty[at.st]);
+        }
+        __syncwarp();
+        n0 += 1 - w;
+        n1 += w;
+        ++g;
+        at.next();
+      }
+    }
+  } else if (kF8 && warp == C::kParWarp) {
+    // ---- scales to what the scores need
+    RingAt at{C::kStages};
+    uint32_t g = 0;
+    bool ok = true;
+    while (ok && walk.next(p)) {
+      for (int i = p.p0; i < p.p1 && ok; ++i, ++g) {
+        const int vb = g & 3, left = p.total() - i * PAGE;
+        // the page is there, and the weights that the place's last scales were for are made
+        ok = all_well(spin(&sh.full[at.st], at.parity, wait) & spin(&sh.v_empty[vb], ((g >> 2) & 1) ^ 1, wait), wait, 3, i);
+        if (!ok) break;
+        const float2 ks = reinterpret_cast<const float2*>(sh.scales[at.st][0])[lane], vs = reinterpret_cast<const float2*>(sh.scales[at.st][1])[lane];
+        auto par = [&](float& k, float v, float& lg, float& inv, int key) {
+          lg = log2f(fmaxf(v, 0x1p-100f));
+          inv = __fdividef(1.f, fmaxf(v, 0x1p-100f));
+          if (!(v < INFINITY)) lg = v, inv = 0.f;             // no number: whoever attends to it gets none either
+          if (key >= left) k = lg = inv = 0.f;
+        };
+        float2 k = ks, lg, inv;
+        par(k.x, vs.x, lg.x, inv.x, 2 * lane);
+        par(k.y, vs.y, lg.y, inv.y, 2 * lane + 1);
+        reinterpret_cast<float2*>(sh.par[vb][0])[lane] = k;
+        reinterpret_cast<float2*>(sh.par[vb][1])[lane] = lg;
+        reinterpret_cast<float2*>(sh.par[vb][2])[lane] = inv;
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&sh.v_full[vb]);
+          mbar_arrive(&sh.par_full[vb]);
           mbar_arrive(&sh.empty[at.st]);
         }
         at.next();
       }
     }
+  } else if (kF8 && warp >= kMathWarps) {
+    // ---- e4m3 values to f16; the next page's codes come into registers while this one's stores finish
+    const int t = tid - kMathWarps * 32, piece = t & 7, r0 = t >> 3, sw = r0 & 7;      // rows r0, r0 + 16, + 32, + 48
+    // sixteen values are two pieces of a half's row; lanes of the other half take them in the other order, for the banks' sake
+    const int from = r0 * D + ((piece ^ sw) << 4), to = (piece >> 2) * (kWideBytes / 2) + r0 * 128;
+    const int lo = to + ((((2 * piece) & 7) ^ sw) << 4), hi = to + ((((2 * piece + 1) & 7) ^ sw) << 4);
+    const bool swap = piece >= 4;
+    RingAt at{C::kStages};
+    uint4 code[4];
+    uint32_t good = 1;
+    int i = 0;
+    // the codes of the piece's page i: rows behind the sequence's end become zeros (a weight of zero would not do: zero times NaN),
+    // and so do drafted tokens' codes that are no numbers, whose scales say so
+    auto fetch = [&]() {
+      good = spin(&sh.full[at.st], at.parity, wait);
+      const uint8_t* src = ring + at.st * C::kStageBytes + C::kPageBytes + from;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) code[j] = *reinterpret_cast<const uint4*>(src + j * 16 * D);
+      const int left = p.total() - i * PAGE, own = p.ctx - i * PAGE;
+      if (own < PAGE) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = j * 16 + r0;
+          auto clean = [](uint32_t w) {
+            const uint32_t nan = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+            return w & ~((nan >> 7) * 0xFFu);
+          };
+          if (row >= left) code[j] = make_uint4(0, 0, 0, 0);
+          else if (row >= own) code[j] = make_uint4(clean(code[j].x), clean(code[j].y), clean(code[j].z), clean(code[j].w));
+        }
+      }
+    };
+    bool more = walk.next(p);
+    if (more) {
+      i = p.p0;
+      fetch();
+    }
+    for (uint32_t g = 0; more; ++g) {
+      const int vb = g & 3;
+      if (!all_well(good & spin(&sh.v_empty[vb], ((g >> 2) & 1) ^ 1, wait), wait, 3, i)) break;
+      uint8_t* dst = wide + vb * kWideBytes;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t x[4], y[4];
+        e4m3x4_to_half2(code[j].x, reinterpret_cast<uint32_t(&)[2]>(x[0]));
+        e4m3x4_to_half2(code[j].y, reinterpret_cast<uint32_t(&)[2]>(x[2]));
+        e4m3x4_to_half2(code[j].z, reinterpret_cast<uint32_t(&)[2]>(y[0]));
+        e4m3x4_to_half2(code[j].w, reinterpret_cast<uint32_t(&)[2]>(y[2]));
+        const uint4 first = make_uint4(x[0], x[1], x[2], x[3]), second = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(dst + j * 16 * 128 + (swap ? hi : lo)) = swap ? second : first;
+        *reinterpret_cast<uint4*>(dst + j * 16 * 128 + (swap ? lo : hi)) = swap ? first : second;
+      }
+      if (lane == 0) mbar_arrive(&sh.empty[at.st]);      // its codes are in registers: every lane's conversions used them
+      at.next();
+      if (++i == p.p1) {
+        more = walk.next(p);
+        i = p.p0;
+      }
+      if (more) fetch();
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.v_full[vb]);
+    }
+  }
   } else {
     // ---- scores to weights, sums to results
+    set_registers<C::kMathRegs, true>();
+    Walk walk(a, sh);
+    Piece p;
     const int w = warp >> 2, quarter = warp & 3;                       // group, lanes of tensor memory
     const uint32_t lanes = tmem + ((uint32_t)quarter << 21);
     const int slot = quarter * 32 + lane, tile_row = slot % kLive, key0 = (slot / kLive) * kKeys;
@@ -460,55 +570,62 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       tmem_st_wait();
     }
     int c = 0, g = 0, tails = 0;      // pages of this group, of the CTA, and last pages of this group
-    uint32_t piece = 0;
+    uint32_t* q_rows = reinterpret_cast<uint32_t*>(scratch);      // between pieces the scratch holds the next one's query rows
     while (walk.next(p)) {
       const int r = p.tile * kRows + tile_row, t = r / a.group;
       const bool live = r < rows && t < p.live;
       const int n = p.p1 - p.p0;
       bool failed = false;
-      if (w == 0) {
-        // the row into tensor memory
-        uint32_t q[64];
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + p.b * a.q_b + t * a.q_t +
-                                                          p.head * a.q_kv + (r % a.group) * a.q_g);
+      // the tile's rows: half a warp loads one, every copy of it goes from shared memory to its lane
+      {
+        const int sub = lane & 15;
+        const unsigned half = 0xFFFFu << (lane & 16);
         const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 2
+        for (int rr = warp * 2 + (lane >> 4); rr < kLive; rr += kMathWarps * 2) {
+          const int qr = p.tile * kRows + rr, qt = qr / a.group;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (qr < rows && qt < p.live)
+            v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + p.b * a.q_b + qt * a.q_t + p.head * a.q_kv +
+                                                     (qr % a.group) * a.q_g) + sub);
+          v.x ^= sign; v.y ^= sign; v.z ^= sign; v.w ^= sign;
+          uint32_t* to = q_rows + rr * kQRow;
+          if constexpr (!kF8) {
+            *reinterpret_cast<uint4*>(to + sub * 4) = v;
+          } else {
+            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+            uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint4 v = live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-          q[4 * i] = v.x ^ sign; q[4 * i + 1] = v.y ^ sign; q[4 * i + 2] = v.z ^ sign; q[4 * i + 3] = v.w ^ sign;
-        }
-        if constexpr (!kF8) {
-          tmem_store(lanes + kColQ, q);
-        } else {
-          uint32_t top = 0;
+            for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
 #pragma unroll
-          for (int i = 0; i < 64; ++i) top = max(top, max(q[i] & 0x7FFFu, (q[i] >> 16) & 0x7FFFu));
-          const int e = (int)(top >> 7);                              // exponent of the largest
-          // a power of two that takes the largest to [128, 256); rows of (nearly) nothing as they are
-          const int up = e == 0xFF ? 0 : min(126, 134 - max(e, 1));
-          const float mul = exp2f((float)up);
-          uint32_t part[32];
+            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(half, top, o));
+            const int e = (int)(top >> 7);                            // exponent of the largest
+            // a power of two that takes the largest to [128, 256); rows of (nearly) nothing as they are
+            const int up = e == 0xFF ? 0 : min(126, 134 - max(e, 1));
+            const float mul = exp2f((float)up);
+            uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
 #pragma unroll
-          for (int pass = 0; pass < 2; ++pass) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              uint32_t word = 0;
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float2 f = make_float2(bf_lo(q[2 * i + j]) * mul, bf_hi(q[2 * i + j]) * mul);
-                const uint32_t hi = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-                if (pass == 0) {
-                  word |= hi << (16 * j);
-                } else {
-                  const float2 h = e4m3x2_to_float2(hi);
-                  word |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f.x - h.x, f.y - h.y), __NV_SATFINITE, __NV_E4M3) << (16 * j);
-                }
-              }
-              part[i] = word;
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = make_float2(bf_lo(u[j]) * mul, bf_hi(u[j]) * mul);
+              const uint32_t c8 = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+              const float2 h = e4m3x2_to_float2(c8);
+              hi[j >> 1] |= c8 << (16 * (j & 1));
+              lo[j >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f.x - h.x, f.y - h.y), __NV_SATFINITE, __NV_E4M3) << (16 * (j & 1));
             }
-            tmem_store(lanes + kColQ + pass * 32, part);
+            *reinterpret_cast<uint2*>(to + sub * 2) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(to + 32 + sub * 2) = make_uint2(lo[0], lo[1]);
+            if (sub == 0) sh.q_mul[rr] = e == 0xFF ? NAN : exp2f((float)-up);
           }
-          sh.q_mul[slot] = e == 0xFF ? NAN : exp2f((float)-up);
+        }
+      }
+      math_sync();
+      if (w == 0) {
+#pragma unroll
+        for (int j = 0; j < 64; j += 16) {
+          uint32_t q[16];
+#pragma unroll
+          for (int k = 0; k < 16; k += 4) *reinterpret_cast<uint4*>(q + k) = *reinterpret_cast<const uint4*>(q_rows + tile_row * kQRow + j + k);
+          tmem_store(lanes + kColQ + j, q);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -517,53 +634,43 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       }
       // the sequence's whole page table: a page outside the pool leaves the sequence out, in every piece alike
       bool bad = false;
-      for (int i = tid; i < p.np; i += kMathWarps * 32) {
-        const int id = __ldg(reinterpret_cast<const int*>(a.pages) + p.b * a.pages_b + i);
-        if (id < 0 || id >= a.cache.n_pages) {
-          bad = true;
-          report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, p.b, id);
+      if (w == 1) {
+        for (int i0 = tid - 128; i0 < p.np; i0 += 128 * 8) {
+          int id[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) id[j] = i0 + 128 * j < p.np ? __ldg(reinterpret_cast<const int*>(a.pages) + p.b * a.pages_b + i0 + 128 * j) : 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (id[j] < 0 || id[j] >= a.cache.n_pages) {
+              bad = true;
+              report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, p.b, id[j]);
+            }
         }
       }
       float row_scale = scale;
-      if constexpr (kF8) {
-        failed = !wait.warp_wait(&sh.q_full, piece & 1, 4, -1);
-        row_scale = scale * sh.q_mul[slot];
-      }
-      ++piece;
-
+      if constexpr (kF8) row_scale *= sh.q_mul[tile_row];
       float m = -INFINITY, l = 0.f;
-      for (int i = 0; i < n && !failed; ++i, ++g) {
-        if ((i & 1) != w) continue;
+      for (int i = w; i < n; i += 2) {
+        const uint32_t gi = g + i;                  // the page among the CTA's
         const int page = p.p0 + i;
+        uint32_t good = spin(&sh.s_full[w], c & 1, wait);
         const bool tail = (page + 1) * PAGE > p.ctx;
         uint64_t bits = ~0ull;
         if (tail) bits = live ? seen_bits(a, p, page, t) : 0;
         uint32_t raw[kKeys];
-        if (!wait.warp_wait(&sh.s_full[w], c & 1, 4, i)) {
-          failed = true;
-          break;
-        }
         tc_fence_after();
         tmem_load(lanes + kColS + w * PAGE + key0, raw);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.s_empty[w]);
         float s[kKeys];
-        if constexpr (kF8) {
-          if (!wait.warp_wait(&sh.par_full[g & 3], (g >> 2) & 1, 4, i)) {
-            failed = true;
-            break;
-          }
-        }
+        if constexpr (kF8) good &= spin(&sh.par_full[gi & 3], (gi >> 2) & 1, wait);
         uint64_t poison = 0;
         if (tail && !kF8) {
           // values behind the sequence's end become zeros (a weight of zero would not do: zero times NaN); so do drafted tokens'
           // that are no numbers, whose readers get none by their scores
-          const int st = g % C::kStages;
-          if (!wait.warp_wait(&sh.full[st], (g / C::kStages) & 1, 4, i)) {
-            failed = true;
-            break;
-          }
+          const int st = gi % C::kStages;
+          good &= spin(&sh.full[st], (gi / C::kStages) & 1, wait);
           const int row = (tid & 127) >> 1, key = page * PAGE + row;
           uint4* v = reinterpret_cast<uint4*>(ring + st * C::kStageBytes + C::kPageBytes + (tid & 1) * (C::kPageBytes / 2) + row * 128);
           bool none = key >= p.total();
@@ -585,10 +692,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
           if (quarter == 0 && lane < 2) sh.poison[w][(tails + 2) & 3][lane] = 0;
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.tail[w]);
-          if (!wait.warp_wait(&sh.tail[w], tails & 1, 4, i)) {
-            failed = true;
-            break;
-          }
+          good &= spin(&sh.tail[w], tails & 1, wait);
           volatile uint32_t* po = sh.poison[w][tails & 3];
           poison = (uint64_t)po[1] << 32 | po[0];
           ++tails;
@@ -596,10 +700,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
 #pragma unroll
         for (int j = 0; j < kKeys; ++j) {
           s[j] = __uint_as_float(raw[j]);
-          if constexpr (kF8) {
-            const float4 k = sh.par[g & 3][key0 + j];
-            s[j] = fmaf(s[j] * k.x, row_scale, k.y);
-          }
+          if constexpr (kF8) s[j] = fmaf(s[j] * sh.par[gi & 3][0][key0 + j], row_scale, sh.par[gi & 3][1][key0 + j]);
         }
         if (tail) {
           bits >>= key0;
@@ -615,7 +716,8 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         for (int j = 0; j < kKeys; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if constexpr (!kF8) top *= row_scale;
-        if (c > 0 && !wait.warp_wait(&sh.o_done[w], (c - 1) & 1, 4, i)) {
+        good &= spin(&sh.o_done[w], (c & 1) ^ 1, wait);      // the page before: its weights are read, its sums complete
+        if (!all_well(good, wait, 4, i)) {
           failed = true;
           break;
         }
@@ -643,8 +745,8 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
           const float p0 = kF8 ? exp2_ftz(s[j] - ref) : exp2_ftz(fmaf(s[j], row_scale, -ref));
           const float p1 = kF8 ? exp2_ftz(s[j + 1] - ref) : exp2_ftz(fmaf(s[j + 1], row_scale, -ref));
           if constexpr (kF8) {
-            sum[j & 3] = fmaf(p0, sh.par[g & 3][key0 + j].z, sum[j & 3]);
-            sum[(j + 1) & 3] = fmaf(p1, sh.par[g & 3][key0 + j + 1].z, sum[(j + 1) & 3]);
+            sum[j & 3] = fmaf(p0, sh.par[gi & 3][2][key0 + j], sum[j & 3]);
+            sum[(j + 1) & 3] = fmaf(p1, sh.par[gi & 3][2][key0 + j + 1], sum[(j + 1) & 3]);
             const __half2 h = __floats2half2_rn(p0, p1);
             pk[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
           } else {
@@ -662,7 +764,8 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         ++c;
       }
       const bool has = n > w;                  // this group had pages
-      if (!failed && has && !wait.warp_wait(&sh.o_done[w], (c - 1) & 1, 5, n)) failed = true;
+      g += n;
+      if (!failed && has) failed = !all_well(spin(&sh.o_done[w], (c & 1) ^ 1, wait), wait, 5, n);
       sh.stats[warp][lane] = make_float2(m, l);
       if (math_any(failed)) break;
       bad = math_any(bad);
@@ -738,7 +841,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
   tc_fence_before();
   __syncthreads();
   wait.drain();
-  if (warp == C::kMmaWarp) {
+  if (warp == C::kScoreWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, kCols);
   }
