@@ -35,16 +35,16 @@ struct Cfg {
   static constexpr int kPageBytes = PAGE * D * (kF8 ? 1 : 2);
   static constexpr int kStageBytes = 2 * kPageBytes;
   static constexpr int kTx = kStageBytes + (kF8 ? 2 * PAGE * 4 : 0);
-  static constexpr int kWideWarps = kF8 ? 4 : 0;
+  static constexpr int kWideTeams = 2, kWideWarps = kF8 ? 4 * kWideTeams : 0;
   static constexpr int kLoadWarp = kMathWarps + kWideWarps, kScoreWarp = kLoadWarp + 1, kSumWarp = kLoadWarp + 2, kParWarp = kLoadWarp + 3;
-  static constexpr int kThreads = kF8 ? 512 : 384;        // whole groups of four warps
-  // registers of a thread: at launch, then of the math warps and of the others (512 * 128 = 256 * 168 + 256 * 88, 384 * 168 =
+  static constexpr int kThreads = kF8 ? 640 : 384;        // whole groups of four warps
+  // registers of a thread: at launch (640 * 96, 384 * 168), then of the math warps and of the others (256 * 144 + 384 * 64,
   // 256 * 208 + 128 * 88)
-  static constexpr int kMathRegs = kF8 ? 168 : 208, kOtherRegs = 88;
+  static constexpr int kMathRegs = kF8 ? 144 : 208, kOtherRegs = kF8 ? 64 : 88;
   static constexpr float kSlack = kF8 ? 4.f : 8.f;      // powers of two by which a score may exceed its row's reference
   static constexpr float kLift = kF8 ? 11.f : 0.f;      // f16 weights are kept that much larger: 2^15 at most, 2^-25 of the largest with all bits
 };
-constexpr int kWideBufs = 4, kWideBytes = PAGE * D * 2;
+constexpr int kSeqs = 512, kWideBufs = 4, kWideBytes = PAGE * D * 2;
 constexpr int kScratchRow = 36;                         // floats of a row's 32 sums on their way between warps
 constexpr int kScratch = kMathWarps * 32 * kScratchRow * 4;
 constexpr int kQRow = 68;                               // words of a query row on its way to tensor memory: 256 bytes, apart for the banks' sake
@@ -59,35 +59,41 @@ struct TreeShared {
   volatile int fail;
   int first_b;
   long long begin, end, first_base;
+  int2 seq[kSeqs];                    // rows and drafted tokens of the first sequences
+  int bad[2];
   uint32_t poison[2][4][2];
   float q_mul[kRows];
   float2 stats[kMathWarps][32];       // of the rows on a warp's lanes: reference, sum of weights
-  float2 row[kRows];                  // of a row over all its copies: the same
   alignas(16) float par[kWideBufs][3][PAGE];   // of the keys of an e4m3 page: scale, log2 of the value's, 1 / the value's
   alignas(16) float scales[8][2][PAGE];
 };
 
-// Pages of sequence b (0 where there is nothing to compute, or something is wrong).
-__device__ __forceinline__ int seq_pages(const vdc_tree_attention_args& a, int b, int& ctx, int& live, bool* wrong = nullptr) {
-  ctx = __ldg(reinterpret_cast<const int*>(a.lengths) + b);
-  live = a.counts ? max(0, min(a.T, __ldg(reinterpret_cast<const int*>(a.counts) + b))) : a.T;
-  const int64_t keys = (int64_t)ctx + live;
-  const bool bad = ctx < 0 || keys > (int64_t)a.max_pages * PAGE;
-  if (wrong) *wrong = bad;
-  return bad || live == 0 ? 0 : (int)((keys + PAGE - 1) / PAGE);
+// Rows and drafted tokens of sequence b: x = the rows, negative where they or the drafted ones do not fit the page table.
+__device__ __forceinline__ int2 seq_load(const vdc_tree_attention_args& a, int b) {
+  const int ctx = __ldg(reinterpret_cast<const int*>(a.lengths) + b);
+  const int live = a.counts ? max(0, min(a.T, __ldg(reinterpret_cast<const int*>(a.counts) + b))) : a.T;
+  return make_int2(ctx < 0 || (int64_t)ctx + live > (int64_t)a.max_pages * PAGE ? -1 : ctx, live);
+}
+__device__ __forceinline__ int pages_of(int2 seq) {      // 0 where there is nothing to compute
+  return seq.x < 0 || seq.y == 0 ? 0 : (int)(((int64_t)seq.x + seq.y + PAGE - 1) / PAGE);
+}
+__device__ __forceinline__ int2 seq_of(const vdc_tree_attention_args& a, const TreeShared& sh, int b) {
+  return b < kSeqs ? sh.seq[b] : seq_load(a, b);
 }
 
-__device__ __forceinline__ int tiles_of(const vdc_tree_attention_args& a) { return (a.T * a.group + kRows - 1) / kRows; }
+__host__ __device__ __forceinline__ int tiles_of(const vdc_tree_attention_args& a) { return (a.T * a.group + kRows - 1) / kRows; }
 
-// A warp adds up the pages of all sequences.
-__device__ __forceinline__ long long all_pages(const vdc_tree_attention_args& a, int lane) {
-  long long n = 0;
-  int ctx, live;
-  for (int b = lane; b < a.B; b += 32) n += seq_pages(a, b, ctx, live);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
-  return n;
-}
+// Query row -> token and head of its group (rows are few enough for the reciprocal to be exact).
+struct RowOf {
+  uint32_t mul;
+  int group;
+  __device__ __forceinline__ explicit RowOf(int g) : mul(g == 1 ? 0u : 0xFFFFFFFFu / (uint32_t)g + 1u), group(g) {}
+  __device__ __forceinline__ int token(int r) const { return mul ? (int)__umulhi((uint32_t)r, mul) : r; }
+  __device__ __forceinline__ int64_t at(int r, int64_t per_token, int64_t per_head) const {
+    const int t = token(r);
+    return t * per_token + (r - t * group) * per_head;
+  }
+};
 
 struct Piece {
   int b, head, tile, p0, p1, np, ctx, live;
@@ -98,24 +104,28 @@ struct Piece {
 // The pieces of a CTA, in order; every role walks them by itself.
 struct Walk {
   const vdc_tree_attention_args& a;
+  const TreeShared& sh;
   long long x, end, base;     // place among all units' pages, its end, where sequence b begins
   int b;
-  __device__ __forceinline__ Walk(const vdc_tree_attention_args& a_, const TreeShared& sh)
-      : a(a_), x(sh.begin), end(sh.end), base(sh.first_base), b(sh.first_b) {}
+  __device__ __forceinline__ Walk(const vdc_tree_attention_args& a_, const TreeShared& sh_)
+      : a(a_), sh(sh_), x(sh_.begin), end(sh_.end), base(sh_.first_base), b(sh_.first_b) {}
   __device__ __forceinline__ bool next(Piece& p) {
     if (x >= end) return false;
     const int tiles = tiles_of(a), units = a.cache.n_kv * tiles;
     for (;; ++b) {
       if (b >= a.B) return false;
-      p.np = seq_pages(a, b, p.ctx, p.live);
+      const int2 seq = seq_of(a, sh, b);
+      p.ctx = seq.x;
+      p.live = seq.y;
+      p.np = pages_of(seq);
       if (x < base + (long long)p.np * units) break;
       base += (long long)p.np * units;
     }
     const int u = (int)((x - base) / p.np);
     p.b = b;
-    p.head = u / tiles;
-    p.tile = u % tiles;
-    p.p0 = (int)((x - base) % p.np);
+    p.head = tiles == 1 ? u : u / tiles;
+    p.tile = tiles == 1 ? 0 : u % tiles;
+    p.p0 = (int)(x - base - (long long)u * p.np);
     p.p1 = (int)min((long long)p.np, p.p0 + (end - x));
     x += p.p1 - p.p0;
     return true;
@@ -267,8 +277,8 @@ __host__ __device__ __forceinline__ long long record_floats(const vdc_tree_atten
   return ((long long)(rows < kRows ? rows : kRows) * (D + 2) + 3) & ~3ll;
 }
 
-__device__ __forceinline__ __nv_bfloat16* out_row(const vdc_tree_attention_args& a, int b, int head, int r) {
-  return reinterpret_cast<__nv_bfloat16*>(a.out) + b * a.o_b + (r / a.group) * a.o_t + head * a.o_kv + (r % a.group) * a.o_g;
+__device__ __forceinline__ __nv_bfloat16* out_row(const vdc_tree_attention_args& a, const RowOf& of, int b, int head, int r) {
+  return reinterpret_cast<__nv_bfloat16*>(a.out) + b * a.o_b + head * a.o_kv + of.at(r, a.o_t, a.o_g);
 }
 
 template <bool kF8, int kReps>
@@ -285,12 +295,14 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
   const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
   const Waiter wait{&sh.fail, status, timeout_ns, VDC_TREE_ATTENTION_KIND};
 
+  grid_dep_launch();
   if (warp == C::kScoreWarp) tmem_alloc(&sh.tmem, kCols);
+  for (int b = tid; b < min(a.B, kSeqs); b += C::kThreads) sh.seq[b] = seq_load(a, b);
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < C::kStages; ++i) {
         mbar_init(&sh.full[i], 1);
-        mbar_init(&sh.empty[i], kF8 ? 1 + C::kWideWarps + 1 : 1);
+        mbar_init(&sh.empty[i], kF8 ? 1 + 4 + 1 : 1);       // the scores; a team that widens; the scales
       }
       mbar_init(&sh.q_full, 4);
       for (int i = 0; i < 2; ++i) {
@@ -309,15 +321,29 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (lane < 16) reinterpret_cast<uint32_t*>(sh.poison)[lane] = 0;
+    if (lane < 2) sh.bad[lane] = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int rows = a.T * a.group;
+  const RowOf row_of(a.group);
+  if (warp == 0) {
     // this CTA's share of all units' pages, and the sequence it begins in
-    const long long units = (long long)a.cache.n_kv * tiles_of(a), total = all_pages(a, lane) * units;
+    const long long units = (long long)a.cache.n_kv * tiles_of(a);
+    long long total = 0;
+    for (int b = lane; b < a.B; b += 32) total += pages_of(seq_of(a, sh, b));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+    total *= units;
     const long long ctas = min((long long)gridDim.x, max(total, 1ll)), me = min((long long)blockIdx.x, ctas);    // a page each at least
     const long long begin = total * me / ctas, end = total * min(me + 1, ctas) / ctas;
     long long base = 0;
     int first = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
-      int ctx, live;
-      long long n = b0 + lane < a.B ? seq_pages(a, b0 + lane, ctx, live) * units : 0, sum = n;
+      const long long n = b0 + lane < a.B ? pages_of(seq_of(a, sh, b0 + lane)) * units : 0;
+      long long sum = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long below = __shfl_up_sync(~0u, sum, o);
@@ -339,11 +365,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       sh.first_b = first;
     }
   }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = sh.tmem;
-  const int rows = a.T * a.group;
 
   if (warp >= kMathWarps) {
     set_registers<C::kOtherRegs, false>();
@@ -491,21 +513,22 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       }
     }
   } else if (kF8 && warp >= kMathWarps) {
-    // ---- e4m3 values to f16; the next page's codes come into registers while this one's stores finish
-    const int t = tid - kMathWarps * 32, piece = t & 7, r0 = t >> 3, sw = r0 & 7;      // rows r0, r0 + 16, + 32, + 48
+    // ---- e4m3 values to f16, by two teams of four warps that take the pages in turn; a team's next codes come into registers
+    // while its stores finish
+    const int t = tid & 127, piece = t & 7, r0 = t >> 3, sw = r0 & 7;      // rows r0, r0 + 16, + 32, + 48
     // sixteen values are two pieces of a half's row; lanes of the other half take them in the other order, for the banks' sake
     const int from = r0 * D + ((piece ^ sw) << 4), to = (piece >> 2) * (kWideBytes / 2) + r0 * 128;
     const int lo = to + ((((2 * piece) & 7) ^ sw) << 4), hi = to + ((((2 * piece + 1) & 7) ^ sw) << 4);
     const bool swap = piece >= 4;
-    RingAt at{C::kStages};
     uint4 code[4];
-    uint32_t good = 1;
+    uint32_t good = 1, g = (warp - kMathWarps) >> 2;     // the page among the CTA's
     int i = 0;
     // the codes of the piece's page i: rows behind the sequence's end become zeros (a weight of zero would not do: zero times NaN),
     // and so do drafted tokens' codes that are no numbers, whose scales say so
     auto fetch = [&]() {
-      good = spin(&sh.full[at.st], at.parity, wait);
-      const uint8_t* src = ring + at.st * C::kStageBytes + C::kPageBytes + from;
+      const uint32_t st = g % C::kStages;
+      good = spin(&sh.full[st], (g / C::kStages) & 1, wait);
+      const uint8_t* src = ring + st * C::kStageBytes + C::kPageBytes + from;
 #pragma unroll
       for (int j = 0; j < 4; ++j) code[j] = *reinterpret_cast<const uint4*>(src + j * 16 * D);
       const int left = p.total() - i * PAGE, own = p.ctx - i * PAGE;
@@ -522,12 +545,22 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         }
       }
     };
+    // i += n in the walk's pages; false at their end
+    auto ahead = [&](int n) {
+      for (i += n; i >= p.p1;) {
+        const int over = i - p.p1;
+        if (!walk.next(p)) return false;
+        i = p.p0 + over;
+      }
+      return true;
+    };
     bool more = walk.next(p);
     if (more) {
       i = p.p0;
-      fetch();
+      more = ahead((int)g);
     }
-    for (uint32_t g = 0; more; ++g) {
+    if (more) fetch();
+    while (more) {
       const int vb = g & 3;
       if (!all_well(good & spin(&sh.v_empty[vb], ((g >> 2) & 1) ^ 1, wait), wait, 3, i)) break;
       uint8_t* dst = wide + vb * kWideBytes;
@@ -542,16 +575,15 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         *reinterpret_cast<uint4*>(dst + j * 16 * 128 + (swap ? hi : lo)) = swap ? second : first;
         *reinterpret_cast<uint4*>(dst + j * 16 * 128 + (swap ? lo : hi)) = swap ? first : second;
       }
-      if (lane == 0) mbar_arrive(&sh.empty[at.st]);      // its codes are in registers: every lane's conversions used them
-      at.next();
-      if (++i == p.p1) {
-        more = walk.next(p);
-        i = p.p0;
-      }
-      if (more) fetch();
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.v_full[vb]);
+      if (lane == 0) {
+        mbar_arrive(&sh.v_full[vb]);
+        mbar_arrive(&sh.empty[g % C::kStages]);
+      }
+      g += C::kWideTeams;
+      more = ahead(C::kWideTeams);
+      if (more) fetch();
     }
   }
   } else {
@@ -571,8 +603,8 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
     }
     int c = 0, g = 0, tails = 0;      // pages of this group, of the CTA, and last pages of this group
     uint32_t* q_rows = reinterpret_cast<uint32_t*>(scratch);      // between pieces the scratch holds the next one's query rows
-    while (walk.next(p)) {
-      const int r = p.tile * kRows + tile_row, t = r / a.group;
+    for (int turn = 0; walk.next(p); ++turn) {
+      const int r = p.tile * kRows + tile_row, t = row_of.token(r);
       const bool live = r < rows && t < p.live;
       const int n = p.p1 - p.p0;
       bool failed = false;
@@ -581,13 +613,13 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         const int sub = lane & 15;
         const unsigned half = 0xFFFFu << (lane & 16);
         const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll 2
+#pragma unroll
         for (int rr = warp * 2 + (lane >> 4); rr < kLive; rr += kMathWarps * 2) {
-          const int qr = p.tile * kRows + rr, qt = qr / a.group;
+          const int qr = p.tile * kRows + rr;
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (qr < rows && qt < p.live)
-            v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + p.b * a.q_b + qt * a.q_t + p.head * a.q_kv +
-                                                     (qr % a.group) * a.q_g) + sub);
+          if (qr < rows && row_of.token(qr) < p.live)
+            v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + p.b * a.q_b + p.head * a.q_kv +
+                                                     row_of.at(qr, a.q_t, a.q_g)) + sub);
           v.x ^= sign; v.y ^= sign; v.z ^= sign; v.w ^= sign;
           uint32_t* to = q_rows + rr * kQRow;
           if constexpr (!kF8) {
@@ -633,7 +665,6 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         if (lane == 0) mbar_arrive(&sh.q_full);
       }
       // the sequence's whole page table: a page outside the pool leaves the sequence out, in every piece alike
-      bool bad = false;
       if (w == 1) {
         for (int i0 = tid - 128; i0 < p.np; i0 += 128 * 8) {
           int id[8];
@@ -642,7 +673,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             if (id[j] < 0 || id[j] >= a.cache.n_pages) {
-              bad = true;
+              sh.bad[turn & 1] = 1;
               report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, p.b, id[j]);
             }
         }
@@ -716,17 +747,13 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         for (int j = 0; j < kKeys; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if constexpr (!kF8) top *= row_scale;
-        good &= spin(&sh.o_done[w], (c & 1) ^ 1, wait);      // the page before: its weights are read, its sums complete
-        if (!all_well(good, wait, 4, i)) {
-          failed = true;
-          break;
-        }
-        tc_fence_after();
         if (__any_sync(~0u, top > m + C::kSlack)) {
           const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : exp2_ftz(m - m2);
           l *= f;
           m = m2;
           if (i > 1) {
+            good &= spin(&sh.o_done[w], (c & 1) ^ 1, wait);
+            tc_fence_after();
 #pragma unroll
             for (int j = 0; j < D; j += 32) {
               uint32_t o[32];
@@ -756,6 +783,12 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
           }
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // the page before: its weights are read, its sums complete
+        if (!all_well(good & spin(&sh.o_done[w], (c & 1) ^ 1, wait), wait, 4, i)) {
+          failed = true;
+          break;
+        }
+        tc_fence_after();
         tmem_store(lanes + kColP + w * 32 + key0 / 2, pk);
         tmem_st_wait();
         tc_fence_before();
@@ -768,75 +801,75 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       if (!failed && has) failed = !all_well(spin(&sh.o_done[w], (c & 1) ^ 1, wait), wait, 5, n);
       sh.stats[warp][lane] = make_float2(m, l);
       if (math_any(failed)) break;
-      bad = math_any(bad);
-      // ---- the row's copies meet: reference and sum of weights first, then 32 columns at a time
-      if (tid < kLive) {
-        float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-        for (int k = 0; k < 2 * kReps; ++k) mm = fmaxf(mm, sh.stats[(k / kReps) * 4 + (k % kReps) * (4 / kReps) + (tid >> 5)][lane].x);
+      // ---- the row's copies meet: statistics first (every copy looks at all), then 32 columns at a time
+      float mm = -INFINITY, ll = 0.f;
+      {
+        float2 st[2 * kReps];
 #pragma unroll
         for (int k = 0; k < 2 * kReps; ++k) {
-          const float2 st = sh.stats[(k / kReps) * 4 + (k % kReps) * (4 / kReps) + (tid >> 5)][lane];
-          // a copy that saw nothing has no weight; one without a number passes that on
-          ll += st.x == -INFINITY && st.y == 0.f ? 0.f : st.x == -INFINITY ? st.y : st.y * exp2_ftz(st.x - mm);
+          st[k] = sh.stats[(k / kReps) * 4 + (k % kReps) * (4 / kReps) + (tile_row >> 5)][lane];
+          mm = fmaxf(mm, st[k].x);
         }
-        if (bad || !live) mm = -INFINITY, ll = 0.f;
-        sh.row[tid] = make_float2(mm, ll);
+        // a copy that saw nothing has no weight; one without a number passes that on
+#pragma unroll
+        for (int k = 0; k < 2 * kReps; ++k) ll += st[k].y * (st[k].x == -INFINITY ? 1.f : exp2_ftz(st[k].x - mm));
       }
-      math_sync();
-      const float2 all = sh.row[tile_row];
-      const bool none = !has || all.y == 0.f || (m == -INFINITY && l == 0.f);
-      const float f = m == -INFINITY ? 1.f : exp2_ftz(m - all.x);
-      const bool whole = p.whole();
+      if (sh.bad[turn & 1] || !live) mm = -INFINITY, ll = 0.f;
+      const bool whole = p.whole(), none = !has || ll == 0.f || (m == -INFINITY && l == 0.f);
+      const float f = (m == -INFINITY ? 1.f : exp2_ftz(m - mm)) * (whole && ll != 0.f ? 1.f / ll : 1.f);
       float* rec = reinterpret_cast<float*>(a.work) + (2 * blockIdx.x + (p.p1 == p.np ? 0 : 1)) * record_floats(a);
-      const int rec_rows = min(rows, kRows), tile_rows = min(rows - p.tile * kRows, kRows);
+      const int tile_rows = min(rows - p.tile * kRows, kRows);
+      if (!whole && tid < min(kLive, tile_rows)) *reinterpret_cast<float2*>(rec + min(rows, kRows) * D + 2 * tid) = make_float2(mm, ll);
+      __nv_bfloat16* to[kLive / 32];
+#pragma unroll
+      for (int k = 0; k < kLive / 32; ++k) {
+        const int rr = (tid >> 3) + k * 32;
+        to[k] = out_row(a, row_of, p.b, p.head, p.tile * kRows + rr) + (tid & 7) * 4;
+      }
       tc_fence_after();
+      float* mine = scratch + (warp * 32 + lane) * kScratchRow;
+      const float* theirs = scratch + (tid >> 3) * kScratchRow + (tid & 7) * 4;
 #pragma unroll 1
       for (int col = 0; col < D; col += 32) {
         uint32_t o[32];
         if (has) tmem_load(lanes + kColO + w * D + col, o);
-        float* row = scratch + (warp * 32 + lane) * kScratchRow;
+        if (tile_row < tile_rows) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<float4*>(row + j) = none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                     : make_float4(__uint_as_float(o[j]) * f, __uint_as_float(o[j + 1]) * f,
-                                                                   __uint_as_float(o[j + 2]) * f, __uint_as_float(o[j + 3]) * f);
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(mine + j) = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                        : make_float4(__uint_as_float(o[j]) * f, __uint_as_float(o[j + 1]) * f,
+                                                                      __uint_as_float(o[j + 2]) * f, __uint_as_float(o[j + 3]) * f);
+        }
         math_sync();
 #pragma unroll
         for (int k = 0; k < kLive / 32; ++k) {
-          const int rr = (tid >> 3) + k * 32, c4 = (tid & 7) * 4;
+          const int rr = (tid >> 3) + k * 32;
           if (rr < tile_rows) {
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int q = 0; q < 2 * kReps; ++q) {
-              const int from = (q / kReps) * 4 + (q % kReps) * (4 / kReps) + (rr >> 5);
-              const float4 x = *reinterpret_cast<const float4*>(scratch + (from * 32 + (rr & 31)) * kScratchRow + c4);
+              const int from = (q / kReps) * 4 + (q % kReps) * (4 / kReps) + k;
+              const float4 x = *reinterpret_cast<const float4*>(theirs + from * 32 * kScratchRow);
               sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
             }
-            if (whole) {
-              const float ll = sh.row[rr].y, inv = ll == 0.f ? 0.f : 1.f / ll;
-              *reinterpret_cast<uint2*>(out_row(a, p.b, p.head, p.tile * kRows + rr) + col + c4) =
-                  make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
-            } else {
-              *reinterpret_cast<float4*>(rec + rr * D + col + c4) = sum;
-            }
+            if (whole) *reinterpret_cast<uint2*>(to[k] + col) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+            else *reinterpret_cast<float4*>(rec + rr * D + col + (tid & 7) * 4) = sum;
           }
         }
         math_sync();
       }
-      if (!whole && tid < tile_rows) *reinterpret_cast<float2*>(rec + rec_rows * D + 2 * tid) = sh.row[tid];
+      if (tid == 0) sh.bad[turn & 1] = 0;
       tc_fence_before();
     }
   }
   // sequences without anything to attend with, or that do not fit their tables, get zeros
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    int ctx, live;
-    bool wrong;
-    if (seq_pages(a, b, ctx, live, &wrong)) continue;
-    if (wrong && tid == 0) report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 0, b, ctx);
+    const int2 seq = seq_of(a, sh, b);
+    if (pages_of(seq)) continue;
+    if (seq.x < 0 && tid == 0) report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 0, b, __ldg(reinterpret_cast<const int*>(a.lengths) + b));
     const int heads = a.cache.n_kv, n = rows * heads * (D / 8);
     for (int i = tid; i < n; i += C::kThreads)
-      *reinterpret_cast<uint4*>(out_row(a, b, (i / (D / 8)) % heads, i / (D / 8) / heads) + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(out_row(a, row_of, b, (i / (D / 8)) % heads, i / (D / 8) / heads) + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
   }
   tc_fence_before();
   __syncthreads();
@@ -850,42 +883,68 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
 // Joins the pieces of units that several CTAs shared: a warp per row, lane i the values 4i .. 4i + 3.  Pieces are taken in order,
 // so that the result does not depend on when they came.
 constexpr int kJoinWarps = 4;
-__global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_constant__ vdc_tree_attention_args a, int ctas, vdc_status* status) {
-  grid_dep_wait();
-  const int lane = threadIdx.x & 31, rr = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
-  const int tiles = tiles_of(a), units = a.cache.n_kv * tiles, b = blockIdx.x / units, u = blockIdx.x % units;
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_constant__ vdc_tree_attention_args a, int ctas) {
+  __shared__ long long part[2][kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rr = blockIdx.y * kJoinWarps + warp;
+  const int tiles = tiles_of(a), units = a.cache.n_kv * tiles, b = blockIdx.x / units, u = blockIdx.x - b * units;
   const int rows = a.T * a.group, r = (u % tiles) * kRows + rr, rec_rows = min(rows, kRows);
-  int ctx, live;
-  const int np = seq_pages(a, b, ctx, live);
-  if (np == 0) return;
-  long long before = 0;
-  for (int i = lane; i < b; i += 32) {
-    int c2, l2;
-    before += seq_pages(a, i, c2, l2);
+  grid_dep_wait();
+  // pages of all sequences and of those in front of this one
+  const int2 seq = seq_load(a, b);
+  long long total = 0, before = 0;
+  for (int i = threadIdx.x; i < a.B; i += kJoinWarps * 32) {
+    const int n = pages_of(seq_load(a, i));
+    total += n;
+    before += i < b ? n : 0;
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
-  const long long total = all_pages(a, lane) * units, first = before * units + (long long)u * np;
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(~0u, total, o);
+    before += __shfl_xor_sync(~0u, before, o);
+  }
+  if (lane == 0) part[0][warp] = total, part[1][warp] = before;
+  __syncthreads();
+  total = before = 0;
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) total += part[0][i], before += part[1][i];
+  const int np = pages_of(seq);
+  if (np == 0 || r >= rows || rr >= kRows) return;
+  total *= units;
+  const long long first = before * units + (long long)u * np;
   ctas = (int)min((long long)ctas, total);
   const int c0 = (int)(((first + 1) * ctas - 1) / total), c1 = (int)(((first + np) * ctas - 1) / total);
-  if (c0 == c1 || r >= rows || rr >= kRows) return;
+  if (c0 == c1) return;
   const long long rec = record_floats(a);
   auto record = [&](int c) { return reinterpret_cast<const float*>(a.work) + (2ll * c + (c == c1 ? 0 : 1)) * rec; };
-  float m = -INFINITY, l = 0.f;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, __ldg(record(c) + rec_rows * D + 2 * rr));
+  auto stats = [&](int c) { return __ldg(reinterpret_cast<const float2*>(record(c) + rec_rows * D + 2 * rr)); };
+  float2 st = c0 + lane <= c1 ? stats(c0 + lane) : make_float2(-INFINITY, 0.f);
+  float m = st.x;
+  for (int c = c0 + 32 + lane; c <= c1; c += 32) m = fmaxf(m, stats(c).x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-  for (int c = c0; c <= c1; ++c) {
-    const float* p = record(c);
-    const float2 st = *reinterpret_cast<const float2*>(p + rec_rows * D + 2 * rr);
-    const float4 x = *reinterpret_cast<const float4*>(p + rr * D + lane * 4);
-    const float f = st.x == -INFINITY ? 1.f : exp2_ftz(st.x - m);      // no reference: nothing, or no number
-    l += st.y * f;
-    sum.x += x.x * f; sum.y += x.y * f; sum.z += x.z * f; sum.w += x.w * f;
+  float l = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = c0; c <= c1; c += 32) {
+    if (c > c0) st = c + lane <= c1 ? stats(c + lane) : make_float2(-INFINITY, 0.f);
+    const float mine = st.x == -INFINITY ? 1.f : exp2_ftz(st.x - m);      // no reference: nothing, or no number
+    l += st.y * mine;
+    const int n = min(32, c1 - c + 1);
+    for (int i = 0; i < n; i += 8) {
+      float4 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        x[j] = i + j < n ? __ldg(reinterpret_cast<const float4*>(record(c + i + j) + rr * D) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float f = __shfl_sync(~0u, mine, (i + j) & 31);
+        sum.x += x[j].x * f; sum.y += x[j].y * f; sum.z += x[j].z * f; sum.w += x[j].w * f;
+      }
+    }
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(out_row(a, b, u / tiles, r) + lane * 4) =
+  *reinterpret_cast<uint2*>(out_row(a, RowOf(a.group), b, u / tiles, r) + lane * 4) =
       make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
 }
 
@@ -912,6 +971,7 @@ extern "C" const char* vdc_tree_attention_refuses(const vdc_tree_attention_args*
   if (a->B < 1 || a->T < 1 || a->T > 4096 || a->group < 1 || a->group > 128 || a->max_pages < 1 || a->max_pages > 0x7FFFFFFF / VDC_KV_PAGE ||
       a->cache.n_kv < 1 || (long long)a->B * a->cache.n_kv * ((a->T * a->group + kRows - 1) / kRows) > 0x7FFFFFFF)
     return "tree_attention: tokens or heads out of range";
+  if (a->T * a->group > 1 << 18) return "tree_attention: more than 262144 query rows to a KV head";
   if (a->words * 64 < a->T) return "tree_attention: the mask has fewer bits than there are tokens";
   if (!(a->scale > -INFINITY && a->scale < INFINITY)) return "tree_attention: the scale is no number";
   if (!pointers) return nullptr;
@@ -974,5 +1034,5 @@ extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* 
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, tree_join, *a, ctas, status);
+  return cudaLaunchKernelEx(&cfg, tree_join, *a, ctas);
 }
