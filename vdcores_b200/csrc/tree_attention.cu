@@ -20,6 +20,7 @@
 // sum of weights is that of P' / vs: one exponential, and no product per value.  Q becomes two e4m3 parts with a common power of two
 // per row, which are exact for bf16 values down to 2^-10 of the row's largest (below, 2^-18 of it), so K is used as it lies in
 // memory, in two passes of the 8-bit tensor cores.  V is widened to f16 (exact) by four more warps; P is f16 as well.
+#include <stdlib.h>
 #include "mk_stage.cuh"
 
 namespace vdc {
@@ -52,15 +53,19 @@ constexpr int kQRow = 68;                               // words of a query row 
 // columns of tensor memory
 constexpr int kColO = 0, kColS = 256, kColP = 384, kColQ = 448, kCols = 512;
 
-struct TreeShared {
+// What a CTA knows of its share.
+struct ShareShared {
+  int2 seq[kSeqs];                    // rows and drafted tokens of the first sequences
+  long long begin, end, first_base;   // the share among all units' pages; where sequence first_b begins
+  int first_b;
+  volatile int fail;
+  int bad[2];                         // the piece's page table names a page that is none
+};
+
+struct TreeShared : ShareShared {
   uint64_t full[8], empty[8], q_full, s_full[2], s_empty[2], p_full[2], o_done[2], tail[2];
   uint64_t v_full[kWideBufs], v_empty[kWideBufs], par_full[kWideBufs];
   uint32_t tmem;
-  volatile int fail;
-  int first_b;
-  long long begin, end, first_base;
-  int2 seq[kSeqs];                    // rows and drafted tokens of the first sequences
-  int bad[2];
   uint32_t poison[2][4][2];
   float q_mul[kRows];
   float2 stats[kMathWarps][32];       // of the rows on a warp's lanes: reference, sum of weights
@@ -77,11 +82,16 @@ __device__ __forceinline__ int2 seq_load(const vdc_tree_attention_args& a, int b
 __device__ __forceinline__ int pages_of(int2 seq) {      // 0 where there is nothing to compute
   return seq.x < 0 || seq.y == 0 ? 0 : (int)(((int64_t)seq.x + seq.y + PAGE - 1) / PAGE);
 }
-__device__ __forceinline__ int2 seq_of(const vdc_tree_attention_args& a, const TreeShared& sh, int b) {
+__device__ __forceinline__ int2 seq_of(const vdc_tree_attention_args& a, const ShareShared& sh, int b) {
   return b < kSeqs ? sh.seq[b] : seq_load(a, b);
 }
 
 __host__ __device__ __forceinline__ int tiles_of(const vdc_tree_attention_args& a) { return (a.T * a.group + kRows - 1) / kRows; }
+
+// x / y of what mostly fits 32 bits (the long division is much code for a kernel's first microsecond).
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+  return ((unsigned long long)x | (unsigned long long)y) >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y);
+}
 
 // Query row -> token and head of its group (rows are few enough for the reciprocal to be exact).
 struct RowOf {
@@ -101,13 +111,50 @@ struct Piece {
   __device__ __forceinline__ bool whole() const { return p0 == 0 && p1 == np; }
 };
 
+// One warp: this CTA's share of all units' pages, and the sequence it begins in.
+__device__ __forceinline__ void find_share(const vdc_tree_attention_args& a, ShareShared& sh, int lane) {
+  const long long units = (long long)a.cache.n_kv * tiles_of(a);
+  long long total = 0;
+  for (int b = lane; b < a.B; b += 32) total += pages_of(seq_of(a, sh, b));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
+  total *= units;
+  const long long ctas = min((long long)gridDim.x, max(total, 1ll)), me = min((long long)blockIdx.x, ctas);    // a page each at least
+  const long long begin = quotient(total * me, ctas), end = quotient(total * min(me + 1, ctas), ctas);
+  long long base = 0;
+  int first = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const long long n = b0 + lane < a.B ? pages_of(seq_of(a, sh, b0 + lane)) * units : 0;
+    long long sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long below = __shfl_up_sync(~0u, sum, o);
+      if (lane >= o) sum += below;
+    }
+    const unsigned past = __ballot_sync(~0u, base + sum > begin);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      base += __shfl_sync(~0u, sum - n, at);
+      first = b0 + at;
+      break;
+    }
+    base += __shfl_sync(~0u, sum, 31);
+  }
+  if (lane == 0) {
+    sh.begin = begin;
+    sh.end = end;
+    sh.first_base = base;
+    sh.first_b = first;
+  }
+}
+
 // The pieces of a CTA, in order; every role walks them by itself.
 struct Walk {
   const vdc_tree_attention_args& a;
-  const TreeShared& sh;
+  const ShareShared& sh;
   long long x, end, base;     // place among all units' pages, its end, where sequence b begins
   int b;
-  __device__ __forceinline__ Walk(const vdc_tree_attention_args& a_, const TreeShared& sh_)
+  __device__ __forceinline__ Walk(const vdc_tree_attention_args& a_, const ShareShared& sh_)
       : a(a_), sh(sh_), x(sh_.begin), end(sh_.end), base(sh_.first_base), b(sh_.first_b) {}
   __device__ __forceinline__ bool next(Piece& p) {
     if (x >= end) return false;
@@ -121,7 +168,7 @@ struct Walk {
       if (x < base + (long long)p.np * units) break;
       base += (long long)p.np * units;
     }
-    const int u = (int)((x - base) / p.np);
+    const int u = (int)quotient(x - base, p.np);
     p.b = b;
     p.head = tiles == 1 ? u : u / tiles;
     p.tile = tiles == 1 ? 0 : u % tiles;
@@ -167,7 +214,8 @@ __device__ __forceinline__ bool elect_one() {
 // Bounded wait on an mbarrier: 1 when its phase is over, 0 when another role has failed or the wait took longer than the limit.  The
 // loop is in the statement, and callers look at the answers of a page's waits once, together: a branch of one warp costs some 20
 // cycles, and a completed wait 56 like this, 131 with a vote and a branch of its own.  After a wait that was given up what the page
-// computes is nothing, but all of its accesses stay where they are.
+// computes is nothing, but all of its accesses stay where they are.  A barrier answers lane by lane, so that lanes may leave the loop
+// in different rounds: they are brought together again, for what follows (tcgen05.ld and st, named barriers) needs the whole warp.
 __device__ __forceinline__ uint32_t spin(uint64_t* bar, uint32_t parity, const Waiter& wait) {
   uint32_t ok;
   asm volatile(
@@ -192,6 +240,7 @@ __device__ __forceinline__ uint32_t spin(uint64_t* bar, uint32_t parity, const W
       : "=&r"(ok)
       : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<int*>(wait.fail))), "l"(wait.timeout_ns)
       : "memory");
+  __syncwarp();
   return ok;
 }
 // Whether all lanes' waits of a page ended well; if not, the status block and the other roles hear of it.
@@ -208,6 +257,14 @@ __device__ __forceinline__ bool all_well(uint32_t ok, const Waiter& wait, int ro
 // Warp-wide loads of N consecutive 32-bit columns of this thread's lane; load and wait are one statement, so that nothing that
 // uses the registers can come between them.
 #define R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : R8(r, 0) : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
@@ -239,6 +296,40 @@ __device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[N
   }
 }
 
+template <int N>
+__device__ __forceinline__ void tmem_store_any(uint32_t taddr, const uint32_t (&r)[N]) {
+  if constexpr (N == 4)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+  else
+    tmem_store(taddr, r);
+}
+
+// Eight bf16 values of a row of 128 (a lane of sixteen): the row times a power of two that takes its largest value to [128, 256), as
+// the sum of two e4m3 numbers; returns the power's inverse, or NaN for a row that has no numbers.
+__device__ __forceinline__ float split_row(const uint4& v, unsigned sixteen, uint2& hi, uint2& lo) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(sixteen, top, o));
+  const int e = (int)(top >> 7);                            // exponent of the largest
+  const int up = e == 0xFF ? 0 : min(126, 134 - max(e, 1)); // (rows of nearly nothing: as far as it goes)
+  const float mul = exp2f((float)up);
+  uint32_t h[2] = {0, 0}, l[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = make_float2(bf_lo(u[j]) * mul, bf_hi(u[j]) * mul);
+    const uint32_t c8 = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+    const float2 x = e4m3x2_to_float2(c8);
+    h[j >> 1] |= c8 << (16 * (j & 1));
+    l[j >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f.x - x.x, f.y - x.y), __NV_SATFINITE, __NV_E4M3) << (16 * (j & 1));
+  }
+  hi = make_uint2(h[0], h[1]);
+  lo = make_uint2(l[0], l[1]);
+  return e == 0xFF ? NAN : exp2f((float)-up);
+}
+
 __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int x, int head, int page, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
@@ -249,11 +340,15 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
 // The math warps meet; true for all of them if one says so.  None of them waits for anything without a limit elsewhere, so all arrive.
 __device__ __forceinline__ bool math_any(bool x) {
   int r;
+  __syncwarp();
   asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, 1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
                : "=r"(r) : "r"((int)x), "n"(kMathWarps * 32) : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void math_sync() { asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(kMathWarps * 32) : "memory"); }
+__device__ __forceinline__ void math_sync() {
+  __syncwarp();
+  asm volatile("barrier.cta.sync.aligned 1, %0;" ::"n"(kMathWarps * 32) : "memory");
+}
 
 // Bit j: the row of token t attends to key page * 64 + j.
 __device__ __forceinline__ uint64_t seen_bits(const vdc_tree_attention_args& a, const Piece& p, int page, int t) {
@@ -271,6 +366,24 @@ __device__ __forceinline__ uint64_t seen_bits(const vdc_tree_attention_args& a, 
   return n < 64 ? m & ((1ull << n) - 1) : m;
 }
 
+// kThreads threads look at a sequence's whole page table; true for one that found a page outside the pool.
+template <int kThreads>
+__device__ __forceinline__ bool names_no_page(const vdc_tree_attention_args& a, const Piece& p, int tid, vdc_status* status) {
+  bool found = false;
+  for (int i0 = tid; i0 < p.np; i0 += kThreads * 8) {
+    int id[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) id[j] = i0 + kThreads * j < p.np ? __ldg(reinterpret_cast<const int*>(a.pages) + p.b * a.pages_b + i0 + kThreads * j) : 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (id[j] < 0 || id[j] >= a.cache.n_pages) {
+        found = true;
+        report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, p.b, id[j]);
+      }
+  }
+  return found;
+}
+
 // A record of a piece: sums [rows][128], then (reference, sum of weights) [rows]; a multiple of 16 bytes.
 __host__ __device__ __forceinline__ long long record_floats(const vdc_tree_attention_args& a) {
   const int rows = a.T * a.group;
@@ -279,6 +392,19 @@ __host__ __device__ __forceinline__ long long record_floats(const vdc_tree_atten
 
 __device__ __forceinline__ __nv_bfloat16* out_row(const vdc_tree_attention_args& a, const RowOf& of, int b, int head, int r) {
   return reinterpret_cast<__nv_bfloat16*>(a.out) + b * a.o_b + head * a.o_kv + of.at(r, a.o_t, a.o_g);
+}
+
+// Sequences without anything to attend with, or that do not fit their tables, get zeros (the first `threads` threads).
+__device__ __forceinline__ void write_zeros(const vdc_tree_attention_args& a, const ShareShared& sh, const RowOf& of, vdc_status* status, int threads) {
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    const int2 seq = seq_of(a, sh, b);
+    if (pages_of(seq)) continue;
+    if (seq.x < 0 && threadIdx.x == 0)
+      report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 0, b, __ldg(reinterpret_cast<const int*>(a.lengths) + b));
+    const int heads = a.cache.n_kv, n = a.T * a.group * heads * (D / 8);
+    for (int i = threadIdx.x; i < n; i += threads)
+      *reinterpret_cast<uint4*>(out_row(a, of, b, (i / (D / 8)) % heads, i / (D / 8) / heads) + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+  }
 }
 
 template <bool kF8, int kReps>
@@ -329,42 +455,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
   const uint32_t tmem = sh.tmem;
   const int rows = a.T * a.group;
   const RowOf row_of(a.group);
-  if (warp == 0) {
-    // this CTA's share of all units' pages, and the sequence it begins in
-    const long long units = (long long)a.cache.n_kv * tiles_of(a);
-    long long total = 0;
-    for (int b = lane; b < a.B; b += 32) total += pages_of(seq_of(a, sh, b));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
-    total *= units;
-    const long long ctas = min((long long)gridDim.x, max(total, 1ll)), me = min((long long)blockIdx.x, ctas);    // a page each at least
-    const long long begin = total * me / ctas, end = total * min(me + 1, ctas) / ctas;
-    long long base = 0;
-    int first = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-      const long long n = b0 + lane < a.B ? pages_of(seq_of(a, sh, b0 + lane)) * units : 0;
-      long long sum = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long below = __shfl_up_sync(~0u, sum, o);
-        if (lane >= o) sum += below;
-      }
-      const unsigned past = __ballot_sync(~0u, base + sum > begin);
-      if (past) {
-        const int at = __ffs(past) - 1;
-        base += __shfl_sync(~0u, sum - n, at);
-        first = b0 + at;
-        break;
-      }
-      base += __shfl_sync(~0u, sum, 31);
-    }
-    if (lane == 0) {
-      sh.begin = begin;
-      sh.end = end;
-      sh.first_base = base;
-      sh.first_b = first;
-    }
-  }
+  if (warp == 0) find_share(a, sh, lane);
   __syncthreads();
 
   if (warp >= kMathWarps) {
@@ -625,28 +716,11 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
           if constexpr (!kF8) {
             *reinterpret_cast<uint4*>(to + sub * 4) = v;
           } else {
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(half, top, o));
-            const int e = (int)(top >> 7);                            // exponent of the largest
-            // a power of two that takes the largest to [128, 256); rows of (nearly) nothing as they are
-            const int up = e == 0xFF ? 0 : min(126, 134 - max(e, 1));
-            const float mul = exp2f((float)up);
-            uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 f = make_float2(bf_lo(u[j]) * mul, bf_hi(u[j]) * mul);
-              const uint32_t c8 = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-              const float2 h = e4m3x2_to_float2(c8);
-              hi[j >> 1] |= c8 << (16 * (j & 1));
-              lo[j >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f.x - h.x, f.y - h.y), __NV_SATFINITE, __NV_E4M3) << (16 * (j & 1));
-            }
-            *reinterpret_cast<uint2*>(to + sub * 2) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(to + 32 + sub * 2) = make_uint2(lo[0], lo[1]);
-            if (sub == 0) sh.q_mul[rr] = e == 0xFF ? NAN : exp2f((float)-up);
+            uint2 hi, lo;
+            const float back = split_row(v, half, hi, lo);
+            *reinterpret_cast<uint2*>(to + sub * 2) = hi;
+            *reinterpret_cast<uint2*>(to + 32 + sub * 2) = lo;
+            if (sub == 0) sh.q_mul[rr] = back;
           }
         }
       }
@@ -665,19 +739,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         if (lane == 0) mbar_arrive(&sh.q_full);
       }
       // the sequence's whole page table: a page outside the pool leaves the sequence out, in every piece alike
-      if (w == 1) {
-        for (int i0 = tid - 128; i0 < p.np; i0 += 128 * 8) {
-          int id[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) id[j] = i0 + 128 * j < p.np ? __ldg(reinterpret_cast<const int*>(a.pages) + p.b * a.pages_b + i0 + 128 * j) : 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (id[j] < 0 || id[j] >= a.cache.n_pages) {
-              sh.bad[turn & 1] = 1;
-              report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, p.b, id[j]);
-            }
-        }
-      }
+      if (w == 1 && names_no_page<128>(a, p, tid - 128, status)) sh.bad[turn & 1] = 1;
       float row_scale = scale;
       if constexpr (kF8) row_scale *= sh.q_mul[tile_row];
       float m = -INFINITY, l = 0.f;
@@ -687,7 +749,10 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         uint32_t good = spin(&sh.s_full[w], c & 1, wait);
         const bool tail = (page + 1) * PAGE > p.ctx;
         uint64_t bits = ~0ull;
-        if (tail) bits = live ? seen_bits(a, p, page, t) : 0;
+        if (tail) {
+          bits = live ? seen_bits(a, p, page, t) : 0;
+          __syncwarp();
+        }
         uint32_t raw[kKeys];
         tc_fence_after();
         tmem_load(lanes + kColS + w * PAGE + key0, raw);
@@ -832,6 +897,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
 #pragma unroll 1
       for (int col = 0; col < D; col += 32) {
         uint32_t o[32];
+        __syncwarp();
         if (has) tmem_load(lanes + kColO + w * D + col, o);
         if (tile_row < tile_rows) {
 #pragma unroll
@@ -861,15 +927,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       if (tid == 0) sh.bad[turn & 1] = 0;
       tc_fence_before();
     }
-  }
-  // sequences without anything to attend with, or that do not fit their tables, get zeros
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    const int2 seq = seq_of(a, sh, b);
-    if (pages_of(seq)) continue;
-    if (seq.x < 0 && tid == 0) report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 0, b, __ldg(reinterpret_cast<const int*>(a.lengths) + b));
-    const int heads = a.cache.n_kv, n = rows * heads * (D / 8);
-    for (int i = tid; i < n; i += C::kThreads)
-      *reinterpret_cast<uint4*>(out_row(a, row_of, b, (i / (D / 8)) % heads, i / (D / 8) / heads) + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
+    write_zeros(a, sh, row_of, status, kMathWarps * 32);
   }
   tc_fence_before();
   __syncthreads();
@@ -877,6 +935,637 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
   if (warp == C::kScoreWarp) {
     tc_fence_after();
     tmem_dealloc(tmem, kCols);
+  }
+}
+
+// ------------------------------------------------------------------------- //
+// Up to 64 rows: the keys lie on the lanes.  A step is two pages: S^T = K Q^T (128 keys by the rows), a thread has one key's scores
+// and, of e4m3, its scales; O^T += V^T P^T (128 values by the rows) with P in shared memory, written by its key's thread, eight rows
+// of a key in 16 bytes.  The tensor cores then work for the rows that exist and not for 128, a thread needs no other key's scale,
+// the drafted tokens' tests are a thread's own, and two pages pass each role at a time.
+//
+// Two groups of four warps take the steps in turn, with references and sums O^T of their own (a warp reaches 32 of the 128 values
+// only, so that a group has to rescale together); with more than 32 rows they share each step, half of the rows to a group
+// (registers).  A step first asks whether any of the group's scores exceeds its row's reference by too much (one barrier of the
+// group); only then, which after the first steps is rare, the maxima are looked for, and the sums rescaled.
+// ------------------------------------------------------------------------- //
+template <bool kF8, int R>
+struct KeysCfg {
+  static constexpr bool kSplit = R > 32;                                // the groups share a step's rows
+  static constexpr int kOwn = kSplit ? R / 2 : R;                       // rows of a thread
+  static constexpr int kN = R < 16 ? 16 : R, kSums = kSplit ? 1 : 2;    // columns of S^T and O^T; how many O^T there are
+  static constexpr int kCols = (2 + kSums) * kN <= 64 ? 64 : (2 + kSums) * kN <= 128 ? 128 : 256;
+  static constexpr int kPart = 2 * PAGE * D * (kF8 ? 1 : 2);            // keys or values of a step
+  // keys and values have rings of their own: a role that follows one of them sees every use of its slots
+  static constexpr int kKeySlots = kF8 ? (R >= 32 ? 3 : 4) : 3, kValSlots = kF8 ? kKeySlots : R >= 32 ? 2 : 3, kSlots = kKeySlots + kValSlots;
+  static constexpr int kQBytes = kN * D * 2;                            // bf16, or twice e4m3
+  static constexpr int kPBytes = kN / 8 * 2048;                         // of one buffer of two
+  static constexpr int kWide = kF8 ? 2 * PAGE * D * 2 : 0;              // widened values of a step, two buffers
+  static constexpr int kBytes = 1024 + kSlots * kPart + 2 * kWide + kQBytes + 2 * kPBytes;
+  static_assert(kBytes + 14336 <= 232448, "shared memory of a CTA");
+  static constexpr int kLoadWarp = kMathWarps + (kF8 ? 8 : 0), kScoreWarp = kLoadWarp + 1, kSumWarp = kLoadWarp + 2;
+  static constexpr int kThreads = kF8 ? 640 : 384, kMathRegs = kF8 ? 128 : 208, kOtherRegs = kF8 ? 72 : 88;
+  // powers of two by which a score may exceed its reference, and by which f16 weights are kept larger (2^15 at most)
+  static constexpr float kSlack = kF8 ? 4.f : 8.f, kLift = kF8 ? 11.f : 0.f;
+};
+constexpr float kNoRef = 1e30f;              // minus the reference of a row that has none yet
+
+struct KeysShared : ShareShared {
+  uint64_t full[8], empty[8], q_full, s_full[2], s_empty[2], p_full[2], o_done[2], v_full[2], v_empty[2], checked;
+  uint32_t tmem;
+  uint64_t sees[64];                         // of a drafted token: the rows that attend to it
+  __nv_bfloat16* out[64];                    // of a row: its result
+  alignas(16) float mul[64];                 // of a row: what its scores are multiplied by
+  alignas(16) float ref[2][64];              // of a group's rows: minus the reference
+  alignas(16) float factor[2][64];           // what their sums are multiplied by
+  float most[kMathWarps][64];                // of a warp's rows: largest score, or sum of weights
+  uint8_t odd[4][128];                       // of a key: a drafted token whose bf16 values are no numbers
+  alignas(16) float scales[4][2][128];
+};
+
+// The group's 128 threads meet; true for all if one says so.  Every wait between two of these has a limit, and no warp leaves the
+// steps' loop but with its group.
+__device__ __forceinline__ bool group_any(int w, bool x) {
+  int r;
+  __syncwarp();
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, %2, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"((int)x), "r"(2 + w) : "memory");
+  return r != 0;
+}
+
+// The largest of a warp's values, NaN left out.
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Two fp32 values in one 64-bit register, and the instructions that work on both.
+__device__ __forceinline__ uint64_t two(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 apart(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t id, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(id), "r"(accumulate)
+      : "memory");
+}
+
+template <bool kF8, int R>
+__global__ void __launch_bounds__(KeysCfg<kF8, R>::kThreads, 1)
+tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __grid_constant__ CUtensorMap k_map,
+                    const __grid_constant__ CUtensorMap v_map, vdc_status* status, uint64_t timeout_ns) {
+  using C = KeysCfg<kF8, R>;
+  constexpr int RT = C::kOwn, kStep = 2 * PAGE, kArrive = C::kSplit ? kMathWarps : 4;      // warps that a step's scores are for
+  extern __shared__ __align__(1024) uint8_t dyn[];
+  __shared__ KeysShared sh;
+  uint8_t* ring = dyn + (-(int)smem_u32(dyn) & 1023);
+  uint8_t* wide = ring + C::kSlots * C::kPart;
+  uint8_t* q_rows = wide + 2 * C::kWide;
+  uint8_t* weights = q_rows + C::kQBytes;
+  const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
+  const Waiter wait{&sh.fail, status, timeout_ns, VDC_TREE_ATTENTION_KIND};
+  const int rows = a.T * a.group;
+  const RowOf row_of(a.group);
+
+  grid_dep_launch();
+  if (warp == C::kScoreWarp) tmem_alloc(&sh.tmem, C::kCols);
+  for (int b = tid; b < min(a.B, kSeqs); b += C::kThreads) sh.seq[b] = seq_load(a, b);
+  if (warp == C::kLoadWarp && lane == 0) {
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&sh.full[i], 1);
+      // e4m3: keys are given back by the scores and by the warps that take the scales, values by a team that widens them
+      mbar_init(&sh.empty[i], !kF8 ? 1 : i >= C::kKeySlots ? 4 : 1 + kArrive);
+    }
+    mbar_init(&sh.q_full, kMathWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.s_empty[i], kArrive);
+      mbar_init(&sh.p_full[i], kArrive);
+      mbar_init(&sh.o_done[i], 1);
+      mbar_init(&sh.v_full[i], 4);
+      mbar_init(&sh.v_empty[i], 1);
+    }
+    mbar_init(&sh.checked, 4);
+    sh.fail = sh.bad[0] = sh.bad[1] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem, col_s = tmem, col_o = tmem + 2 * C::kN;
+  if (warp == 0) find_share(a, sh, lane);
+  __syncthreads();
+
+  // Slot and phase of step g's keys, and of its values.
+  auto key_slot = [](uint32_t g) { return g % C::kKeySlots; };
+  auto key_phase = [](uint32_t g) { return (g / C::kKeySlots) & 1; };
+  auto val_slot = [](uint32_t g) { return C::kKeySlots + g % C::kValSlots; };
+  auto val_phase = [](uint32_t g) { return (g / C::kValSlots) & 1; };
+  if (warp >= kMathWarps) {
+    set_registers<C::kOtherRegs, false>();
+    Walk walk(a, sh);
+    Piece p;
+    uint32_t g = 0;                       // steps of the CTA so far
+    bool ok = true;
+    if (warp == C::kLoadWarp) {
+      // ---- pages into the ring
+      while (ok && walk.next(p)) {
+        const int* table = reinterpret_cast<const int*>(a.pages) + p.b * a.pages_b;
+        int ids = 0;
+        for (int i = p.p0; i < p.p1; i += 2, ++g) {
+          if (((i - p.p0) & 31) == 0) {
+            ids = i + lane < p.p1 ? __ldg(table + i + lane) : 0;
+            if (ids < 0 || ids >= a.cache.n_pages) ids = 0;       // reported by the math warps, which leave the sequence out
+          }
+          const int page[2] = {__shfl_sync(~0u, ids, (i - p.p0) & 31), __shfl_sync(~0u, ids, (i - p.p0 + 1) & 31)};
+          const int n = min(2, p.p1 - i);
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            const uint32_t st = part == 0 ? key_slot(g) : val_slot(g), ph = part == 0 ? key_phase(g) : val_phase(g);
+            ok = all_well(spin(&sh.empty[st], ph ^ 1, wait), wait, 0, i);
+            if (!ok) break;
+            if (elect_one()) {
+              uint64_t* bar = &sh.full[st];
+              uint8_t* to = ring + st * C::kPart;
+              mbar_arrive_expect_tx(bar, n * (C::kPart / 2 + (kF8 && part == 0 ? 2 * PAGE * 4 : 0)));
+              for (int j = 0; j < n; ++j) {
+                if constexpr (kF8) {
+                  const uint64_t from = part == 0 ? a.cache.k + page[j] * a.cache.k_page + p.head * a.cache.k_head
+                                                  : a.cache.v + page[j] * a.cache.v_page + p.head * a.cache.v_head;
+                  bulk_load_1d(to + j * PAGE * D, reinterpret_cast<const void*>(from), PAGE * D, bar);
+                  if (part == 0) {
+                    bulk_load_1d(&sh.scales[st][0][j * PAGE], reinterpret_cast<const void*>(a.cache.k_scale + page[j] * a.cache.ks_page + p.head * a.cache.ks_head), PAGE * 4, bar);
+                    bulk_load_1d(&sh.scales[st][1][j * PAGE], reinterpret_cast<const void*>(a.cache.v_scale + page[j] * a.cache.vs_page + p.head * a.cache.vs_head), PAGE * 4, bar);
+                  }
+                } else {
+                  for (int h = 0; h < 2; ++h) tma_page(to + h * (C::kPart / 2) + j * PAGE * 128, part == 0 ? &k_map : &v_map, h * 64, p.head, page[j], bar);
+                }
+              }
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+        }
+      }
+    } else if (warp == C::kScoreWarp) {
+      // ---- S^T = K Q^T.  The whole warp walks and waits, an elected lane issues: descriptors are then the same for the warp as far
+      // as the compiler knows, and stay in uniform registers (issued from a branch of lane 0 an MMA took about 120 cycles)
+      constexpr uint32_t id = idesc(kF8 ? 0 : 1, C::kN, false);
+      const uint64_t k_desc = desc_sw128(smem_u32(ring), 16, 1024), q_desc = desc_sw128(smem_u32(q_rows), 16, 1024);
+      const uint32_t d0 = __shfl_sync(~0u, col_s, 0);
+      uint32_t turn = 0;
+      while (ok && walk.next(p)) {
+        uint32_t good = spin(&sh.q_full, turn++ & 1, wait);
+        for (int i = p.p0; i < p.p1; i += 2, ++g) {
+          const uint32_t st = key_slot(g), w = g & 1;
+          good &= spin(&sh.s_empty[w], ((g >> 1) & 1) ^ 1, wait) & spin(&sh.full[st], key_phase(g), wait);
+          ok = all_well(good, wait, 1, i);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t k = k_desc + st * (C::kPart >> 4);
+          const uint32_t d = d0 + w * C::kN;
+          if (elect_one()) {
+            if constexpr (kF8) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)          // the rows' upper parts, then their lower ones
+                umma_f8(d, k + (j & 3) * 2, q_desc + (j >> 2) * (C::kN * 128 >> 4) + (j & 3) * 2, id, j > 0);
+              umma_commit(&sh.s_full[w]);
+              umma_commit(&sh.empty[st]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                umma_bf16(d, k + (j >> 2) * (C::kPart >> 5) + (j & 3) * 2, q_desc + (j >> 2) * (C::kN * 128 >> 4) + (j & 3) * 2, id, j > 0);
+              umma_commit(&sh.s_full[w]);
+              umma_commit(&sh.empty[st]);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    } else if (warp == C::kSumWarp) {
+      // ---- O^T += V^T P^T
+      constexpr uint32_t id = idesc(kF8 ? 0 : 1, C::kN, true) | 1u << 15;
+      const uint64_t v_desc = desc_sw128(smem_u32(kF8 ? wide : ring), 2 * PAGE * 128, 1024), p_desc = umma_desc(smem_u32(weights), 128, 2048);
+      const uint32_t d = __shfl_sync(~0u, col_o, 0);
+      while (ok && walk.next(p)) {
+        for (int i = p.p0; i < p.p1; i += 2, ++g) {
+          const uint32_t st = val_slot(g), w = g & 1, ph = (g >> 1) & 1;
+          ok = all_well((kF8 ? spin(&sh.v_full[w], ph, wait) : spin(&sh.full[st], val_phase(g), wait)) & spin(&sh.p_full[w], ph, wait), wait, 2, i);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t v = v_desc + (kF8 ? w * (C::kWide >> 4) : st * (C::kPart >> 4)), pw = p_desc + w * (C::kPBytes >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              umma_bf16(d + (C::kSplit ? 0 : w * C::kN), v + j * 128, pw + j * 16, id, i > p.p0 + (C::kSplit ? 0 : 2) || j > 0);
+            umma_commit(&sh.o_done[w]);
+            umma_commit(kF8 ? &sh.v_empty[w] : &sh.empty[st]);
+          }
+          __syncwarp();
+        }
+      }
+    } else if (kF8 && warp < C::kLoadWarp) {
+      // ---- e4m3 values to f16, by two teams of four warps that take the steps in turn.  Rows behind the piece's end become zeros (a
+      // weight of zero would not do: zero times NaN), and so do drafted tokens' codes that are no numbers: their scales say so
+      const int t = tid & 127, team = (warp - kMathWarps) >> 2, piece = t & 7, r0 = t >> 3, sw = r0 & 7;      // rows r0, r0 + 16, ...
+      // sixteen values are two pieces of a half's row; lanes of the other half take them in the other order, for the banks' sake
+      const int from = r0 * D + ((piece ^ sw) << 4), to = (piece >> 2) * (kStep * 128) + r0 * 128;
+      const int lo = to + ((((2 * piece) & 7) ^ sw) << 4), hi = to + ((((2 * piece + 1) & 7) ^ sw) << 4);
+      const bool swap = piece >= 4;
+      uint8_t* dst = wide + team * C::kWide;
+      while (ok && walk.next(p)) {
+        const int end = min(p.total(), p.p1 * PAGE);
+        for (int i = p.p0; i < p.p1; i += 2, ++g) {
+          if ((g & 1) != (uint32_t)team) continue;
+          const uint32_t st = val_slot(g);
+          // the buffer first: when the step before the last is in the sums, whatever the slot held before has landed.  (A slot's uses can
+          // alternate between the teams; a parity alone would take the use before the last for this one.)
+          uint32_t good = spin(&sh.v_empty[team], ((g >> 1) & 1) ^ 1, wait);
+          good &= spin(&sh.full[st], val_phase(g), wait);
+          const uint8_t* src = ring + st * C::kPart + from;
+          uint4 code[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) code[j] = *reinterpret_cast<const uint4*>(src + j * 16 * D);
+          const int left = end - i * PAGE, own = p.ctx - i * PAGE;
+          if (min(left, own) < kStep) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int row = j * 16 + r0;
+              auto clean = [](uint32_t w) {
+                const uint32_t x = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                return w & ~((x >> 7) * 0xFFu);
+              };
+              if (row >= left) code[j] = make_uint4(0, 0, 0, 0);
+              else if (row >= own) code[j] = make_uint4(clean(code[j].x), clean(code[j].y), clean(code[j].z), clean(code[j].w));
+            }
+          }
+          ok = all_well(good, wait, 3, i);
+          if (!ok) break;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t x[4], y[4];
+            e4m3x4_to_half2(code[j].x, reinterpret_cast<uint32_t(&)[2]>(x[0]));
+            e4m3x4_to_half2(code[j].y, reinterpret_cast<uint32_t(&)[2]>(x[2]));
+            e4m3x4_to_half2(code[j].z, reinterpret_cast<uint32_t(&)[2]>(y[0]));
+            e4m3x4_to_half2(code[j].w, reinterpret_cast<uint32_t(&)[2]>(y[2]));
+            const uint4 first = make_uint4(x[0], x[1], x[2], x[3]), second = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(dst + j * 16 * 128 + (swap ? hi : lo)) = swap ? second : first;
+            *reinterpret_cast<uint4*>(dst + j * 16 * 128 + (swap ? lo : hi)) = swap ? first : second;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&sh.v_full[team]);
+            mbar_arrive(&sh.empty[st]);
+          }
+        }
+      }
+    }
+  } else {
+    // ---- scores to weights, sums to results
+    set_registers<C::kMathRegs, true>();
+    Walk walk(a, sh);
+    Piece p;
+    const int w = warp >> 2, key = tid & 127, r0 = C::kSplit ? w * RT : 0;           // group, the thread's key of a step, its first row
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+    const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+    uint32_t g = 0, tails = 0;        // steps of the CTA, and those with drafted tokens
+    for (int turn = 0; walk.next(p); ++turn) {
+      // ---- the rows to shared memory as the tensor cores read them (half a warp loads one), the drafted tokens' masks, and a look
+      // at the page table; all loads first
+      const int sub = lane & 15, end = min(p.total(), p.p1 * PAGE);
+      uint4 q[(R + 15) / 16];
+#pragma unroll
+      for (int k = 0; k < (R + 15) / 16; ++k) {
+        const int r = k * 16 + warp * 2 + (lane >> 4);
+        q[k] = make_uint4(0, 0, 0, 0);
+        if (r < rows && row_of.token(r) < p.live)
+          q[k] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + p.b * a.q_b + p.head * a.q_kv + row_of.at(r, a.q_t, a.q_g)) + sub);
+      }
+      uint64_t words[2] = {0, 0};                     // of tokens lane and lane + 32 (64 tokens at most)
+      if (end > p.ctx) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int t = lane + 32 * h;
+          if (t < p.live) words[h] = a.mask ? (uint64_t)__ldg(reinterpret_cast<const long long*>(a.mask) + p.b * a.mask_b + t * a.mask_t) : (2ull << t) - 1;
+        }
+      }
+      if (names_no_page<kMathWarps * 32>(a, p, tid, status)) sh.bad[turn & 1] = 1;
+#pragma unroll
+      for (int k = 0; k < (R + 15) / 16; ++k) {
+        const int r = k * 16 + warp * 2 + (lane >> 4);
+        uint4 v = q[k];
+        v.x ^= sign; v.y ^= sign; v.z ^= sign; v.w ^= sign;
+        float mul = scale;
+        if constexpr (!kF8) {
+          if (r < R) *reinterpret_cast<uint4*>(q_rows + (sub >> 3) * (C::kN * 128) + r * 128 + (((sub & 7) ^ (r & 7)) << 4)) = v;
+        } else {
+          uint2 hi, lo;
+          mul *= split_row(v, 0xFFFFu << (lane & 16), hi, lo);
+          uint8_t* to = q_rows + r * 128 + (((sub >> 1) ^ (r & 7)) << 4) + (sub & 1) * 8;
+          if (r < R) {
+            *reinterpret_cast<uint2*>(to) = hi;
+            *reinterpret_cast<uint2*>(to + C::kN * 128) = lo;
+          }
+        }
+        if (r < R && sub == 0) {
+          sh.mul[r] = mul;
+          sh.out[r] = out_row(a, row_of, p.b, p.head, r);
+        }
+      }
+      if (tid < 128) sh.ref[tid >> 6][tid & 63] = kNoRef;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full);
+      if (end > p.ctx) {
+        // tokens that attend to drafted token j, then rows; a warp takes eight tokens
+        const int t0 = row_of.token(lane), t1 = row_of.token(lane + 32);
+#pragma unroll 1
+        for (int j = warp * 8; j < min(warp * 8 + 8, p.live); ++j) {
+          const uint64_t tokens = (uint64_t)__ballot_sync(~0u, (words[1] >> j) & 1) << 32 | __ballot_sync(~0u, (words[0] >> j) & 1);
+          const uint32_t lower = __ballot_sync(~0u, t0 < 64 && ((tokens >> t0) & 1)), upper = __ballot_sync(~0u, t1 < 64 && ((tokens >> t1) & 1));
+          if (lane == 0) sh.sees[j] = (uint64_t)upper << 32 | lower;
+        }
+      }
+      math_sync();
+
+      uint64_t l[RT / 2];                     // sums of weights of two rows each
+#pragma unroll
+      for (int r = 0; r < RT / 2; ++r) l[r] = 0;
+      const uint32_t mine_o = col_o + lanes + (C::kSplit ? 0 : w * C::kN) + r0;      // the group's sums of the warp's 32 values
+      uint32_t good = 1;
+      bool failed = false;
+      int i = p.p0;
+      if (!C::kSplit && (g & 1) != (uint32_t)w) i += 2, ++g;
+      bool first = true;
+      for (; i < p.p1; i += C::kSplit ? 2 : 4, g += C::kSplit ? 1 : 2) {
+        const uint32_t st = key_slot(g), b = g & 1, ph = (g >> 1) & 1;
+        const int mine = i * PAGE + key;                      // the key among the sequence's
+        good &= spin(&sh.s_full[b], ph, wait);
+        tc_fence_after();
+        uint32_t x[RT];
+        tmem_load(col_s + lanes + b * C::kN + r0, x);
+        float ks = 1.f, lg = 0.f, inv = 1.f;
+        if constexpr (kF8) {
+          good &= spin(&sh.full[st], key_phase(g), wait);
+          ks = sh.scales[st][0][key];
+          const float vs = sh.scales[st][1][key];
+          lg = log2f(fmaxf(vs, 0x1p-100f));
+          inv = __fdividef(1.f, fmaxf(vs, 0x1p-100f));
+          if (!(vs < INFINITY)) lg = vs, inv = 0.f;            // no number: whoever attends to it gets none either
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sh.s_empty[b]);
+          if (kF8) mbar_arrive(&sh.empty[st]);
+        }
+        // ---- scores
+        uint64_t z[RT / 2];
+        const uint64_t ks2 = two(ks, ks), lg2 = two(lg, lg);
+#pragma unroll
+        for (int r = 0; r < RT; r += 4) {
+          const ulonglong2 mul = *reinterpret_cast<const ulonglong2*>(&sh.mul[r0 + r]);
+          const uint64_t x0 = two(__uint_as_float(x[r]), __uint_as_float(x[r + 1])), x1 = two(__uint_as_float(x[r + 2]), __uint_as_float(x[r + 3]));
+          z[r / 2] = kF8 ? fma2(mul2(x0, ks2), mul.x, lg2) : mul2(x0, mul.x);
+          z[r / 2 + 1] = kF8 ? fma2(mul2(x1, ks2), mul.y, lg2) : mul2(x1, mul.y);
+        }
+        if ((i + 2) * PAGE > min(p.ctx, end)) {
+          // drafted tokens, and what is none of the piece's keys.  The values of the latter become zeros (a weight of zero would not
+          // do: zero times NaN); so do those of a drafted token that are no numbers, whose readers get none by their scores
+          const int j = mine - p.ctx;
+          uint64_t see = mine >= end ? 0 : j < 0 ? ~0ull : sh.sees[j];
+          bool none = false;
+          if constexpr (kF8) {
+            if (mine >= end) inv = 0.f;
+          } else if (!C::kSplit || w == 0) {
+            good &= spin(&sh.o_done[b], ph ^ 1, wait);      // (the sums first, as for the teams that widen)
+            good &= spin(&sh.full[val_slot(g)], val_phase(g), wait);
+            uint4* v = reinterpret_cast<uint4*>(ring + val_slot(g) * C::kPart + key * 128);
+            if (j >= 0 && mine < end) {
+#pragma unroll 4
+              for (int x = 0; x < 16; ++x) {
+                const uint4 y = v[(x >> 3) * (C::kPart / 32) + (x & 7)];
+                auto odd = [](uint32_t u) { return (u & 0x7F80u) == 0x7F80u || (u & 0x7F800000u) == 0x7F800000u; };
+                none |= odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w);
+              }
+            }
+            if (none || mine >= end) {
+#pragma unroll 4
+              for (int x = 0; x < 16; ++x) v[(x >> 3) * (C::kPart / 32) + (x & 7)] = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            if constexpr (C::kSplit) {
+              sh.odd[g & 3][key] = none;
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.checked);
+            }
+          } else {                                // the other group has looked at the values
+            good &= spin(&sh.checked, tails & 1, wait);
+            none = sh.odd[g & 3][key];
+          }
+          ++tails;
+          see >>= r0;
+#pragma unroll
+          for (int r = 0; r < RT; r += 2) {
+            float2 y = apart(z[r / 2]);
+            y.x = !((see >> r) & 1) ? -INFINITY : none ? NAN : y.x;
+            y.y = !((see >> (r + 1)) & 1) ? -INFINITY : none ? NAN : y.y;
+            z[r / 2] = two(y.x, y.y);
+          }
+        }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int r = 0; r < RT; r += 4) {
+          const ulonglong2 ref = *reinterpret_cast<const ulonglong2*>(&sh.ref[w][r0 + r]);
+          const float2 x = apart(add2(z[r / 2], ref.x)), y = apart(add2(z[r / 2 + 1], ref.y));
+          top[0] = fmaxf(top[0], fmaxf(x.x, x.y));
+          top[1] = fmaxf(top[1], fmaxf(y.x, y.y));
+        }
+        if (group_any(w, fmaxf(top[0], top[1]) > C::kSlack + C::kLift || !good)) {
+          if (group_any(w, !good)) {
+            failed = true;
+            break;
+          }
+          // new references: the rows' maxima over the group's keys, a thread to a row; all then multiply what they have
+#pragma unroll
+          for (int r = 0; r < RT; r += 2) {
+            const float2 y = apart(z[r / 2]);
+            const float m0 = warp_max(y.x), m1 = warp_max(y.y);
+            if (lane == 0) *reinterpret_cast<float2*>(&sh.most[warp][r0 + r]) = make_float2(m0, m1);
+          }
+          good &= spin(&sh.o_done[C::kSplit ? b ^ 1 : b], C::kSplit ? ((g - 1) >> 1) & 1 : ph ^ 1, wait);      // what there is, is in the sums
+          group_any(w, false);
+          if (key < RT) {
+            const int r = r0 + key;
+            const float ref = sh.ref[w][r], now = fmaxf(fmaxf(sh.most[4 * w][r], sh.most[4 * w + 1][r]), fmaxf(sh.most[4 * w + 2][r], sh.most[4 * w + 3][r]));
+            const bool up = ref == kNoRef ? now > -INFINITY : now + ref > C::kLift;
+            sh.factor[w][r] = !up ? 1.f : ref == kNoRef ? 0.f : exp2_ftz(C::kLift - ref - now);
+            if (up) sh.ref[w][r] = C::kLift - now;
+          }
+          group_any(w, false);
+          tc_fence_after();
+          uint32_t o[RT];
+          if (!first) tmem_load(mine_o, o);
+#pragma unroll
+          for (int r = 0; r < RT; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(&sh.factor[w][r0 + r]);
+            l[r / 2] = mul2(l[r / 2], two(f.x, f.y));
+            l[r / 2 + 1] = mul2(l[r / 2 + 1], two(f.z, f.w));
+            const float fs[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) o[r + y] = __float_as_uint(__uint_as_float(o[r + y]) * fs[y]);
+          }
+          if (!first) {
+            tmem_store_any(mine_o, o);
+            tmem_st_wait();
+          }
+        }
+        first = false;
+        // ---- weights
+        uint32_t h[RT / 2];
+        const uint64_t inv2 = two(inv, inv);
+#pragma unroll
+        for (int r = 0; r < RT; r += 4) {
+          const ulonglong2 ref = *reinterpret_cast<const ulonglong2*>(&sh.ref[w][r0 + r]);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float2 x = apart(add2(z[r / 2 + y], y ? ref.y : ref.x));
+            const float e0 = exp2_ftz(x.x), e1 = exp2_ftz(x.y);
+            l[r / 2 + y] = kF8 ? fma2(two(e0, e1), inv2, l[r / 2 + y]) : add2(l[r / 2 + y], two(e0, e1));
+            if constexpr (kF8) {
+              const __half2 v = __floats2half2_rn(e0, e1);
+              h[r / 2 + y] = *reinterpret_cast<const uint32_t*>(&v);
+            } else {
+              h[r / 2 + y] = pack_bf16x2(e0, e1);
+            }
+          }
+        }
+        good &= spin(&sh.o_done[b], ph ^ 1, wait);              // the sums have taken the buffer's last weights
+        uint8_t* to = weights + b * C::kPBytes + (r0 >> 3) * 2048 + key * 16;
+#pragma unroll
+        for (int v = 0; v < RT / 8; ++v) *reinterpret_cast<uint4*>(to + v * 2048) = make_uint4(h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full[b]);
+      }
+      if (!C::kSplit && i > p.p1 + 1) --g;       // the last step was this group's: the CTA's counter stands behind the piece
+      // sums of weights over the warp's keys: halves of the rows change places until a lane has one row's
+      {
+        float v[RT];
+#pragma unroll
+        for (int r = 0; r < RT; r += 2) {
+          const float2 y = apart(l[r / 2]);
+          v[r] = y.x;
+          v[r + 1] = y.y;
+        }
+        int d = 16;
+#pragma unroll
+        for (int n = RT / 2; n >= 1; n /= 2, d /= 2) {
+#pragma unroll
+          for (int r = 0; r < n; ++r) {
+            const bool upper = lane & d;
+            const float give = upper ? v[r] : v[r + n], keep = upper ? v[r + n] : v[r];
+            v[r] = keep + __shfl_xor_sync(~0u, give, d);
+          }
+        }
+        for (; d > 0; d /= 2) v[0] += __shfl_xor_sync(~0u, v[0], d);
+        if (lane % (32 / RT) == 0) sh.most[warp][r0 + lane / (32 / RT)] = v[0];
+      }
+      if (!failed) failed = !all_well(good & spin(&sh.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, wait), wait, 5, i);
+      if (failed && lane == 0 && !sh.fail) {
+        report(status, VDC_ERR_TIMEOUT, VDC_TREE_ATTENTION_KIND, 4, i, 0);
+        sh.fail = 1;
+      }
+      if (math_any(failed)) break;
+      // ---- the groups' sums meet: a thread looks at a row's references, then everybody at one of the 128 values
+      const bool whole = p.whole();
+      float* rec = reinterpret_cast<float*>(a.work) + (2 * blockIdx.x + (p.p1 == p.np ? 0 : 1)) * record_floats(a);
+      if (tid < R) {
+        const int from = C::kSplit ? tid / RT : 0;
+        float mm = -INFINITY, ll = 0.f, ref[C::kSums], sum[C::kSums];
+#pragma unroll
+        for (int k = 0; k < C::kSums; ++k) {
+          const float x = sh.ref[from + k][tid];
+          ref[k] = x == kNoRef ? -INFINITY : -x;
+          mm = fmaxf(mm, ref[k]);
+          const float(*part)[64] = &sh.most[4 * (from + k)];
+          sum[k] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+        }
+#pragma unroll
+        for (int k = 0; k < C::kSums; ++k) ll += sum[k] * (ref[k] == -INFINITY ? 1.f : exp2_ftz(ref[k] - mm));
+        if (sh.bad[turn & 1] || tid >= rows || row_of.token(tid) >= p.live) mm = -INFINITY, ll = 0.f;
+        const float scale = ll == 0.f ? 0.f : whole ? 1.f / ll : 1.f;
+        // a group that saw nothing has no part; one without a number passes that on
+#pragma unroll
+        for (int k = 0; k < C::kSums; ++k)
+          sh.factor[k][tid] = ll == 0.f || (ref[k] == -INFINITY && sum[k] == 0.f) ? 0.f : scale * (ref[k] == -INFINITY ? 1.f : exp2_ftz(ref[k] - mm));
+        if (!whole && tid < rows) *reinterpret_cast<float2*>(rec + rows * D + 2 * tid) = make_float2(mm, ll);
+      }
+      math_sync();
+      tc_fence_after();
+      constexpr int RO = R / 2;                       // rows that a group writes
+      float sum[RO];
+#pragma unroll
+      for (int k = 0; k < C::kSums; ++k) {
+        uint32_t x[RO];
+        tmem_load(col_o + lanes + k * C::kN + w * RO, x);
+#pragma unroll
+        for (int r = 0; r < RO; r += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(&sh.factor[k][w * RO + r]);
+          const float fs[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) sum[r + y] = (k ? sum[r + y] : 0.f) + (fs[y] == 0.f ? 0.f : __uint_as_float(x[r + y]) * fs[y]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < RO; ++r) {
+        const int rr = w * RO + r;
+        if (rr < rows) {
+          if (whole) sh.out[rr][key] = __float2bfloat16_rn(sum[r]);
+          else rec[rr * D + key] = sum[r];
+        }
+      }
+      tc_fence_before();
+      math_sync();
+      if (tid == 0) sh.bad[turn & 1] = 0;
+    }
+    write_zeros(a, sh, row_of, status, kMathWarps * 32);
+  }
+  tc_fence_before();
+  __syncthreads();
+  wait.drain();
+  if (warp == C::kScoreWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
   }
 }
 
@@ -912,7 +1601,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_consta
   total *= units;
   const long long first = before * units + (long long)u * np;
   ctas = (int)min((long long)ctas, total);
-  const int c0 = (int)(((first + 1) * ctas - 1) / total), c1 = (int)(((first + np) * ctas - 1) / total);
+  const int c0 = (int)quotient((first + 1) * ctas - 1, total), c1 = (int)quotient((first + np) * ctas - 1, total);
   if (c0 == c1) return;
   const long long rec = record_floats(a);
   auto record = [&](int c) { return reinterpret_cast<const float*>(a.work) + (2ll * c + (c == c1 ? 0 : 1)) * rec; };
@@ -988,17 +1677,30 @@ extern "C" long long vdc_tree_attention_bytes(const vdc_tree_attention_args* a) 
 }
 
 namespace {
-using Kernel = void (*)(const vdc_tree_attention_args, const CUtensorMap, const CUtensorMap, vdc_status*, uint64_t);
-const Kernel kKernels[2][3] = {{tree_attention<false, 1>, tree_attention<false, 2>, tree_attention<false, 4>},
-                               {tree_attention<true, 1>, tree_attention<true, 2>, tree_attention<true, 4>}};
+struct Variant {
+  void (*run)(const vdc_tree_attention_args, const CUtensorMap, const CUtensorMap, vdc_status*, uint64_t);
+  int threads, bytes;
+};
+template <bool kF8, int R>
+constexpr Variant keys() { return {tree_attention_keys<kF8, R>, KeysCfg<kF8, R>::kThreads, KeysCfg<kF8, R>::kBytes}; }
+template <bool kF8, int kReps>
+constexpr Variant lanes() { return {tree_attention<kF8, kReps>, Cfg<kF8>::kThreads, dynamic_bytes<kF8>()}; }
+const Variant kKeys[2][4] = {{keys<false, 8>(), keys<false, 16>(), keys<false, 32>(), keys<false, 64>()},
+                             {keys<true, 8>(), keys<true, 16>(), keys<true, 32>(), keys<true, 64>()}};
+const Variant kRowsOnLanes[2][3] = {{lanes<false, 1>(), lanes<false, 2>(), lanes<false, 4>()}, {lanes<true, 1>(), lanes<true, 2>(), lanes<true, 4>()}};
+int kKeysRows[2] = {64, 64};
 }  // namespace
 
 extern "C" cudaError_t vdc_tree_attention_prepare() {
-  for (int f8 = 0; f8 < 2; ++f8)
-    for (int i = 0; i < 3; ++i)
-      if (cudaError_t e = cudaFuncSetAttribute((const void*)kKernels[f8][i], cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               f8 ? dynamic_bytes<true>() : dynamic_bytes<false>()))
-        return e;
+  if (const char* e = getenv("FEW_BF16")) kKeysRows[0] = atoi(e);
+  if (const char* e = getenv("FEW_F8")) kKeysRows[1] = atoi(e);
+  auto prepare = [](const Variant& v) { return cudaFuncSetAttribute((const void*)v.run, cudaFuncAttributeMaxDynamicSharedMemorySize, v.bytes); };
+  for (int f8 = 0; f8 < 2; ++f8) {
+    for (const Variant& v : kKeys[f8])
+      if (cudaError_t e = prepare(v)) return e;
+    for (const Variant& v : kRowsOnLanes[f8])
+      if (cudaError_t e = prepare(v)) return e;
+  }
   return cudaSuccess;
 }
 
@@ -1009,6 +1711,7 @@ extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* 
                                                  cudaStream_t stream) {
   alignas(64) CUtensorMap maps[2] = {};
   const vdc_cache& c = a->cache;
+  const int rows = a->T * a->group, ctas = ctas_of(a, sms), units = a->B * c.n_kv * tiles_of(*a);
   if (!c.kind) {
     // a page of a head in two halves of 64 values, rows of 128 bytes
     const uint64_t shape[4] = {VDC_HEAD_DIM, VDC_KV_PAGE, (uint64_t)c.n_kv, (uint64_t)c.n_pages};
@@ -1020,10 +1723,9 @@ extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* 
         vdc_build_tma_desc(&maps[1], reinterpret_cast<const void*>(c.v), 2, 4, shape, vs, box, ones, 0, 0) != VDC_OK)
       return cudaErrorInvalidValue;
   }
-  const int rows = a->T * a->group, reps = rows <= 32 ? 2 : rows <= 64 ? 1 : 0, ctas = ctas_of(a, sms);
-  const int units = a->B * c.n_kv * ((rows + kRows - 1) / kRows);
-  kKernels[c.kind][reps]<<<ctas, c.kind ? Cfg<true>::kThreads : Cfg<false>::kThreads,
-                           c.kind ? dynamic_bytes<true>() : dynamic_bytes<false>(), stream>>>(*a, maps[0], maps[1], status, timeout_ns);
+  const Variant& v = rows <= kKeysRows[c.kind] ? kKeys[c.kind][rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 3]
+                                               : kRowsOnLanes[c.kind][rows <= 32 ? 2 : rows <= 64 ? 1 : 0];
+  v.run<<<ctas, v.threads, v.bytes, stream>>>(*a, maps[0], maps[1], status, timeout_ns);
   if (cudaError_t e = cudaGetLastError()) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)units, (unsigned)(((rows < kRows ? rows : kRows) + kJoinWarps - 1) / kJoinWarps));
