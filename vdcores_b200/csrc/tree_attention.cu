@@ -13,14 +13,10 @@
 // warps take the pages in turn: each reads its S, makes the weights P and puts them into tensor memory, first operand of
 // O += P V.  Each group sums its own O; the two meet at the end of the piece.
 //
-// Few rows (decoding, small trees) would leave most lanes idle: they are repeated over the lanes, each copy takes a part of every
-// page's keys (the other columns of its P stay zero), and the copies' sums meet like the groups'.
-//
 // e4m3 caches: a key's scale multiplies its scores.  A value's scale vs goes into its weight, P' = 2^(s + log2 vs - m), and the
 // sum of weights is that of P' / vs: one exponential, and no product per value.  Q becomes two e4m3 parts with a common power of two
 // per row, which are exact for bf16 values down to 2^-10 of the row's largest (below, 2^-18 of it), so K is used as it lies in
 // memory, in two passes of the 8-bit tensor cores.  V is widened to f16 (exact) by four more warps; P is f16 as well.
-#include <stdlib.h>
 #include "mk_stage.cuh"
 
 namespace vdc {
@@ -315,7 +311,7 @@ __device__ __forceinline__ float split_row(const uint4& v, unsigned sixteen, uin
   for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(sixteen, top, o));
   const int e = (int)(top >> 7);                            // exponent of the largest
   const int up = e == 0xFF ? 0 : min(126, 134 - max(e, 1)); // (rows of nearly nothing: as far as it goes)
-  const float mul = exp2f((float)up);
+  const float mul = __uint_as_float((uint32_t)(127 + up) << 23);      // 2^up
   uint32_t h[2] = {0, 0}, l[2] = {0, 0};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -327,7 +323,7 @@ __device__ __forceinline__ float split_row(const uint4& v, unsigned sixteen, uin
   }
   hi = make_uint2(h[0], h[1]);
   lo = make_uint2(l[0], l[1]);
-  return e == 0xFF ? NAN : exp2f((float)-up);
+  return e == 0xFF ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
 }
 
 __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int x, int head, int page, uint64_t* bar) {
@@ -370,6 +366,7 @@ __device__ __forceinline__ uint64_t seen_bits(const vdc_tree_attention_args& a, 
 template <int kThreads>
 __device__ __forceinline__ bool names_no_page(const vdc_tree_attention_args& a, const Piece& p, int tid, vdc_status* status) {
   bool found = false;
+  int which = 0;
   for (int i0 = tid; i0 < p.np; i0 += kThreads * 8) {
     int id[8];
 #pragma unroll
@@ -378,16 +375,21 @@ __device__ __forceinline__ bool names_no_page(const vdc_tree_attention_args& a, 
     for (int j = 0; j < 8; ++j)
       if (id[j] < 0 || id[j] >= a.cache.n_pages) {
         found = true;
-        report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, p.b, id[j]);
+        which = id[j];
       }
   }
+  if (found) report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, p.b, which);
   return found;
 }
 
-// A record of a piece: sums [rows][128], then (reference, sum of weights) [rows]; a multiple of 16 bytes.
+// The workspace: two records for each CTA, of a piece that reaches its unit's end and of one that does not: sums [rows][128] and
+// (reference, sum of weights) [rows], a multiple of 16 bytes.
 __host__ __device__ __forceinline__ long long record_floats(const vdc_tree_attention_args& a) {
   const int rows = a.T * a.group;
   return ((long long)(rows < kRows ? rows : kRows) * (D + 2) + 3) & ~3ll;
+}
+__device__ __forceinline__ float* record_of(const vdc_tree_attention_args& a, long long cta, bool reaches_end) {
+  return reinterpret_cast<float*>(a.work) + (2 * cta + (reaches_end ? 0 : 1)) * record_floats(a);
 }
 
 __device__ __forceinline__ __nv_bfloat16* out_row(const vdc_tree_attention_args& a, const RowOf& of, int b, int head, int r) {
@@ -407,12 +409,11 @@ __device__ __forceinline__ void write_zeros(const vdc_tree_attention_args& a, co
   }
 }
 
-template <bool kF8, int kReps>
+template <bool kF8>
 __global__ void __launch_bounds__(Cfg<kF8>::kThreads, 1)
 tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_constant__ CUtensorMap k_map,
                const __grid_constant__ CUtensorMap v_map, vdc_status* status, uint64_t timeout_ns) {
   using C = Cfg<kF8>;
-  constexpr int kKeys = PAGE / kReps, kLive = kRows / kReps;     // keys of a page that a copy takes, rows of a tile that may exist
   extern __shared__ __align__(1024) uint8_t dyn[];
   __shared__ TreeShared sh;
   uint8_t* ring = dyn + (-(int)smem_u32(dyn) & 1023);
@@ -684,14 +685,8 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
     Piece p;
     const int w = warp >> 2, quarter = warp & 3;                       // group, lanes of tensor memory
     const uint32_t lanes = tmem + ((uint32_t)quarter << 21);
-    const int slot = quarter * 32 + lane, tile_row = slot % kLive, key0 = (slot / kLive) * kKeys;
+    const int tile_row = quarter * 32 + lane;
     const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
-    {
-      const uint32_t zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < 32; i += 8) tmem_st8(lanes + kColP + w * 32 + i, zero);
-      tmem_st_wait();
-    }
     int c = 0, g = 0, tails = 0;      // pages of this group, of the CTA, and last pages of this group
     uint32_t* q_rows = reinterpret_cast<uint32_t*>(scratch);      // between pieces the scratch holds the next one's query rows
     for (int turn = 0; walk.next(p); ++turn) {
@@ -705,7 +700,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         const unsigned half = 0xFFFFu << (lane & 16);
         const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-        for (int rr = warp * 2 + (lane >> 4); rr < kLive; rr += kMathWarps * 2) {
+        for (int rr = warp * 2 + (lane >> 4); rr < kRows; rr += kMathWarps * 2) {
           const int qr = p.tile * kRows + rr;
           uint4 v = make_uint4(0, 0, 0, 0);
           if (qr < rows && row_of.token(qr) < p.live)
@@ -753,13 +748,13 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
           bits = live ? seen_bits(a, p, page, t) : 0;
           __syncwarp();
         }
-        uint32_t raw[kKeys];
+        uint32_t raw[PAGE];
         tc_fence_after();
-        tmem_load(lanes + kColS + w * PAGE + key0, raw);
+        tmem_load(lanes + kColS + w * PAGE, raw);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.s_empty[w]);
-        float s[kKeys];
+        float s[PAGE];
         if constexpr (kF8) good &= spin(&sh.par_full[gi & 3], (gi >> 2) & 1, wait);
         uint64_t poison = 0;
         if (tail && !kF8) {
@@ -794,22 +789,20 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
           ++tails;
         }
 #pragma unroll
-        for (int j = 0; j < kKeys; ++j) {
+        for (int j = 0; j < PAGE; ++j) {
           s[j] = __uint_as_float(raw[j]);
-          if constexpr (kF8) s[j] = fmaf(s[j] * sh.par[gi & 3][0][key0 + j], row_scale, sh.par[gi & 3][1][key0 + j]);
+          if constexpr (kF8) s[j] = fmaf(s[j] * sh.par[gi & 3][0][j], row_scale, sh.par[gi & 3][1][j]);
         }
         if (tail) {
-          bits >>= key0;
-          poison >>= key0;
 #pragma unroll
-          for (int j = 0; j < kKeys; ++j) {
+          for (int j = 0; j < PAGE; ++j) {
             if (!((bits >> j) & 1)) s[j] = -INFINITY;
             else if (!kF8 && ((poison >> j) & 1)) s[j] = NAN;
           }
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < kKeys; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+        for (int j = 0; j < PAGE; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if constexpr (!kF8) top *= row_scale;
         if (__any_sync(~0u, top > m + C::kSlack)) {
@@ -830,15 +823,15 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
           }
         }
         const float ref = (m == -INFINITY ? 0.f : m) - C::kLift;
-        uint32_t pk[kKeys / 2];
+        uint32_t pk[PAGE / 2];
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < kKeys; j += 2) {
+        for (int j = 0; j < PAGE; j += 2) {
           const float p0 = kF8 ? exp2_ftz(s[j] - ref) : exp2_ftz(fmaf(s[j], row_scale, -ref));
           const float p1 = kF8 ? exp2_ftz(s[j + 1] - ref) : exp2_ftz(fmaf(s[j + 1], row_scale, -ref));
           if constexpr (kF8) {
-            sum[j & 3] = fmaf(p0, sh.par[gi & 3][2][key0 + j], sum[j & 3]);
-            sum[(j + 1) & 3] = fmaf(p1, sh.par[gi & 3][2][key0 + j + 1], sum[(j + 1) & 3]);
+            sum[j & 3] = fmaf(p0, sh.par[gi & 3][2][j], sum[j & 3]);
+            sum[(j + 1) & 3] = fmaf(p1, sh.par[gi & 3][2][j + 1], sum[(j + 1) & 3]);
             const __half2 h = __floats2half2_rn(p0, p1);
             pk[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
           } else {
@@ -854,7 +847,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
           break;
         }
         tc_fence_after();
-        tmem_store(lanes + kColP + w * 32 + key0 / 2, pk);
+        tmem_store(lanes + kColP + w * 32, pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -866,28 +859,20 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       if (!failed && has) failed = !all_well(spin(&sh.o_done[w], (c & 1) ^ 1, wait), wait, 5, n);
       sh.stats[warp][lane] = make_float2(m, l);
       if (math_any(failed)) break;
-      // ---- the row's copies meet: statistics first (every copy looks at all), then 32 columns at a time
-      float mm = -INFINITY, ll = 0.f;
-      {
-        float2 st[2 * kReps];
-#pragma unroll
-        for (int k = 0; k < 2 * kReps; ++k) {
-          st[k] = sh.stats[(k / kReps) * 4 + (k % kReps) * (4 / kReps) + (tile_row >> 5)][lane];
-          mm = fmaxf(mm, st[k].x);
-        }
-        // a copy that saw nothing has no weight; one without a number passes that on
-#pragma unroll
-        for (int k = 0; k < 2 * kReps; ++k) ll += st[k].y * (st[k].x == -INFINITY ? 1.f : exp2_ftz(st[k].x - mm));
-      }
+      // ---- the groups' sums meet: statistics first (both look at both), then 32 columns at a time
+      const float2 other = sh.stats[warp ^ 4][lane];
+      float mm = fmaxf(m, other.x);
+      // a group that saw nothing has no weight; one without a number passes that on
+      float ll = l * (m == -INFINITY ? 1.f : exp2_ftz(m - mm)) + other.y * (other.x == -INFINITY ? 1.f : exp2_ftz(other.x - mm));
       if (sh.bad[turn & 1] || !live) mm = -INFINITY, ll = 0.f;
       const bool whole = p.whole(), none = !has || ll == 0.f || (m == -INFINITY && l == 0.f);
       const float f = (m == -INFINITY ? 1.f : exp2_ftz(m - mm)) * (whole && ll != 0.f ? 1.f / ll : 1.f);
-      float* rec = reinterpret_cast<float*>(a.work) + (2 * blockIdx.x + (p.p1 == p.np ? 0 : 1)) * record_floats(a);
+      float* rec = record_of(a, blockIdx.x, p.p1 == p.np);
       const int tile_rows = min(rows - p.tile * kRows, kRows);
-      if (!whole && tid < min(kLive, tile_rows)) *reinterpret_cast<float2*>(rec + min(rows, kRows) * D + 2 * tid) = make_float2(mm, ll);
-      __nv_bfloat16* to[kLive / 32];
+      if (!whole && tid < tile_rows) *reinterpret_cast<float2*>(rec + min(rows, kRows) * D + 2 * tid) = make_float2(mm, ll);
+      __nv_bfloat16* to[kRows / 32];
 #pragma unroll
-      for (int k = 0; k < kLive / 32; ++k) {
+      for (int k = 0; k < kRows / 32; ++k) {
         const int rr = (tid >> 3) + k * 32;
         to[k] = out_row(a, row_of, p.b, p.head, p.tile * kRows + rr) + (tid & 7) * 4;
       }
@@ -908,16 +893,12 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         }
         math_sync();
 #pragma unroll
-        for (int k = 0; k < kLive / 32; ++k) {
+        for (int k = 0; k < kRows / 32; ++k) {
           const int rr = (tid >> 3) + k * 32;
           if (rr < tile_rows) {
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int q = 0; q < 2 * kReps; ++q) {
-              const int from = (q / kReps) * 4 + (q % kReps) * (4 / kReps) + k;
-              const float4 x = *reinterpret_cast<const float4*>(theirs + from * 32 * kScratchRow);
-              sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-            }
+            const float4 x = *reinterpret_cast<const float4*>(theirs + k * 32 * kScratchRow);
+            const float4 y = *reinterpret_cast<const float4*>(theirs + (4 + k) * 32 * kScratchRow);
+            const float4 sum = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
             if (whole) *reinterpret_cast<uint2*>(to[k] + col) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
             else *reinterpret_cast<float4*>(rec + rr * D + col + (tid & 7) * 4) = sum;
           }
@@ -961,8 +942,9 @@ struct KeysCfg {
   static constexpr int kQBytes = kN * D * 2;                            // bf16, or twice e4m3
   static constexpr int kPBytes = kN / 8 * 2048;                         // of one buffer of two
   static constexpr int kWide = kF8 ? 2 * PAGE * D * 2 : 0;              // widened values of a step, two buffers
-  static constexpr int kBytes = 1024 + kSlots * kPart + 2 * kWide + kQBytes + 2 * kPBytes;
-  static_assert(kBytes + 14336 <= 232448, "shared memory of a CTA");
+  static constexpr int kQBufs = R > 32 ? 1 : 2;                         // (what fits)
+  static constexpr int kBytes = 1024 + kSlots * kPart + 2 * kWide + kQBufs * kQBytes + 2 * kPBytes;
+  static_assert(kBytes + 15360 <= 232448, "shared memory of a CTA");
   static constexpr int kLoadWarp = kMathWarps + (kF8 ? 8 : 0), kScoreWarp = kLoadWarp + 1, kSumWarp = kLoadWarp + 2;
   static constexpr int kThreads = kF8 ? 640 : 384, kMathRegs = kF8 ? 128 : 208, kOtherRegs = kF8 ? 72 : 88;
   // powers of two by which a score may exceed its reference, and by which f16 weights are kept larger (2^15 at most)
@@ -973,9 +955,12 @@ constexpr float kNoRef = 1e30f;              // minus the reference of a row tha
 struct KeysShared : ShareShared {
   uint64_t full[8], empty[8], q_full, s_full[2], s_empty[2], p_full[2], o_done[2], v_full[2], v_empty[2], checked;
   uint32_t tmem;
-  uint64_t sees[64];                         // of a drafted token: the rows that attend to it
-  __nv_bfloat16* out[64];                    // of a row: its result
-  alignas(16) float mul[64];                 // of a row: what its scores are multiplied by
+  Piece piece[2];                            // the math warps' (this one and the next, live < 0: there is none), and where their walk is
+  long long walk_x, walk_base;
+  int walk_b;
+  uint64_t sees[2][64];                      // (of this piece and of the next) of a drafted token: the rows that attend to it
+  __nv_bfloat16* out[2][64];                 // of a row: its result
+  alignas(16) float mul[2][64];              // of a row: what its scores are multiplied by
   alignas(16) float ref[2][64];              // of a group's rows: minus the reference
   alignas(16) float factor[2][64];           // what their sums are multiplied by
   float most[kMathWarps][64];                // of a warp's rows: largest score, or sum of weights
@@ -991,6 +976,11 @@ __device__ __forceinline__ bool group_any(int w, bool x) {
   asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, %2, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
                : "=r"(r) : "r"((int)x), "r"(2 + w) : "memory");
   return r != 0;
+}
+
+__device__ __forceinline__ void st_global_bf16(__nv_bfloat16* p, float x) {
+  const __nv_bfloat16 v = __float2bfloat16_rn(x);
+  asm volatile("st.global.b16 [%0], %1;" ::"l"(__cvta_generic_to_global(p)), "h"(__bfloat16_as_ushort(v)));
 }
 
 // The largest of a warp's values, NaN left out.
@@ -1047,7 +1037,7 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
   uint8_t* ring = dyn + (-(int)smem_u32(dyn) & 1023);
   uint8_t* wide = ring + C::kSlots * C::kPart;
   uint8_t* q_rows = wide + 2 * C::kWide;
-  uint8_t* weights = q_rows + C::kQBytes;
+  uint8_t* weights = q_rows + C::kQBufs * C::kQBytes;
   const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
   const Waiter wait{&sh.fail, status, timeout_ns, VDC_TREE_ATTENTION_KIND};
   const int rows = a.T * a.group;
@@ -1141,7 +1131,9 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
       const uint32_t d0 = __shfl_sync(~0u, col_s, 0);
       uint32_t turn = 0;
       while (ok && walk.next(p)) {
-        uint32_t good = spin(&sh.q_full, turn++ & 1, wait);
+        uint32_t good = spin(&sh.q_full, turn & 1, wait);
+        const uint64_t q = q_desc + (C::kQBufs > 1 ? turn & 1 : 0) * (C::kQBytes >> 4);
+        ++turn;
         for (int i = p.p0; i < p.p1; i += 2, ++g) {
           const uint32_t st = key_slot(g), w = g & 1;
           good &= spin(&sh.s_empty[w], ((g >> 1) & 1) ^ 1, wait) & spin(&sh.full[st], key_phase(g), wait);
@@ -1154,13 +1146,13 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
             if constexpr (kF8) {
 #pragma unroll
               for (int j = 0; j < 8; ++j)          // the rows' upper parts, then their lower ones
-                umma_f8(d, k + (j & 3) * 2, q_desc + (j >> 2) * (C::kN * 128 >> 4) + (j & 3) * 2, id, j > 0);
+                umma_f8(d, k + (j & 3) * 2, q + (j >> 2) * (C::kN * 128 >> 4) + (j & 3) * 2, id, j > 0);
               umma_commit(&sh.s_full[w]);
               umma_commit(&sh.empty[st]);
             } else {
 #pragma unroll
               for (int j = 0; j < 8; ++j)
-                umma_bf16(d, k + (j >> 2) * (C::kPart >> 5) + (j & 3) * 2, q_desc + (j >> 2) * (C::kN * 128 >> 4) + (j & 3) * 2, id, j > 0);
+                umma_bf16(d, k + (j >> 2) * (C::kPart >> 5) + (j & 3) * 2, q + (j >> 2) * (C::kN * 128 >> 4) + (j & 3) * 2, id, j > 0);
               umma_commit(&sh.s_full[w]);
               umma_commit(&sh.empty[st]);
             }
@@ -1250,17 +1242,31 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
   } else {
     // ---- scores to weights, sums to results
     set_registers<C::kMathRegs, true>();
-    Walk walk(a, sh);
-    Piece p;
     const int w = warp >> 2, key = tid & 127, r0 = C::kSplit ? w * RT : 0;           // group, the thread's key of a step, its first row
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
-    const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
-    const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+    const uint32_t mine_o = col_o + lanes + (C::kSplit ? 0 : w * C::kN) + r0;        // the group's sums of the warp's 32 values
     uint32_t g = 0, tails = 0;        // steps of the CTA, and those with drafted tokens
-    for (int turn = 0; walk.next(p); ++turn) {
-      // ---- the rows to shared memory as the tensor cores read them (half a warp loads one), the drafted tokens' masks, and a look
-      // at the page table; all loads first
-      const int sub = lane & 15, end = min(p.total(), p.p1 * PAGE);
+    uint64_t l[RT / 2];               // sums of weights of two rows each
+    // One thread's walk over the pieces (in shared memory: there are no registers to spare).
+    auto step = [&](int turn) {
+      Walk walk(a, sh);
+      if (turn > 0) walk.x = sh.walk_x, walk.base = sh.walk_base, walk.b = sh.walk_b;
+      Piece p;
+      if (!walk.next(p)) p.live = -1;
+      sh.piece[turn & 1] = p;
+      sh.walk_x = walk.x;
+      sh.walk_base = walk.base;
+      sh.walk_b = walk.b;
+    };
+    // A piece's rows to shared memory as the tensor cores read them (half a warp loads one), the drafted tokens' masks, and a look at the
+    // page table; all loads first.
+    auto prepare = [&](int turn) {
+      const int sub = lane & 15, buf = turn & 1;
+      const Piece p = sh.piece[buf];
+      const int end = min(p.total(), p.p1 * PAGE);
+      const float scale = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);
+      const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+      uint8_t* rows_at = q_rows + (C::kQBufs > 1 ? buf : 0) * C::kQBytes;
       uint4 q[(R + 15) / 16];
 #pragma unroll
       for (int k = 0; k < (R + 15) / 16; ++k) {
@@ -1277,7 +1283,7 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
           if (t < p.live) words[h] = a.mask ? (uint64_t)__ldg(reinterpret_cast<const long long*>(a.mask) + p.b * a.mask_b + t * a.mask_t) : (2ull << t) - 1;
         }
       }
-      if (names_no_page<kMathWarps * 32>(a, p, tid, status)) sh.bad[turn & 1] = 1;
+      if (names_no_page<kMathWarps * 32>(a, p, tid, status)) sh.bad[buf] = 1;
 #pragma unroll
       for (int k = 0; k < (R + 15) / 16; ++k) {
         const int r = k * 16 + warp * 2 + (lane >> 4);
@@ -1285,47 +1291,150 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
         v.x ^= sign; v.y ^= sign; v.z ^= sign; v.w ^= sign;
         float mul = scale;
         if constexpr (!kF8) {
-          if (r < R) *reinterpret_cast<uint4*>(q_rows + (sub >> 3) * (C::kN * 128) + r * 128 + (((sub & 7) ^ (r & 7)) << 4)) = v;
+          if (r < R) *reinterpret_cast<uint4*>(rows_at + (sub >> 3) * (C::kN * 128) + r * 128 + (((sub & 7) ^ (r & 7)) << 4)) = v;
         } else {
           uint2 hi, lo;
           mul *= split_row(v, 0xFFFFu << (lane & 16), hi, lo);
-          uint8_t* to = q_rows + r * 128 + (((sub >> 1) ^ (r & 7)) << 4) + (sub & 1) * 8;
+          uint8_t* to = rows_at + r * 128 + (((sub >> 1) ^ (r & 7)) << 4) + (sub & 1) * 8;
           if (r < R) {
             *reinterpret_cast<uint2*>(to) = hi;
             *reinterpret_cast<uint2*>(to + C::kN * 128) = lo;
           }
         }
         if (r < R && sub == 0) {
-          sh.mul[r] = mul;
-          sh.out[r] = out_row(a, row_of, p.b, p.head, r);
+          sh.mul[buf][r] = mul;
+          sh.out[buf][r] = out_row(a, row_of, p.b, p.head, r);
         }
       }
-      if (tid < 128) sh.ref[tid >> 6][tid & 63] = kNoRef;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
       if (end > p.ctx) {
-        // tokens that attend to drafted token j, then rows; a warp takes eight tokens
+        // tokens that attend to drafted token j, then rows; the warps take turns
         const int t0 = row_of.token(lane), t1 = row_of.token(lane + 32);
 #pragma unroll 1
-        for (int j = warp * 8; j < min(warp * 8 + 8, p.live); ++j) {
+        for (int j = warp; j < p.live; j += kMathWarps) {
           const uint64_t tokens = (uint64_t)__ballot_sync(~0u, (words[1] >> j) & 1) << 32 | __ballot_sync(~0u, (words[0] >> j) & 1);
           const uint32_t lower = __ballot_sync(~0u, t0 < 64 && ((tokens >> t0) & 1)), upper = __ballot_sync(~0u, t1 < 64 && ((tokens >> t1) & 1));
-          if (lane == 0) sh.sees[j] = (uint64_t)upper << 32 | lower;
+          if (lane == 0) sh.sees[buf][j] = (uint64_t)upper << 32 | lower;
         }
       }
-      math_sync();
+    };
 
-      uint64_t l[RT / 2];                     // sums of weights of two rows each
+    // Round `turn` ends piece turn - 1 and works through piece `turn`, whose rows were prepared in front of that end: the scores
+    // are at its first steps while the sums of the piece before are still on their way.
+    bool failed = false;
+    uint32_t good = 1;
+    if (tid == 0) step(0);
+    math_sync();
+    for (int turn = 0;; ++turn) {
+      const bool more = sh.piece[turn & 1].live >= 0;
+      if (C::kQBufs > 1 && more) prepare(turn);
+      if (turn > 0) {
+        const int buf = (turn - 1) & 1;
+        const Piece& p = sh.piece[buf];
+        // sums of weights over the warp's keys: halves of the rows change places until a lane has one row's
+        {
+          float v[RT];
+#pragma unroll
+          for (int r = 0; r < RT; r += 2) {
+            const float2 y = apart(l[r / 2]);
+            v[r] = y.x;
+            v[r + 1] = y.y;
+          }
+          int d = 16;
+#pragma unroll
+          for (int n = RT / 2; n >= 1; n /= 2, d /= 2) {
+#pragma unroll
+            for (int r = 0; r < n; ++r) {
+              const bool upper = lane & d;
+              const float give = upper ? v[r] : v[r + n], keep = upper ? v[r + n] : v[r];
+              v[r] = keep + __shfl_xor_sync(~0u, give, d);
+            }
+          }
+          for (; d > 0; d /= 2) v[0] += __shfl_xor_sync(~0u, v[0], d);
+          if (lane % (32 / RT) == 0) sh.most[warp][r0 + lane / (32 / RT)] = v[0];
+        }
+        if (!failed) failed = !all_well(good & spin(&sh.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, wait), wait, 5, p.p1);
+        if (failed && lane == 0 && !sh.fail) {
+          report(status, VDC_ERR_TIMEOUT, VDC_TREE_ATTENTION_KIND, 4, p.p1, 0);
+          sh.fail = 1;
+        }
+        if (math_any(failed)) break;
+        // ---- the groups' sums meet: a thread looks at a row's references, then everybody at one of the 128 values
+        const bool whole = p.whole();
+        float* rec = record_of(a, blockIdx.x, p.p1 == p.np);
+        if (tid < R) {
+          const int from = C::kSplit ? tid / RT : 0;
+          float mm = -INFINITY, ll = 0.f, ref[C::kSums], sum[C::kSums];
+#pragma unroll
+          for (int k = 0; k < C::kSums; ++k) {
+            const float x = sh.ref[from + k][tid];
+            ref[k] = x == kNoRef ? -INFINITY : -x;
+            mm = fmaxf(mm, ref[k]);
+            const float(*part)[64] = &sh.most[4 * (from + k)];
+            sum[k] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+          }
+#pragma unroll
+          for (int k = 0; k < C::kSums; ++k) ll += sum[k] * (ref[k] == -INFINITY ? 1.f : exp2_ftz(ref[k] - mm));
+          if (sh.bad[buf] || tid >= rows || row_of.token(tid) >= p.live) mm = -INFINITY, ll = 0.f;
+          const float scale = ll == 0.f ? 0.f : whole ? 1.f / ll : 1.f;
+          // a group that saw nothing has no part; one without a number passes that on
+#pragma unroll
+          for (int k = 0; k < C::kSums; ++k)
+            sh.factor[k][tid] = ll == 0.f || (ref[k] == -INFINITY && sum[k] == 0.f) ? 0.f : scale * (ref[k] == -INFINITY ? 1.f : exp2_ftz(ref[k] - mm));
+          if (!whole && tid < rows) *reinterpret_cast<float2*>(rec + rows * D + 2 * tid) = make_float2(mm, ll);
+        }
+        math_sync();
+        tc_fence_after();
+        constexpr int RO = R / 2;                       // rows that a group writes
+        float sum[RO];
+#pragma unroll
+        for (int k = 0; k < C::kSums; ++k) {
+          uint32_t x[RO];
+          tmem_load(col_o + lanes + k * C::kN + w * RO, x);
+#pragma unroll
+          for (int r = 0; r < RO; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(&sh.factor[k][w * RO + r]);
+            const float fs[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) sum[r + y] = (k ? sum[r + y] : 0.f) + (fs[y] == 0.f ? 0.f : __uint_as_float(x[r + y]) * fs[y]);
+          }
+        }
+        tc_fence_before();
+        if (whole) {
+#pragma unroll
+          for (int r = 0; r < RO; r += 4) {
+            __nv_bfloat16* to[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) to[y] = sh.out[buf][w * RO + r + y];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (w * RO + r + y < rows) st_global_bf16(to[y] + key, sum[r + y]);
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < RO; ++r)
+            if (w * RO + r < rows) rec[(w * RO + r) * D + key] = sum[r];
+        }
+        if (tid == 0) sh.bad[buf] = 0;
+      }
+      if (C::kQBufs == 1 && more) prepare(turn);
+      math_sync();
+      if (tid == 128) step(turn + 1);
+      if (tid < 128) sh.ref[tid >> 6][tid & 63] = kNoRef;
+      math_sync();
+      if (!more) break;
+      const int ctx = sh.piece[turn & 1].ctx, p1 = sh.piece[turn & 1].p1, end = min(sh.piece[turn & 1].total(), p1 * PAGE);
+      const float* mul_of = sh.mul[turn & 1];
+      const uint64_t* sees = sh.sees[turn & 1];
 #pragma unroll
       for (int r = 0; r < RT / 2; ++r) l[r] = 0;
-      const uint32_t mine_o = col_o + lanes + (C::kSplit ? 0 : w * C::kN) + r0;      // the group's sums of the warp's 32 values
-      uint32_t good = 1;
-      bool failed = false;
-      int i = p.p0;
+      good = 1;
+      int i = sh.piece[turn & 1].p0;
       if (!C::kSplit && (g & 1) != (uint32_t)w) i += 2, ++g;
       bool first = true;
-      for (; i < p.p1; i += C::kSplit ? 2 : 4, g += C::kSplit ? 1 : 2) {
+      for (; i < p1; i += C::kSplit ? 2 : 4, g += C::kSplit ? 1 : 2) {
         const uint32_t st = key_slot(g), b = g & 1, ph = (g >> 1) & 1;
         const int mine = i * PAGE + key;                      // the key among the sequence's
         good &= spin(&sh.s_full[b], ph, wait);
@@ -1352,16 +1461,16 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
         const uint64_t ks2 = two(ks, ks), lg2 = two(lg, lg);
 #pragma unroll
         for (int r = 0; r < RT; r += 4) {
-          const ulonglong2 mul = *reinterpret_cast<const ulonglong2*>(&sh.mul[r0 + r]);
+          const ulonglong2 mul = *reinterpret_cast<const ulonglong2*>(&mul_of[r0 + r]);
           const uint64_t x0 = two(__uint_as_float(x[r]), __uint_as_float(x[r + 1])), x1 = two(__uint_as_float(x[r + 2]), __uint_as_float(x[r + 3]));
           z[r / 2] = kF8 ? fma2(mul2(x0, ks2), mul.x, lg2) : mul2(x0, mul.x);
           z[r / 2 + 1] = kF8 ? fma2(mul2(x1, ks2), mul.y, lg2) : mul2(x1, mul.y);
         }
-        if ((i + 2) * PAGE > min(p.ctx, end)) {
+        if ((i + 2) * PAGE > min(ctx, end)) {
           // drafted tokens, and what is none of the piece's keys.  The values of the latter become zeros (a weight of zero would not
           // do: zero times NaN); so do those of a drafted token that are no numbers, whose readers get none by their scores
-          const int j = mine - p.ctx;
-          uint64_t see = mine >= end ? 0 : j < 0 ? ~0ull : sh.sees[j];
+          const int j = mine - ctx;
+          uint64_t see = mine >= end ? 0 : j < 0 ? ~0ull : sees[j];
           bool none = false;
           if constexpr (kF8) {
             if (mine >= end) inv = 0.f;
@@ -1432,21 +1541,23 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
           }
           group_any(w, false);
           tc_fence_after();
-          uint32_t o[RT];
-          if (!first) tmem_load(mine_o, o);
+          constexpr int RC = RT < 16 ? RT : 16;             // (a part at a time: registers)
 #pragma unroll
-          for (int r = 0; r < RT; r += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(&sh.factor[w][r0 + r]);
-            l[r / 2] = mul2(l[r / 2], two(f.x, f.y));
-            l[r / 2 + 1] = mul2(l[r / 2 + 1], two(f.z, f.w));
-            const float fs[4] = {f.x, f.y, f.z, f.w};
+          for (int c = 0; c < RT; c += RC) {
+            uint32_t o[RC];
+            if (!first) tmem_load(mine_o + c, o);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) o[r + y] = __float_as_uint(__uint_as_float(o[r + y]) * fs[y]);
+            for (int r = 0; r < RC; r += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(&sh.factor[w][r0 + c + r]);
+              l[(c + r) / 2] = mul2(l[(c + r) / 2], two(f.x, f.y));
+              l[(c + r) / 2 + 1] = mul2(l[(c + r) / 2 + 1], two(f.z, f.w));
+              const float fs[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+              for (int y = 0; y < 4; ++y) o[r + y] = __float_as_uint(__uint_as_float(o[r + y]) * fs[y]);
+            }
+            if (!first) tmem_store_any(mine_o + c, o);
           }
-          if (!first) {
-            tmem_store_any(mine_o, o);
-            tmem_st_wait();
-          }
+          if (!first) tmem_st_wait();
         }
         first = false;
         // ---- weights
@@ -1477,86 +1588,7 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.p_full[b]);
       }
-      if (!C::kSplit && i > p.p1 + 1) --g;       // the last step was this group's: the CTA's counter stands behind the piece
-      // sums of weights over the warp's keys: halves of the rows change places until a lane has one row's
-      {
-        float v[RT];
-#pragma unroll
-        for (int r = 0; r < RT; r += 2) {
-          const float2 y = apart(l[r / 2]);
-          v[r] = y.x;
-          v[r + 1] = y.y;
-        }
-        int d = 16;
-#pragma unroll
-        for (int n = RT / 2; n >= 1; n /= 2, d /= 2) {
-#pragma unroll
-          for (int r = 0; r < n; ++r) {
-            const bool upper = lane & d;
-            const float give = upper ? v[r] : v[r + n], keep = upper ? v[r + n] : v[r];
-            v[r] = keep + __shfl_xor_sync(~0u, give, d);
-          }
-        }
-        for (; d > 0; d /= 2) v[0] += __shfl_xor_sync(~0u, v[0], d);
-        if (lane % (32 / RT) == 0) sh.most[warp][r0 + lane / (32 / RT)] = v[0];
-      }
-      if (!failed) failed = !all_well(good & spin(&sh.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, wait), wait, 5, i);
-      if (failed && lane == 0 && !sh.fail) {
-        report(status, VDC_ERR_TIMEOUT, VDC_TREE_ATTENTION_KIND, 4, i, 0);
-        sh.fail = 1;
-      }
-      if (math_any(failed)) break;
-      // ---- the groups' sums meet: a thread looks at a row's references, then everybody at one of the 128 values
-      const bool whole = p.whole();
-      float* rec = reinterpret_cast<float*>(a.work) + (2 * blockIdx.x + (p.p1 == p.np ? 0 : 1)) * record_floats(a);
-      if (tid < R) {
-        const int from = C::kSplit ? tid / RT : 0;
-        float mm = -INFINITY, ll = 0.f, ref[C::kSums], sum[C::kSums];
-#pragma unroll
-        for (int k = 0; k < C::kSums; ++k) {
-          const float x = sh.ref[from + k][tid];
-          ref[k] = x == kNoRef ? -INFINITY : -x;
-          mm = fmaxf(mm, ref[k]);
-          const float(*part)[64] = &sh.most[4 * (from + k)];
-          sum[k] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
-        }
-#pragma unroll
-        for (int k = 0; k < C::kSums; ++k) ll += sum[k] * (ref[k] == -INFINITY ? 1.f : exp2_ftz(ref[k] - mm));
-        if (sh.bad[turn & 1] || tid >= rows || row_of.token(tid) >= p.live) mm = -INFINITY, ll = 0.f;
-        const float scale = ll == 0.f ? 0.f : whole ? 1.f / ll : 1.f;
-        // a group that saw nothing has no part; one without a number passes that on
-#pragma unroll
-        for (int k = 0; k < C::kSums; ++k)
-          sh.factor[k][tid] = ll == 0.f || (ref[k] == -INFINITY && sum[k] == 0.f) ? 0.f : scale * (ref[k] == -INFINITY ? 1.f : exp2_ftz(ref[k] - mm));
-        if (!whole && tid < rows) *reinterpret_cast<float2*>(rec + rows * D + 2 * tid) = make_float2(mm, ll);
-      }
-      math_sync();
-      tc_fence_after();
-      constexpr int RO = R / 2;                       // rows that a group writes
-      float sum[RO];
-#pragma unroll
-      for (int k = 0; k < C::kSums; ++k) {
-        uint32_t x[RO];
-        tmem_load(col_o + lanes + k * C::kN + w * RO, x);
-#pragma unroll
-        for (int r = 0; r < RO; r += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(&sh.factor[k][w * RO + r]);
-          const float fs[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-          for (int y = 0; y < 4; ++y) sum[r + y] = (k ? sum[r + y] : 0.f) + (fs[y] == 0.f ? 0.f : __uint_as_float(x[r + y]) * fs[y]);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < RO; ++r) {
-        const int rr = w * RO + r;
-        if (rr < rows) {
-          if (whole) sh.out[rr][key] = __float2bfloat16_rn(sum[r]);
-          else rec[rr * D + key] = sum[r];
-        }
-      }
-      tc_fence_before();
-      math_sync();
-      if (tid == 0) sh.bad[turn & 1] = 0;
+      if (!C::kSplit && i > p1 + 1) --g;       // the last step was this group's: the CTA's counter stands behind the piece
     }
     write_zeros(a, sh, row_of, status, kMathWarps * 32);
   }
@@ -1570,59 +1602,70 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
 }
 
 // Joins the pieces of units that several CTAs shared: a warp per row, lane i the values 4i .. 4i + 3.  Pieces are taken in order,
-// so that the result does not depend on when they came.
+// so that the result does not depend on when they came.  What it needs to know of the sequences it looks up before the kernel in front
+// has ended (that one began when everything before it was done).
 constexpr int kJoinWarps = 4;
 __global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_constant__ vdc_tree_attention_args a, int ctas) {
   __shared__ long long part[2][kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rr = blockIdx.y * kJoinWarps + warp;
   const int tiles = tiles_of(a), units = a.cache.n_kv * tiles, b = blockIdx.x / units, u = blockIdx.x - b * units;
   const int rows = a.T * a.group, r = (u % tiles) * kRows + rr, rec_rows = min(rows, kRows);
-  grid_dep_wait();
   // pages of all sequences and of those in front of this one
-  const int2 seq = seq_load(a, b);
+  const int np = pages_of(seq_load(a, b));
   long long total = 0, before = 0;
   for (int i = threadIdx.x; i < a.B; i += kJoinWarps * 32) {
     const int n = pages_of(seq_load(a, i));
     total += n;
     before += i < b ? n : 0;
   }
+  if (a.B > 1) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(~0u, total, o);
-    before += __shfl_xor_sync(~0u, before, o);
+    for (int o = 16; o > 0; o >>= 1) {
+      total += __shfl_xor_sync(~0u, total, o);
+      before += __shfl_xor_sync(~0u, before, o);
+    }
+    if (lane == 0) part[0][warp] = total, part[1][warp] = before;
+    __syncthreads();
+    total = before = 0;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) total += part[0][i], before += part[1][i];
+  } else {
+    total = np;
   }
-  if (lane == 0) part[0][warp] = total, part[1][warp] = before;
-  __syncthreads();
-  total = before = 0;
-#pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) total += part[0][i], before += part[1][i];
-  const int np = pages_of(seq);
   if (np == 0 || r >= rows || rr >= kRows) return;
   total *= units;
   const long long first = before * units + (long long)u * np;
   ctas = (int)min((long long)ctas, total);
   const int c0 = (int)quotient((first + 1) * ctas - 1, total), c1 = (int)quotient((first + np) * ctas - 1, total);
   if (c0 == c1) return;
-  const long long rec = record_floats(a);
-  auto record = [&](int c) { return reinterpret_cast<const float*>(a.work) + (2ll * c + (c == c1 ? 0 : 1)) * rec; };
-  auto stats = [&](int c) { return __ldg(reinterpret_cast<const float2*>(record(c) + rec_rows * D + 2 * rr)); };
+  __nv_bfloat16* out = out_row(a, RowOf(a.group), b, u / tiles, r) + lane * 4;
+  const float* rec0 = record_of(a, c0, false);
+  const long long step = record_floats(a);
+  auto record = [&](int c) { return rec0 + (2 * (c - c0) - (c == c1 ? 1 : 0)) * step; };
+  auto stats = [&](int c) { return __ldcg(reinterpret_cast<const float2*>(record(c) + rec_rows * D + 2 * rr)); };
+  grid_dep_wait();
   float2 st = c0 + lane <= c1 ? stats(c0 + lane) : make_float2(-INFINITY, 0.f);
   float m = st.x;
   for (int c = c0 + 32 + lane; c <= c1; c += 32) m = fmaxf(m, stats(c).x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
   float l = 0.f;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int c = c0; c <= c1; c += 32) {
-    if (c > c0) st = c + lane <= c1 ? stats(c + lane) : make_float2(-INFINITY, 0.f);
-    const float mine = st.x == -INFINITY ? 1.f : exp2_ftz(st.x - m);      // no reference: nothing, or no number
-    l += st.y * mine;
     const int n = min(32, c1 - c + 1);
+    if (c > c0) st = c + lane <= c1 ? stats(c + lane) : make_float2(-INFINITY, 0.f);
+    float mine = 0.f;
     for (int i = 0; i < n; i += 8) {
       float4 x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        x[j] = i + j < n ? __ldg(reinterpret_cast<const float4*>(record(c + i + j) + rr * D) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[j] = i + j < n ? __ldcg(reinterpret_cast<const float4*>(record(c + i + j) + rr * D) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i == 0) {                       // (behind the first loads: both are on their way)
+        if (c == c0) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        }
+        mine = st.x == -INFINITY ? 1.f : exp2_ftz(st.x - m);      // no reference: nothing, or no number
+        l += st.y * mine;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float f = __shfl_sync(~0u, mine, (i + j) & 31);
@@ -1633,8 +1676,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_consta
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(out_row(a, RowOf(a.group), b, u / tiles, r) + lane * 4) =
-      make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
 }
 
 template <bool kF8>
@@ -1683,24 +1725,16 @@ struct Variant {
 };
 template <bool kF8, int R>
 constexpr Variant keys() { return {tree_attention_keys<kF8, R>, KeysCfg<kF8, R>::kThreads, KeysCfg<kF8, R>::kBytes}; }
-template <bool kF8, int kReps>
-constexpr Variant lanes() { return {tree_attention<kF8, kReps>, Cfg<kF8>::kThreads, dynamic_bytes<kF8>()}; }
-const Variant kKeys[2][4] = {{keys<false, 8>(), keys<false, 16>(), keys<false, 32>(), keys<false, 64>()},
-                             {keys<true, 8>(), keys<true, 16>(), keys<true, 32>(), keys<true, 64>()}};
-const Variant kRowsOnLanes[2][3] = {{lanes<false, 1>(), lanes<false, 2>(), lanes<false, 4>()}, {lanes<true, 1>(), lanes<true, 2>(), lanes<true, 4>()}};
-int kKeysRows[2] = {64, 64};
+template <bool kF8>
+constexpr Variant lanes() { return {tree_attention<kF8>, Cfg<kF8>::kThreads, dynamic_bytes<kF8>()}; }
+const Variant kVariants[2][5] = {{keys<false, 8>(), keys<false, 16>(), keys<false, 32>(), keys<false, 64>(), lanes<false>()},
+                                 {keys<true, 8>(), keys<true, 16>(), keys<true, 32>(), keys<true, 64>(), lanes<true>()}};
 }  // namespace
 
 extern "C" cudaError_t vdc_tree_attention_prepare() {
-  if (const char* e = getenv("FEW_BF16")) kKeysRows[0] = atoi(e);
-  if (const char* e = getenv("FEW_F8")) kKeysRows[1] = atoi(e);
-  auto prepare = [](const Variant& v) { return cudaFuncSetAttribute((const void*)v.run, cudaFuncAttributeMaxDynamicSharedMemorySize, v.bytes); };
-  for (int f8 = 0; f8 < 2; ++f8) {
-    for (const Variant& v : kKeys[f8])
-      if (cudaError_t e = prepare(v)) return e;
-    for (const Variant& v : kRowsOnLanes[f8])
-      if (cudaError_t e = prepare(v)) return e;
-  }
+  for (const auto& kind : kVariants)
+    for (const Variant& v : kind)
+      if (cudaError_t e = cudaFuncSetAttribute((const void*)v.run, cudaFuncAttributeMaxDynamicSharedMemorySize, v.bytes)) return e;
   return cudaSuccess;
 }
 
@@ -1711,7 +1745,7 @@ extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* 
                                                  cudaStream_t stream) {
   alignas(64) CUtensorMap maps[2] = {};
   const vdc_cache& c = a->cache;
-  const int rows = a->T * a->group, ctas = ctas_of(a, sms), units = a->B * c.n_kv * tiles_of(*a);
+  const int rows = a->T * a->group;
   if (!c.kind) {
     // a page of a head in two halves of 64 values, rows of 128 bytes
     const uint64_t shape[4] = {VDC_HEAD_DIM, VDC_KV_PAGE, (uint64_t)c.n_kv, (uint64_t)c.n_pages};
@@ -1723,12 +1757,12 @@ extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* 
         vdc_build_tma_desc(&maps[1], reinterpret_cast<const void*>(c.v), 2, 4, shape, vs, box, ones, 0, 0) != VDC_OK)
       return cudaErrorInvalidValue;
   }
-  const Variant& v = rows <= kKeysRows[c.kind] ? kKeys[c.kind][rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 3]
-                                               : kRowsOnLanes[c.kind][rows <= 32 ? 2 : rows <= 64 ? 1 : 0];
+  const Variant& v = kVariants[c.kind][rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 3 : 4];
+  const int ctas = ctas_of(a, sms);
   v.run<<<ctas, v.threads, v.bytes, stream>>>(*a, maps[0], maps[1], status, timeout_ns);
   if (cudaError_t e = cudaGetLastError()) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)units, (unsigned)(((rows < kRows ? rows : kRows) + kJoinWarps - 1) / kJoinWarps));
+  cfg.gridDim = dim3((unsigned)(a->B * c.n_kv * tiles_of(*a)), (unsigned)(((rows < kRows ? rows : kRows) + kJoinWarps - 1) / kJoinWarps));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute at{};
