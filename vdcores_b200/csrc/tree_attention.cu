@@ -946,7 +946,9 @@ struct KeysCfg {
   static constexpr int kBytes = 1024 + kSlots * kPart + 2 * kWide + kQBufs * kQBytes + 2 * kPBytes;
   static_assert(kBytes + 15360 <= 232448, "shared memory of a CTA");
   static constexpr int kLoadWarp = kMathWarps + (kF8 ? 8 : 0), kScoreWarp = kLoadWarp + 1, kSumWarp = kLoadWarp + 2;
-  static constexpr int kThreads = kF8 ? 640 : 384, kMathRegs = kF8 ? 128 : 208, kOtherRegs = kF8 ? 72 : 88;
+  static constexpr int kThreads = kF8 ? 640 : 384, kMathRegs = kF8 ? (R <= 16 ? 104 : R <= 32 ? 120 : 128) : 208, kOtherRegs = kF8 ? (R <= 16 ? 88 : R <= 32 ? 80 : 72) : 88;
+  static_assert(kMathWarps * 32 * kMathRegs + (kThreads - kMathWarps * 32) * kOtherRegs <= kThreads * (kF8 ? 96 : 168), "registers of a launch");
+  static constexpr int kCodes = R <= 16 ? 8 : 4;                        // pieces of codes that a thread widens at a time
   // powers of two by which a score may exceed its reference, and by which f16 weights are kept larger (2^15 at most)
   static constexpr float kSlack = kF8 ? 4.f : 8.f, kLift = kF8 ? 11.f : 0.f;
 };
@@ -1201,34 +1203,37 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
           uint32_t good = spin(&sh.v_empty[team], ((g >> 1) & 1) ^ 1, wait);
           good &= spin(&sh.full[st], val_phase(g), wait);
           const uint8_t* src = ring + st * C::kPart + from;
-          uint4 code[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) code[j] = *reinterpret_cast<const uint4*>(src + j * 16 * D);
-          const int left = end - i * PAGE, own = p.ctx - i * PAGE;
-          if (min(left, own) < kStep) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int row = j * 16 + r0;
-              auto clean = [](uint32_t w) {
-                const uint32_t x = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-                return w & ~((x >> 7) * 0xFFu);
-              };
-              if (row >= left) code[j] = make_uint4(0, 0, 0, 0);
-              else if (row >= own) code[j] = make_uint4(clean(code[j].x), clean(code[j].y), clean(code[j].z), clean(code[j].w));
-            }
-          }
           ok = all_well(good, wait, 3, i);
           if (!ok) break;
+          const int left = end - i * PAGE, own = p.ctx - i * PAGE;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            uint32_t x[4], y[4];
-            e4m3x4_to_half2(code[j].x, reinterpret_cast<uint32_t(&)[2]>(x[0]));
-            e4m3x4_to_half2(code[j].y, reinterpret_cast<uint32_t(&)[2]>(x[2]));
-            e4m3x4_to_half2(code[j].z, reinterpret_cast<uint32_t(&)[2]>(y[0]));
-            e4m3x4_to_half2(code[j].w, reinterpret_cast<uint32_t(&)[2]>(y[2]));
-            const uint4 first = make_uint4(x[0], x[1], x[2], x[3]), second = make_uint4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<uint4*>(dst + j * 16 * 128 + (swap ? hi : lo)) = swap ? second : first;
-            *reinterpret_cast<uint4*>(dst + j * 16 * 128 + (swap ? lo : hi)) = swap ? first : second;
+          for (int j0 = 0; j0 < 8; j0 += C::kCodes) {
+            uint4 code[C::kCodes];
+#pragma unroll
+            for (int j = 0; j < C::kCodes; ++j) code[j] = *reinterpret_cast<const uint4*>(src + (j0 + j) * 16 * D);
+            if (min(left, own) < kStep) {
+#pragma unroll
+              for (int j = 0; j < C::kCodes; ++j) {
+                const int row = (j0 + j) * 16 + r0;
+                auto clean = [](uint32_t w) {
+                  const uint32_t x = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                  return w & ~((x >> 7) * 0xFFu);
+                };
+                if (row >= left) code[j] = make_uint4(0, 0, 0, 0);
+                else if (row >= own) code[j] = make_uint4(clean(code[j].x), clean(code[j].y), clean(code[j].z), clean(code[j].w));
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < C::kCodes; ++j) {
+              uint32_t x[4], y[4];
+              e4m3x4_to_half2(code[j].x, reinterpret_cast<uint32_t(&)[2]>(x[0]));
+              e4m3x4_to_half2(code[j].y, reinterpret_cast<uint32_t(&)[2]>(x[2]));
+              e4m3x4_to_half2(code[j].z, reinterpret_cast<uint32_t(&)[2]>(y[0]));
+              e4m3x4_to_half2(code[j].w, reinterpret_cast<uint32_t(&)[2]>(y[2]));
+              const uint4 first = make_uint4(x[0], x[1], x[2], x[3]), second = make_uint4(y[0], y[1], y[2], y[3]);
+              *reinterpret_cast<uint4*>(dst + (j0 + j) * 16 * 128 + (swap ? hi : lo)) = swap ? second : first;
+              *reinterpret_cast<uint4*>(dst + (j0 + j) * 16 * 128 + (swap ? lo : hi)) = swap ? first : second;
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -1291,24 +1296,22 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
         v.x ^= sign; v.y ^= sign; v.z ^= sign; v.w ^= sign;
         float mul = scale;
         if constexpr (!kF8) {
-          if (r < R) *reinterpret_cast<uint4*>(rows_at + (sub >> 3) * (C::kN * 128) + r * 128 + (((sub & 7) ^ (r & 7)) << 4)) = v;
+          if (R % 16 == 0 || r < R) *reinterpret_cast<uint4*>(rows_at + (sub >> 3) * (C::kN * 128) + r * 128 + (((sub & 7) ^ (r & 7)) << 4)) = v;
         } else {
           uint2 hi, lo;
           mul *= split_row(v, 0xFFFFu << (lane & 16), hi, lo);
           uint8_t* to = rows_at + r * 128 + (((sub >> 1) ^ (r & 7)) << 4) + (sub & 1) * 8;
-          if (r < R) {
+          if (R % 16 == 0 || r < R) {
             *reinterpret_cast<uint2*>(to) = hi;
             *reinterpret_cast<uint2*>(to + C::kN * 128) = lo;
           }
         }
-        if (r < R && sub == 0) {
-          sh.mul[buf][r] = mul;
-          sh.out[buf][r] = out_row(a, row_of, p.b, p.head, r);
-        }
+        if (sub == 0 && (R % 16 == 0 || r < R)) sh.mul[buf][r] = mul;
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
+      if (tid < R) sh.out[buf][tid] = out_row(a, row_of, p.b, p.head, tid);
       if (end > p.ctx) {
         // tokens that attend to drafted token j, then rows; the warps take turns
         const int t0 = row_of.token(lane), t1 = row_of.token(lane + 32);
