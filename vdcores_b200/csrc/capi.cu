@@ -33,7 +33,7 @@ extern "C" const char* vdc_read_cache_refuses(const vdc_read_cache_args* a);
 extern "C" cudaError_t vdc_read_cache_launch(const vdc_read_cache_args* a, vdc_status* status, cudaStream_t stream);
 extern "C" const char* vdc_adjust_logits_refuses(const vdc_adjust_logits_args* a);
 extern "C" cudaError_t vdc_adjust_logits_prepare();
-extern "C" cudaError_t vdc_adjust_logits_launch(const vdc_adjust_logits_args* a, vdc_status* status, cudaStream_t stream);
+extern "C" cudaError_t vdc_adjust_logits_launch(const vdc_adjust_logits_args* a, int sms, vdc_status* status, cudaStream_t stream);
 extern "C" const char* vdc_tree_attention_refuses(const vdc_tree_attention_args* a, bool pointers);
 extern "C" long long vdc_tree_attention_bytes(const vdc_tree_attention_args* a);
 extern "C" cudaError_t vdc_tree_attention_prepare();
@@ -313,11 +313,12 @@ int vdc_launch_step(const vdc_step* step, uint64_t stream, uint64_t timeout_ns) 
 }
 
 // The operators for drafted tokens: what they refuse, then the launch.
-static int ready(vdc_status** status) {
+static int ready(vdc_status** status, int* device = nullptr) {
   int dev;
   if (int r = current_device(&dev)) return r;
   if (!g_status[dev]) return fail_arg("vdc_init was not called on this device");
   *status = g_status[dev];
+  if (device) *device = dev;
   return VDC_OK;
 }
 
@@ -340,8 +341,9 @@ int vdc_read_cache(const vdc_read_cache_args* args, uint64_t stream) {
 int vdc_adjust_logits(const vdc_adjust_logits_args* args, uint64_t stream) {
   if (const char* why = args ? vdc_adjust_logits_refuses(args) : "null argument") return fail_arg(why);
   vdc_status* status;
-  if (int r = ready(&status)) return r;
-  cudaError_t e = vdc_adjust_logits_launch(args, status, reinterpret_cast<cudaStream_t>(stream));
+  int dev;
+  if (int r = ready(&status, &dev)) return r;
+  cudaError_t e = vdc_adjust_logits_launch(args, g_sm_count[dev], status, reinterpret_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? VDC_OK : fail_cuda(e, "adjust_logits launch");
 }
 
@@ -355,9 +357,8 @@ int vdc_tree_attention_workspace(const vdc_tree_attention_args* args, uint64_t* 
 int vdc_tree_attention(const vdc_tree_attention_args* args, uint64_t stream, uint64_t timeout_ns) {
   if (const char* why = args ? vdc_tree_attention_refuses(args, true) : "null argument") return fail_arg(why);
   vdc_status* status;
-  if (int r = ready(&status)) return r;
   int dev;
-  if (int r = current_device(&dev)) return r;
+  if (int r = ready(&status, &dev)) return r;
   cudaError_t e = vdc_tree_attention_launch(args, g_sm_count[dev], status, timeout_ns ? timeout_ns : 2000000000ull,
                                             reinterpret_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? VDC_OK : fail_cuda(e, "tree_attention launch");

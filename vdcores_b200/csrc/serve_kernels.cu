@@ -285,21 +285,39 @@ __global__ void __launch_bounds__(kReadThreads) read_cache(const vdc_read_cache_
 }
 
 // ------------------------------------------------------------------------- //
-// adjust_logits: a row is shared by the CTAs of a cluster, a contiguous part of the vocabulary each, walked in tiles.  For a tile a
-// CTA counts the row's ids that fall into it in shared memory: a word a token with the times generated and, above them, a bit for
-// "biased" and one for "in the prompt".  Then one pass over the tile's logits, eight at a time: most have a word of zero and need
-// nothing.  The words have 16 bits where the ids cannot overflow 14 of them, otherwise 32 and half the tile.
-// The largest logits meet over the cluster.
+// adjust_logits: a CTA takes `chunk` rows in a row, which mostly are one request's; where there are few rows, the CTAs of a cluster share
+// them, a contiguous part of the vocabulary each.  The tokens that a request's text, drafted paths or biases name are few: a bit a token
+// says that it is one of them, and their counts and biases stand in the tokens' order, so that the bits in front of a token say where.
+// That list is made once for rows of one request in a row; what only some of the rows' paths name is looked up in the row's path.
+// Then rows stream through: logits come to shared memory several groups of eight ahead, are masked two at a time, written, and
+// compared; a listed one takes a turn by itself.
+// (Gathering the listed ones' logits afterwards, one to a thread, took as long as the rows themselves.)
 // ------------------------------------------------------------------------- //
-constexpr int kLogitThreads = 512, kLogitCountBytes = 65536, kLogitMaxBias = 4096, kLogitShort = 0x3FFF;
+constexpr int kLogitThreads = 512, kLogitChunk = 8, kLogitMaxBias = 4096, kLogitMaxPath = 64;
+constexpr int kLogitTile = 262144, kLogitMaxNamed = 12288, kLogitSmallTile = 16384;      // tokens of a tile with so many listed ones at most, with more
+constexpr int kLogitAhead = 5, kLogitRing = kLogitThreads * kLogitAhead * 16;        // bytes on their way to a CTA, 16 a thread each
+constexpr uint32_t kPrompt = 0x80000000u, kOnPath = 0x40000000u, kBiased = 0x20000000u;      // of a count: in the prompt, on some row's path
+
+// Shared memory of a CTA: the list, a bit a token, for 32 of them the number of listed ones in front, the biases, then the logits on
+// their way.
+struct LogitEntry {
+  uint32_t count;
+  float bias;
+};
+struct LogitPlan {
+  int parts, chunk, tile, cap;      // CTAs of a cluster, rows of one, tokens of a tile (a multiple of 8), list entries
+  __host__ __device__ int words() const { return (tile + 31) / 32; }
+  __host__ __device__ int bits() const { return cap * (int)sizeof(LogitEntry); }
+  __host__ __device__ int ranks() const { return bits() + words() * 4; }
+  __host__ __device__ int biases() const { return (ranks() + words() * 2 + 3) & ~3; }
+  __host__ __device__ int ring(int n_bias) const { return (biases() + n_bias * 8 + 15) & ~15; }
+  __host__ __device__ int bytes(int n_bias) const { return ring(n_bias) + kLogitRing; }
+};
 
 __device__ __forceinline__ float2 pair_of(uint32_t u, __nv_bfloat16) { return make_float2(bf_lo(u), bf_hi(u)); }
 __device__ __forceinline__ float2 pair_of(uint32_t u, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
-__device__ __forceinline__ uint32_t pair_to(float x, float y, __nv_bfloat16) { return pack_bf16x2(x, y); }
-__device__ __forceinline__ uint32_t pair_to(float x, float y, __half) {
-  const __half2 h = __floats2half2_rn(x, y);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
+__device__ constexpr uint32_t pair_none(__nv_bfloat16) { return 0xFF80FF80u; }      // -inf twice
+__device__ constexpr uint32_t pair_none(__half) { return 0xFC00FC00u; }
 template <class T> __device__ __forceinline__ float to_f32(T x);
 template <> __device__ __forceinline__ float to_f32(float x) { return x; }
 template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -309,220 +327,395 @@ template <> __device__ __forceinline__ float from_f32(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
 
+__device__ __forceinline__ uint32_t max_pair(uint32_t x, uint32_t y, __nv_bfloat16) {
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t max_pair(uint32_t x, uint32_t y, __half) {
+  const __half2 m = __hmax2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <uint32_t kSelect>      // bytes of x, or (8 + i) the sign of byte i all over
+__device__ __forceinline__ uint32_t permute(uint32_t x) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(x), "n"(kSelect));
+  return r;
+}
+
+// 16 bytes to shared memory, past L1, without a register to wait for.
+__device__ __forceinline__ void fetch16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLater>
+__device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLater) : "memory"); }
+
 // Eight logits as they lie in memory, at a multiple of 16 bytes.
 template <class T>
 struct Eight {
-  uint4 v[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void get(float (&x)[8]) const {
+  static constexpr int kPieces = sizeof(T) / 2;
+  uint4 v[kPieces];
+  // -inf for what is not allowed; the largest of those that are, and are not listed.  Two 16-bit logits at a time: a product puts four bits into the signs of four bytes, which a permutation spreads.
+  __device__ __forceinline__ float mask(uint32_t allowed, uint32_t listed) {
     if constexpr (sizeof(T) == 4) {
-      const uint32_t u[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+      uint32_t* u = reinterpret_cast<uint32_t*>(v);
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(u[i]);
+      for (int i = 0; i < 8; ++i) {
+        const bool may = allowed >> i & 1, own = listed >> i & 1;
+        if (!may) u[i] = 0xFF800000u;
+        top = fmaxf(top, own ? -INFINITY : __uint_as_float(u[i]));
+      }
+      return top;
     } else {
-      const uint32_t u[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+      constexpr uint32_t none = pair_none(T());
+      uint32_t* u = reinterpret_cast<uint32_t*>(v);
+      uint32_t may[4], own[4];
+      auto spread = [](uint32_t bits, uint32_t (&m)[4]) {
+        const uint32_t lo = (bits & 15) * 0x10204080u, hi = (bits >> 4 & 15) * 0x10204080u;
+        m[0] = permute<0x9988>(lo); m[1] = permute<0xBBAA>(lo); m[2] = permute<0x9988>(hi); m[3] = permute<0xBBAA>(hi);
+      };
+      spread(allowed, may);
+      spread(listed, own);
+      uint32_t z[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 f = pair_of(u[i], T());
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
+        u[i] = (u[i] & may[i]) | (none & ~may[i]);
+        z[i] = (u[i] & ~own[i]) | (none & own[i]);
       }
+      const float2 t = pair_of(max_pair(max_pair(z[0], z[1], T()), max_pair(z[2], z[3], T()), T()), T());
+      return fmaxf(t.x, t.y);
     }
   }
-};
-template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pair_to(x[0], x[1], T()), pair_to(x[2], x[3], T()), pair_to(x[4], x[5], T()), pair_to(x[6], x[7], T()));
+  template <class To>
+  __device__ __forceinline__ void store(To* p) const {
+    if constexpr (sizeof(To) == sizeof(T)) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) reinterpret_cast<uint4*>(p)[i] = v[i];
+    } else {
+      const float2 a = pair_of(v[0].x, T()), b = pair_of(v[0].y, T()), c = pair_of(v[0].z, T()), d = pair_of(v[0].w, T());
+      reinterpret_cast<float4*>(p)[0] = make_float4(a.x, a.y, b.x, b.y);
+      reinterpret_cast<float4*>(p)[1] = make_float4(c.x, c.y, d.x, d.y);
+    }
   }
-}
+  template <class To>
+  __device__ __forceinline__ void store_singly(To* p) const {
+    const T* x = reinterpret_cast<const T*>(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = from_f32<To>(to_f32(x[i]));
+  }
+};
 
 // Largest first, and the lower id of two equal ones; NaN never.
 __device__ __forceinline__ void better(float& v, int& i, float v2, int i2) {
   if (v2 > v || (v2 == v && i2 < i)) v = v2, i = i2;
 }
+// The best of a warp's, for all lanes: values as whole numbers in their order (both zeros as one), then the lowest id of the largest.
+__device__ __forceinline__ void warp_best(float& v, int& i) {
+  const uint32_t b = __float_as_uint(v + 0.f), key = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u), top = __reduce_max_sync(~0u, key);
+  i = __reduce_min_sync(~0u, key == top ? i : 0x7FFFFFFF);
+  v = __uint_as_float(top & 0x80000000u ? top ^ 0x80000000u : ~top);
+}
 
 struct LogitShared {
-  float best[32];
-  int at[32];
-  float cta_best;
-  int cta_at;
+  float best[kLogitChunk][kLogitThreads / 32];
+  int at[kLogitChunk][kLogitThreads / 32];
+  float cta_best[kLogitChunk];
+  int cta_at[kLogitChunk];
+  int path[kLogitChunk][kLogitMaxPath];      // the chunk's paths, where rows share a list
+  int listed[kLogitThreads / 32];            // in a warp's words
 };
 
-template <class Tin, class Tout, class Count>
-__global__ void __launch_bounds__(kLogitThreads, 3) adjust_logits(const vdc_adjust_logits_args a, int parts, vdc_status* status) {
-  constexpr int kTile = kLogitCountBytes / (int)sizeof(Count);       // tokens
-  constexpr uint32_t kPrompt = 1u << (8 * sizeof(Count) - 1), kBiased = kPrompt >> 1;
-  extern __shared__ uint4 dyn[];                                     // the tile's words, then the row's biases: ids, values
+template <class Tin, class Tout>
+__global__ void __launch_bounds__(kLogitThreads, 2)
+adjust_logits(const __grid_constant__ vdc_adjust_logits_args a, const __grid_constant__ LogitPlan plan, vdc_status* status) {
+  constexpr int kAhead = kLogitAhead * 2 / (int)sizeof(Tin);         // groups of eight logits on their way to a thread
+  extern __shared__ uint4 dyn[];
   __shared__ LogitShared sh;
-  uint32_t* count = reinterpret_cast<uint32_t*>(dyn);
-  int* ids = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(dyn) + kLogitCountBytes);
-  float* add = reinterpret_cast<float*>(ids + a.n_bias);
-  const int row = blockIdx.x / parts, part = blockIdx.x % parts, tid = threadIdx.x;
-  const Tin* in = reinterpret_cast<const Tin*>(a.logits) + row * a.logits_s;
-  Tout* out = reinterpret_cast<Tout*>(a.out) + row * a.out_s;
-  int req = row;
-  if (a.requests) req = __ldg(reinterpret_cast<const int*>(a.requests) + row);
-  const bool known = req >= 0 && req < a.n;
-  if (!known && part == 0 && tid == 0) report(status, VDC_ERR_RANGE, VDC_ADJUST_LOGITS_KIND, 3, row, req);
-  auto factor = [&](uint64_t p, float none) { return p && known ? __ldg(reinterpret_cast<const float*>(p) + req) : none; };
-  const float rep = factor(a.repetition, 1.f), freq = factor(a.frequency, 0.f), pres = factor(a.presence, 0.f);
-  const bool seen_matters = known && (a.repetition || a.frequency || a.presence);
-  const int* hist = reinterpret_cast<const int*>(a.history) + (known ? req * a.history_s : 0);
-  int n_hist = 0, n_prompt = 0;
-  if (seen_matters && a.history) {
-    n_hist = a.history_lens ? max(0, min(a.L, __ldg(reinterpret_cast<const int*>(a.history_lens) + req))) : a.L;
-    n_prompt = a.prompt_lens ? max(0, min(n_hist, __ldg(reinterpret_cast<const int*>(a.prompt_lens) + req))) : 0;
-  }
-  const int n_path = seen_matters && a.path ? a.path_n : 0;
-  const int* path = reinterpret_cast<const int*>(a.path) + row * a.path_s;
-  const int n_bias = known && a.bias_ids ? a.n_bias : 0;
-  const bool counted = n_hist + n_path + n_bias > 0;
-  for (int i = tid; i < n_bias; i += kLogitThreads) {
-    ids[i] = __ldg(reinterpret_cast<const int*>(a.bias_ids) + req * a.bias_s + i);
-    add[i] = __ldg(reinterpret_cast<const float*>(a.bias) + req * a.bias_s + i);
-  }
-  const uint32_t* allowed = a.allowed ? reinterpret_cast<const uint32_t*>(a.allowed) + row * a.allowed_s : nullptr;
+  uint8_t* const base = reinterpret_cast<uint8_t*>(dyn);
+  LogitEntry* list = reinterpret_cast<LogitEntry*>(base);
+  uint32_t* is_listed = reinterpret_cast<uint32_t*>(base + plan.bits());
+  uint16_t* ranks = reinterpret_cast<uint16_t*>(base + plan.ranks());
+  int* bias_token = reinterpret_cast<int*>(base + plan.biases());
+  float* bias_value = reinterpret_cast<float*>(bias_token + a.n_bias);
+  auto entry_of = [&](int k) { return list + ranks[k >> 5] + __popc(is_listed[k >> 5] & ((1u << (k & 31)) - 1)); };
+  uint4* ring = reinterpret_cast<uint4*>(base + plan.ring(a.n_bias)) + threadIdx.x;      // a thread reads what it has fetched itself
+  const int parts = plan.parts, part = blockIdx.x % parts, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int row0 = blockIdx.x / parts * plan.chunk, row1 = min(a.rows, row0 + plan.chunk);
+  const int* requests = reinterpret_cast<const int*>(a.requests);
+  const bool has_list = (a.bias_ids && a.n_bias) || ((a.repetition || a.frequency || a.presence) && (a.history || (a.path && a.path_n)));
+  auto path_of = [&](int row) { return reinterpret_cast<const int*>(a.path) + row * a.path_s; };
 
-  // Groups of eight tokens start where a load of eight logits may: group g holds tokens 8 g - lead .. 8 g - lead + 7, of which the
-  // first and the last group have some only.
-  const int lead = (int)(((uintptr_t)in & 15) / sizeof(Tin)), n_groups = (a.vocab + lead + 7) / 8;
-  const int per = (n_groups + parts - 1) / parts, g_begin = min(n_groups, part * per), g_end = min(n_groups, g_begin + per);
-  const bool wide_out = (((uintptr_t)(out - lead)) & 15) == 0;
-  auto whole = [&](int g) { return 8 * g >= lead && 8 * g + 8 - lead <= a.vocab; };
-
-  float best = -INFINITY;
-  int best_at = 0x7FFFFFFF;
-  for (int g0 = g_begin; g0 < g_end; g0 += kTile / 8) {
-    const int g1 = min(g_end, g0 + kTile / 8), first = 8 * g0 - lead;       // the tile's first token
-    if (counted) {
-      __syncthreads();
-      for (int i = tid; i < (g1 - g0) * (int)sizeof(Count) / 2; i += kLogitThreads) dyn[i] = make_uint4(0, 0, 0, 0);
-      __syncthreads();
-      const unsigned n = (unsigned)(g1 - g0) * 8;
-      auto mark = [&](unsigned k, uint32_t bit, bool once) {
-        if (k >= n) return;
-        uint32_t* word = sizeof(Count) == 4 ? count + k : count + (k >> 1);
-        bit <<= sizeof(Count) == 4 ? 0 : 16 * (k & 1);
-        if (once) atomicOr(word, bit);
-        else atomicAdd(word, bit);
-      };
-#pragma unroll 4
-      for (int i = tid; i < n_hist; i += kLogitThreads) {
-        const unsigned k = (unsigned)(__ldg(hist + i) - first);
-        mark(k, i < n_prompt ? kPrompt : 1u, i < n_prompt);
-      }
-      for (int i = tid; i < n_path; i += kLogitThreads) mark((unsigned)(__ldg(path + i) - first), 1u, false);
-      for (int i = tid; i < n_bias; i += kLogitThreads) mark((unsigned)(ids[i] - first), kBiased, true);
-      __syncthreads();
+  // A row's part of this tile.  Groups of eight tokens start where a load of eight logits may: group g holds tokens 8 g - lead ..
+  // 8 g - lead + 7, of which the row's first and last group may have some only; whole0 .. whole1 have all.
+  struct Range {
+    const Tin* in;
+    int req, lead, g0, g1, whole0, whole1;
+    __device__ __forceinline__ int first() const { return 8 * g0 - lead; }      // the tile's first token
+  };
+  auto range_of = [&](int row, int tile0) {
+    Range r;
+    r.in = reinterpret_cast<const Tin*>(a.logits) + row * a.logits_s;
+    r.req = requests ? __ldg(requests + row) : row;
+    r.lead = (int)(((uintptr_t)r.in & 15) / sizeof(Tin));
+    const int n_groups = (a.vocab + r.lead + 7) / 8, per = (n_groups + parts - 1) / parts;
+    r.g0 = part * per + tile0;
+    r.g1 = min(min(n_groups, (part + 1) * per), r.g0 + plan.tile / 8);
+    r.whole0 = max(r.g0, r.lead > 0);
+    r.whole1 = min(r.g1, (a.vocab + r.lead) / 8);
+    return r;
+  };
+  // a group's logits on their way to shared memory, the two bytes that have its bits of the mask to registers
+  uint32_t next_may[kAhead], next_may_too[kAhead];
+  auto load_one = [&](const Range& r, const uint8_t* may, int g, int slot) {
+    if (g < r.whole1) {
+#pragma unroll
+      for (int i = 0; i < Eight<Tin>::kPieces; ++i) fetch16(ring + (slot * Eight<Tin>::kPieces + i) * kLogitThreads, reinterpret_cast<const uint4*>(r.in + (8 * g - r.lead)) + i);
+      next_may[slot] = may ? __ldg(may + g - (r.lead > 0)) : 0xFFu;
+      next_may_too[slot] = may && r.lead > 0 ? __ldg(may + g) : 0xFFu;
     }
-    Eight<Tin> next;
-    int g = g0 + tid;
-    if (g < g1 && whole(g)) next.load(in + (8 * g - lead));
-    for (; g < g1; g += kLogitThreads) {
-      const int v = 8 * g - lead;
-      const bool full = whole(g);
-      float x[8];
-      uint32_t exist = 0xFF;
-      if (full) {
-        next.get(x);
-      } else {
-        exist = 0;
+    fetch_commit();
+  };
+  auto masks_of = [&](int row) { return a.allowed ? reinterpret_cast<const uint8_t*>(reinterpret_cast<const uint32_t*>(a.allowed) + row * a.allowed_s) : nullptr; };
+  auto load = [&](const Range& r, int row) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool is = v + j >= 0 && v + j < a.vocab;
-          x[j] = is ? to_f32(in[v + j]) : -INFINITY;
-          exist |= (uint32_t)is << j;
+    for (int j = 0; j < kAhead; ++j) load_one(r, masks_of(row), r.whole0 + tid + j * kLogitThreads, j);
+  };
+
+  for (int i = tid; i < kLogitChunk * (kLogitThreads / 32); i += kLogitThreads) (&sh.best[0][0])[i] = -INFINITY, (&sh.at[0][0])[i] = 0x7FFFFFFF;
+  __syncthreads();
+  const int most_per = ((a.vocab + 7 + 7) / 8 + parts - 1) / parts;  // groups of a CTA at most, over all rows' alignments
+  for (int tile0 = 0; tile0 < most_per; tile0 += plan.tile / 8) {
+    int held = -1, held_lead = -1;      // whose list is in shared memory
+    Range r = range_of(row0, tile0);
+    load(r, row0);
+    for (int row = row0; row < row1; ++row) {
+      Tout* out = reinterpret_cast<Tout*>(a.out) + row * a.out_s;
+      const int req = r.req, lead = r.lead, g0 = r.g0, g1 = r.g1, first = r.first();
+      const Tin* in = r.in;
+      const bool known = req >= 0 && req < a.n;
+      if (!known && part == 0 && tid == 0 && tile0 == 0) report(status, VDC_ERR_RANGE, VDC_ADJUST_LOGITS_KIND, 3, row, req);
+      const bool wide_out = (((uintptr_t)(out - lead)) & 15) == 0;
+
+      // ---- the list
+      const bool seen_matters = known && (a.repetition || a.frequency || a.presence);
+      const int n_bias = known && a.bias_ids ? a.n_bias : 0;
+      const int n_path = seen_matters && a.path ? a.path_n : 0;
+      const bool listed = known && has_list;
+      if (listed && (req != held || lead != held_lead)) {
+        __syncthreads();                         // the rows before are through
+        held = req;
+        held_lead = lead;
+        auto place = [&](int token) {            // of the tile, or -1
+          const unsigned k = (unsigned)(token - first);
+          return g1 > g0 && (unsigned)token < (unsigned)a.vocab && k < (unsigned)(g1 - g0) * 8 ? (int)k : -1;
+        };
+        auto enter = [&](int k) { atomicOr(is_listed + (k >> 5), 1u << (k & 31)); };
+        int n_hist = 0, n_prompt = 0;
+        const int* hist = reinterpret_cast<const int*>(a.history) + req * a.history_s;
+        if (seen_matters && a.history) {
+          n_hist = a.history_lens ? max(0, min(a.L, __ldg(reinterpret_cast<const int*>(a.history_lens) + req))) : a.L;
+          n_prompt = a.prompt_lens ? max(0, min(n_hist, __ldg(reinterpret_cast<const int*>(a.prompt_lens) + req))) : 0;
         }
-      }
-      const int g2 = g + kLogitThreads;
-      if (g2 < g1 && whole(g2)) next.load(in + (8 * g2 - lead));
-      if (counted) {
-        uint32_t w[8];
-        uint32_t any;
-        if constexpr (sizeof(Count) == 2) {
-          const uint4 c = dyn[g - g0];
-          any = c.x | c.y | c.z | c.w;
-          w[0] = c.x & 0xFFFF; w[1] = c.x >> 16; w[2] = c.y & 0xFFFF; w[3] = c.y >> 16;
-          w[4] = c.z & 0xFFFF; w[5] = c.z >> 16; w[6] = c.w & 0xFFFF; w[7] = c.w >> 16;
-        } else {
-          const uint4 c = dyn[2 * (g - g0)], d = dyn[2 * (g - g0) + 1];
-          any = c.x | c.y | c.z | c.w | d.x | d.y | d.z | d.w;
-          w[0] = c.x; w[1] = c.y; w[2] = c.z; w[3] = c.w; w[4] = d.x; w[5] = d.y; w[6] = d.z; w[7] = d.w;
+        // all loads first: text, paths, biases
+        constexpr int kBatch = 8;
+        int k[kBatch];
+        int same = 1;                            // rows from here that are the request's
+        {
+          const unsigned m = __ballot_sync(~0u, row + lane < row1 && (requests ? __ldg(requests + row + lane) : row + lane) == req);
+          same = __ffs(~m) - 1;
         }
-        if (any) {
+        const int n_paths = n_path * same;
+        int first_path = -1;
+        if (tid < n_paths) first_path = __ldg(path_of(row + tid / n_path) + tid % n_path);
+        for (int i = tid; i < n_bias; i += kLogitThreads) {
+          bias_token[i] = __ldg(reinterpret_cast<const int*>(a.bias_ids) + req * a.bias_s + i);
+          bias_value[i] = __ldg(reinterpret_cast<const float*>(a.bias) + req * a.bias_s + i);
+        }
+        auto fetch_text = [&](int i0) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (w[j] & ~kBiased) {
-              const uint32_t times = w[j] & (kBiased - 1);
-              if (a.repetition) x[j] = x[j] > 0.f ? __fdiv_rn(x[j], rep) : __fmul_rn(x[j], rep);
-              x[j] = __fsub_rn(x[j], __fmul_rn(freq, (float)times));
-              if (times) x[j] = __fsub_rn(x[j], pres);
-            }
-            if (w[j] & kBiased) {
-              float sum = 0.f;
-              for (int i = 0; i < n_bias; ++i)
-                if (ids[i] == v + j) sum += add[i];
-              x[j] = __fadd_rn(x[j], sum);
-            }
+          for (int j = 0; j < kBatch; ++j) k[j] = n_hist ? __ldg(hist + min(i0 + j * kLogitThreads, n_hist - 1)) : -1;
+        };
+        fetch_text(tid);                         // (the first ones are on their way while the table is cleared)
+        const int n_words = (g1 - g0 + 3) / 4;
+        for (int i = tid; i < n_words; i += kLogitThreads) is_listed[i] = 0;
+        for (int i = tid; i < plan.cap; i += kLogitThreads) list[i] = LogitEntry{0, 0.f};
+        __syncthreads();
+        for (int i0 = tid; i0 < n_hist; i0 += kLogitThreads * kBatch) {
+          if (i0 != tid) fetch_text(i0);
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) {
+            const int at = place(k[j]);
+            if (i0 + j * kLogitThreads < n_hist && at >= 0) enter(at);
           }
         }
-      }
-      if (allowed) {
-        const int v1 = max(v, 0), word = v1 >> 5;
-        const uint32_t lo = __ldg(allowed + word), hi = (v1 & 31) > 24 && 32 * (word + 1) < a.vocab ? __ldg(allowed + word + 1) : 0u;
-        const uint32_t bits = __funnelshift_r(lo, hi, v1 & 31) << (v1 - v);
+        for (int i = tid; i < n_paths; i += kLogitThreads) {
+          const int t = i == tid ? first_path : __ldg(path_of(row + i / n_path) + i % n_path), k = place(t);
+          if (plan.chunk > 1) sh.path[row - row0 + i / n_path][i % n_path] = t;
+          if (k >= 0) enter(k);
+        }
+        for (int i = tid; i < n_bias; i += kLogitThreads) {
+          const int k = place(bias_token[i]);
+          if (k >= 0) enter(k);
+        }
+        __syncthreads();
+        // a thread counts a run of words, and then knows the number in front of each
+        const int run = (n_words + kLogitThreads - 1) / kLogitThreads, w0 = min(n_words, tid * run), w1 = min(n_words, w0 + run);
+        int mine = 0;
+        for (int i = w0; i < w1; ++i) mine += __popc(is_listed[i]);
+        int up_to = mine;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!((bits >> j) & 1)) x[j] = -INFINITY;
-      }
-      const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      if (top > best) {
-        best = top;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int below = __shfl_up_sync(~0u, up_to, o);
+          if (lane >= o) up_to += below;
+        }
+        if (lane == 31) sh.listed[warp] = up_to;
+        __syncthreads();
+        int before = up_to - mine;
+        {
+          const int n = lane < warp ? sh.listed[lane] : 0;
+          before += __reduce_add_sync(~0u, n);
+        }
+        for (int i = w0; i < w1; ++i) {
+          ranks[i] = (uint16_t)before;
+          before += __popc(is_listed[i]);
+        }
+        __syncthreads();
+        for (int i0 = tid; i0 < n_hist; i0 += kLogitThreads * kBatch) {
+          if (n_hist > kLogitThreads * kBatch) fetch_text(i0);
 #pragma unroll
-        for (int j = 7; j >= 0; --j)
-          if (x[j] == top) best_at = v + j;
+          for (int j = 0; j < kBatch; ++j) {
+            const int at = place(k[j]), i = i0 + j * kLogitThreads;
+            if (i >= n_hist || at < 0) continue;
+            uint32_t* count = &entry_of(at)->count;
+            if (i < n_prompt) atomicOr(count, kPrompt);
+            else atomicAdd(count, 1u);
+          }
+        }
+        for (int i = tid; i < n_paths; i += kLogitThreads) {
+          const int k = place(i == tid ? first_path : __ldg(path_of(row + i / n_path) + i % n_path));
+          if (k < 0) continue;
+          if (plan.chunk == 1) atomicAdd(&entry_of(k)->count, 1u);      // (a single row's path counts at once)
+          else atomicOr(&entry_of(k)->count, kOnPath);
+        }
+        for (int i = tid; i < n_bias; i += kLogitThreads) {
+          const int token = bias_token[i], k = place(token);
+          if (k < 0) continue;
+          float sum = 0.f;                       // of all biases of the token, in order; each of them comes to the same
+#pragma unroll 8
+          for (int j = 0; j < n_bias; ++j) {
+            const float more = bias_value[j];
+            sum = bias_token[j] == token ? sum + more : sum;
+          }
+          entry_of(k)->bias = sum;
+          atomicOr(&entry_of(k)->count, kBiased);
+        }
+        __syncthreads();
       }
-      if (full && wide_out) {
-        store8(out + v, x);
-      } else {
+
+      auto factor = [&](uint64_t p, float none) { return p && known ? __ldg(reinterpret_cast<const float*>(p) + req) : none; };
+      const float rep = factor(a.repetition, 1.f), freq = factor(a.frequency, 0.f), pres = factor(a.presence, 0.f);
+
+      // ---- the tile's logits
+      const uint8_t* may_bytes = masks_of(row);
+      const uint32_t* allowed = reinterpret_cast<const uint32_t*>(may_bytes);
+      const int may_shift = (8 - lead) & 7;
+      auto may = [&](int token) { return !allowed || (__ldg(allowed + (token >> 5)) >> (token & 31) & 1); };
+      auto own = [&](int token) { return listed && (is_listed[(token - first) >> 5] >> ((token - first) & 31) & 1); };
+      auto adjusted = [&](float x, int token) {
+        const int k = token - first;
+        const LogitEntry e = *entry_of(k);
+        uint32_t c = e.count & ~(kOnPath | kBiased);
+        if (e.count & kOnPath)
+          for (int i = 0; i < n_path; ++i) c += sh.path[row - row0][i] == token;
+        const uint32_t times = c & ~kPrompt;
+        if (c) {
+          if (a.repetition) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+          x = __fsub_rn(x, __fmul_rn(freq, (float)times));
+          if (times) x = __fsub_rn(x, pres);
+        }
+        return e.count & kBiased ? __fadd_rn(x, e.bias) : x;
+      };
+      float best = -INFINITY;                    // of single tokens
+      int best_at = 0x7FFFFFFF;
+      float most = -INFINITY;                    // of the whole groups, and the first group that has it
+      int most_g = 0x7FFFFFFF;
+      for (int gb = r.whole0 + tid; gb < r.whole1; gb += kLogitThreads * kAhead) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if ((exist >> j) & 1) out[v + j] = from_f32<Tout>(x[j]);
+        for (int j = 0; j < kAhead; ++j) {
+          const int g = gb + j * kLogitThreads;
+          if (g >= r.whole1) break;
+          const int v = 8 * g - lead;
+          fetch_wait<kAhead - 1>();
+          Eight<Tin> x;
+#pragma unroll
+          for (int i = 0; i < Eight<Tin>::kPieces; ++i) x.v[i] = ring[(j * Eight<Tin>::kPieces + i) * kLogitThreads];
+          const uint32_t bits = (next_may[j] | next_may_too[j] << 8) >> may_shift;
+          const uint32_t listed_here = listed ? is_listed[(g - g0) >> 2] >> (8 * ((g - g0) & 3)) & 0xFF : 0u;
+          const float top = x.mask(bits, listed_here);
+          if (top > most) most = top, most_g = g;
+          if (wide_out) x.store(out + v);
+          else x.store_singly(out + v);
+          for (uint32_t m = listed_here & bits; m; m &= m - 1) {
+            const int i = __ffs(m) - 1;
+            const Tin* raw = reinterpret_cast<const Tin*>(ring + (j * Eight<Tin>::kPieces + i * (int)sizeof(Tin) / 16) * kLogitThreads) + i % (16 / (int)sizeof(Tin));
+            const float y = adjusted(to_f32(*raw), v + i);
+            out[v + i] = from_f32<Tout>(y);
+            better(best, best_at, y, v + i);
+          }
+          load_one(r, may_bytes, g + kAhead * kLogitThreads, j);
+        }
+      }
+      warp_best(most, most_g);
+      if (most > -INFINITY) {                    // which of its eight it is
+        __syncwarp();
+        const int token = 8 * most_g - lead + lane;
+        if (lane < 8 && may(token) && !own(token) && to_f32(in[token]) == most) better(best, best_at, most, token);
+      }
+      // tokens of groups that are not whole
+      if (tid < 16) {
+        const int g = tid < 8 ? g0 : g1 - 1, token = 8 * g - lead + (tid & 7);
+        if (g0 < g1 && (g < r.whole0 || g >= r.whole1) && (tid < 8 || g != g0) && token >= 0 && token < a.vocab) {
+          const float x = !may(token) ? -INFINITY : own(token) ? adjusted(to_f32(in[token]), token) : to_f32(in[token]);
+          out[token] = from_f32<Tout>(x);
+          better(best, best_at, x, token);
+        }
+      }
+      if (row + 1 < row1) {                      // (the next row's first logits are on their way while this one ends)
+        r = range_of(row + 1, tile0);
+        load(r, row + 1);
+      }
+      if (a.tokens) {
+        warp_best(best, best_at);
+        if (lane == 0) better(sh.best[row - row0][warp], sh.at[row - row0][warp], best, best_at);
       }
     }
   }
   if (!a.tokens) return;      // the same for every CTA of a cluster
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) better(best, best_at, __shfl_xor_sync(~0u, best, o), __shfl_xor_sync(~0u, best_at, o));
-  if ((tid & 31) == 0) sh.best[tid >> 5] = best, sh.at[tid >> 5] = best_at;
   __syncthreads();
-  if (tid < 32) {
-    best = tid < kLogitThreads / 32 ? sh.best[tid] : -INFINITY;
-    best_at = tid < kLogitThreads / 32 ? sh.at[tid] : 0x7FFFFFFF;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) better(best, best_at, __shfl_xor_sync(~0u, best, o), __shfl_xor_sync(~0u, best_at, o));
-    if (tid == 0) sh.cta_best = best, sh.cta_at = best_at;
+  if (warp < row1 - row0) {
+    float best = lane < kLogitThreads / 32 ? sh.best[warp][lane] : -INFINITY;
+    int best_at = lane < kLogitThreads / 32 ? sh.at[warp][lane] : 0x7FFFFFFF;
+    warp_best(best, best_at);
+    if (lane == 0) sh.cta_best[warp] = best, sh.cta_at[warp] = best_at;
+  }
+  __syncthreads();
+  if (parts > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  if (part == 0 && tid < row1 - row0) {
+    float best = sh.cta_best[tid];
+    int best_at = sh.cta_at[tid];
+    for (int p = 1; p < parts; ++p)
+      better(best, best_at, ld_cluster1(peer_smem(smem_u32(&sh.cta_best[tid]), p)), __float_as_int(ld_cluster1(peer_smem(smem_u32(&sh.cta_at[tid]), p))));
+    const int req = requests ? __ldg(requests + row0 + tid) : row0 + tid;
+    reinterpret_cast<int*>(a.tokens)[row0 + tid] = req >= 0 && req < a.n && best > -INFINITY ? best_at : -1;
   }
   if (parts > 1) {
-    __syncthreads();
-    cluster_arrive();
-    cluster_wait();
-    if (part == 0 && tid == 0) {
-      for (int p = 1; p < parts; ++p)
-        better(best, best_at, ld_cluster1(peer_smem(smem_u32(&sh.cta_best), p)),
-               __float_as_int(ld_cluster1(peer_smem(smem_u32(&sh.cta_at), p))));
-    }
     cluster_arrive();
     cluster_wait();
   }
-  if (part == 0 && tid == 0) reinterpret_cast<int*>(a.tokens)[row] = known && best > -INFINITY ? best_at : -1;
 }
 
 bool al(uint64_t p, int n) { return p % n == 0; }
@@ -607,49 +800,52 @@ extern "C" const char* vdc_adjust_logits_refuses(const vdc_adjust_logits_args* a
   return nullptr;
 }
 
-constexpr int kLogitSmem = kLogitCountBytes + kLogitMaxBias * 8;
-
 template <class Tin, class Tout>
-static cudaError_t launch_logits(const vdc_adjust_logits_args* a, vdc_status* status, cudaStream_t stream) {
-  const bool is_short = (int64_t)a->L + a->path_n <= kLogitShort;
-  // a tile to a CTA; where that leaves SMs idle, more CTAs, of 2048 tokens at least
-  int parts = (a->vocab + 8 + kLogitCountBytes / 2 - 1) / (kLogitCountBytes / 2);
-  if (parts > 8) parts = 8;
-  while (parts < 8 && (int64_t)a->rows * parts < 2 * VDC_MAX_SMS && a->vocab > parts * 2048) ++parts;
+static cudaError_t launch_logits(const vdc_adjust_logits_args* a, int sms, vdc_status* status, cudaStream_t stream) {
+  // Two CTAs an SM.  With fewer rows than that, CTAs share them (2048 tokens each at least); with more, a CTA takes rows in a row.
+  LogitPlan plan;
+  plan.parts = 1;
+  while (plan.parts < 8 && (int64_t)a->rows * (plan.parts + 1) <= 2 * sms && a->vocab > plan.parts * 2048) ++plan.parts;
+  int64_t chunk = ((int64_t)a->rows * plan.parts + 2 * sms - 1) / (2 * sms);
+  if (chunk > kLogitChunk) chunk = kLogitChunk;
+  if (a->path && a->path_n > kLogitMaxPath) chunk = 1;
+  plan.chunk = (int)chunk;
+  const int64_t text = (a->history ? (int64_t)a->L : 0) + (a->path ? chunk * a->path_n : 0), bias = a->bias_ids ? a->n_bias : 0;
+  const int tile = text + bias <= kLogitMaxNamed ? kLogitTile : kLogitSmallTile;      // (a long list has to fit)
+  if (tile == kLogitSmallTile)
+    while (plan.parts < 8 && a->vocab + 14 > (int64_t)plan.parts * tile) ++plan.parts;
+  const int64_t per = (((int64_t)a->vocab + 14) / 8 + plan.parts - 1) / plan.parts * 8;
+  plan.tile = (int)(per < tile ? per : tile);
+  plan.cap = (int)(text + bias < plan.tile ? text + bias : plan.tile);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(a->rows * parts));
+  cfg.gridDim = dim3((unsigned)((a->rows + plan.chunk - 1) / plan.chunk * plan.parts));
   cfg.blockDim = dim3(kLogitThreads);
-  cfg.dynamicSmemBytes = kLogitCountBytes + a->n_bias * 8;
+  cfg.dynamicSmemBytes = plan.bytes(a->n_bias);
   cfg.stream = stream;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = (unsigned)parts;
+  at.val.clusterDim.x = (unsigned)plan.parts;
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return is_short ? cudaLaunchKernelEx(&cfg, adjust_logits<Tin, Tout, uint16_t>, *a, parts, status)
-                  : cudaLaunchKernelEx(&cfg, adjust_logits<Tin, Tout, uint32_t>, *a, parts, status);
+  return cudaLaunchKernelEx(&cfg, adjust_logits<Tin, Tout>, *a, plan, status);
 }
 
-extern "C" cudaError_t vdc_adjust_logits_launch(const vdc_adjust_logits_args* a, vdc_status* status, cudaStream_t stream) {
-  if (a->type == 0) return launch_logits<float, float>(a, status, stream);
+extern "C" cudaError_t vdc_adjust_logits_launch(const vdc_adjust_logits_args* a, int sms, vdc_status* status, cudaStream_t stream) {
+  if (a->type == 0) return launch_logits<float, float>(a, sms, status, stream);
   if (a->type == 1)
-    return a->out_type ? launch_logits<__nv_bfloat16, __nv_bfloat16>(a, status, stream) : launch_logits<__nv_bfloat16, float>(a, status, stream);
-  return a->out_type ? launch_logits<__half, __half>(a, status, stream) : launch_logits<__half, float>(a, status, stream);
+    return a->out_type ? launch_logits<__nv_bfloat16, __nv_bfloat16>(a, sms, status, stream) : launch_logits<__nv_bfloat16, float>(a, sms, status, stream);
+  return a->out_type ? launch_logits<__half, __half>(a, sms, status, stream) : launch_logits<__half, float>(a, sms, status, stream);
 }
 
-template <class Tin, class Tout>
-static cudaError_t prepare_logits() {
-  const void* both[] = {(const void*)adjust_logits<Tin, Tout, uint16_t>, (const void*)adjust_logits<Tin, Tout, uint32_t>};
-  for (const void* f : both)
-    if (cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kLogitSmem)) return e;
-  return cudaSuccess;
-}
 extern "C" cudaError_t vdc_adjust_logits_prepare() {
-  cudaError_t e = prepare_logits<float, float>();
-  if (e == cudaSuccess) e = prepare_logits<__nv_bfloat16, __nv_bfloat16>();
-  if (e == cudaSuccess) e = prepare_logits<__nv_bfloat16, float>();
-  if (e == cudaSuccess) e = prepare_logits<__half, __half>();
-  if (e == cudaSuccess) e = prepare_logits<__half, float>();
-  return e;
+  constexpr int with = kLogitMaxNamed * 8 + kLogitTile / 16 * 3, without = kLogitSmallTile * 8 + kLogitSmallTile / 16 * 3;
+  constexpr int most = (with > without ? with : without) + kLogitMaxBias * 8 + 64 + kLogitRing;
+  const void* all[] = {(const void*)adjust_logits<float, float>, (const void*)adjust_logits<__nv_bfloat16, __nv_bfloat16>,
+                       (const void*)adjust_logits<__nv_bfloat16, float>, (const void*)adjust_logits<__half, __half>,
+                       (const void*)adjust_logits<__half, float>};
+  static_assert(most + sizeof(LogitShared) <= 232448, "shared memory of a CTA");
+  for (const void* f : all)
+    if (cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) return e;
+  return cudaSuccess;
 }
