@@ -15,6 +15,7 @@ holds.  Heads have 128 values and a page 64 rows, as everywhere in the framework
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -24,6 +25,9 @@ from . import isa, runtime
 
 BF16, F8 = torch.bfloat16, torch.float8_e4m3fn
 D, PAGE = isa.HEAD_DIM, isa.KV_PAGE
+# (the public way makes a stream object of it, a microsecond a call)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -38,16 +42,26 @@ def _on_gpu(name, t, dtype, dims):
 
 
 def _stream(t):
-    dev = t.device.index
+    dev = t.get_device()
     if dev != torch.cuda.current_device():
         raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream(dev).cuda_stream
+    return _raw_stream(dev)
 
 
 def _same_device(first, *others):
+    dev = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(device, *sizes):
+    """Bytes of workspace that a tree_attention of these sizes needs."""
+    kind, n_kv, n_pages, B, T, group, max_pages, words = sizes
+    zeros = (0,) * 18
+    return runtime.tree_attention_workspace(runtime.TreeAttention(runtime.Cache(*(0,) * 12, kind, n_kv, n_pages), B, T, group, max_pages, words,
+                                                                  1.0, *zeros))
 
 
 def _vector(name, t, n, dtype=torch.int32):
@@ -224,7 +238,7 @@ def rope_append(q, k, v, cache: KVCache, pages, lengths, table=None, positions=N
         _need(x.shape == (B, T, n_kv, D) and x.stride(3) == 1, f"{name} must be [{B}, {T}, {n_kv}, {D}], a head's values one behind the other")
         kv += x.stride()[:3]
     if out is None:
-        out = torch.empty(q.shape, dtype=BF16, device=q.device)
+        out = torch.empty_like(q)
     else:
         _need(isinstance(out, torch.Tensor) and out.shape == q.shape, "out must have the shape of q")
     os = _heads("out", out, n_kv)[3]
@@ -266,7 +280,8 @@ def read_cache(cache: KVCache, pages, lengths, n: int, start=None) -> Tuple[torc
     _need(n >= 0, "n must not be negative")
     p_start = _vector("start", start, B)
     _same_device(cache.k, start)
-    k, v = (torch.empty(B, n, cache.n_kv_heads, D, dtype=BF16, device=cache.k.device) for _ in range(2))
+    k = torch.empty((B, n, cache.n_kv_heads, D), dtype=BF16, device=cache.k.device)
+    v = torch.empty_like(k)
     if B and n:
         runtime.read_cache(runtime.ReadCache(cache._c, B, n, n_pages, 0, pages_b, p_pages, p_lengths, p_start, k.data_ptr(), v.data_ptr()),
                            _stream(k))
@@ -290,7 +305,7 @@ def tree_attention(q, cache: KVCache, pages, lengths, mask=None, counts=None, sc
     qB, T, group, qs = _heads("q", q, n_kv)
     _need(qB == B, f"q has {qB} sequences, pages {B}")
     if out is None:
-        out = torch.empty(q.shape, dtype=BF16, device=q.device)
+        out = torch.empty_like(q)
     else:
         _need(isinstance(out, torch.Tensor) and out.shape == q.shape, "out must have the shape of q")
         _need(out.data_ptr() != q.data_ptr(), "out must not be q")
@@ -308,8 +323,9 @@ def tree_attention(q, cache: KVCache, pages, lengths, mask=None, counts=None, sc
         return out
     a = runtime.TreeAttention(cache._c, B, T, group, n_pages, words, D ** -0.5 if scale is None else scale, *qs, *os, pages_b, mask_b,
                               mask_t, q.data_ptr(), out.data_ptr(), p_pages, p_lengths, p_counts, p_mask, 0)
-    nbytes = runtime.tree_attention_workspace(a)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    c = cache._c
+    nbytes = _workspace(q.get_device(), c.kind, n_kv, c.n_pages, B, T, group, n_pages, words)
+    work = q.new_empty(nbytes // 2) if nbytes else None
     if nbytes:
         a.work = work.data_ptr()
     runtime.tree_attention(a, _stream(q))
@@ -340,7 +356,7 @@ def adjust_logits(logits, requests=None, history=None, prompt_lens=None, history
     rows, vocab = logits.shape
     _need(vocab >= 1 and (vocab == 1 or logits.stride(1) == 1), "a row's logits must lie one behind the other")
     if out is None:
-        out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     else:
         _need(isinstance(out, torch.Tensor) and out.shape == logits.shape and out.dtype in (logits.dtype, torch.float32) and
               (vocab == 1 or out.stride(1) == 1), "out must be like the logits, or fp32")
@@ -382,7 +398,7 @@ def adjust_logits(logits, requests=None, history=None, prompt_lens=None, history
     n = rows if n is None else n
     _need(requests is not None or n == rows, f"{n} requests for {rows} rows: requests must say which row is whose")
     _same_device(logits, out, history, prompt_lens, history_lens, path, repetition, frequency, presence, bias_ids, bias, allowed, requests)
-    tokens = torch.empty(rows, dtype=i32, device=logits.device)
+    tokens = logits.new_empty(rows, dtype=i32)
     if rows:
         runtime.adjust_logits(runtime.AdjustLogits(
             rows, vocab, _FLOATS[logits.dtype], _FLOATS[out.dtype], n, history.shape[1] if history is not None else 0,
