@@ -1,0 +1,231 @@
+"""Greedy decoding of several sequences at once, several drafted tokens a step, on a DecodeEngine's weights.
+
+    dec = DraftedDecoder(engine, n_seqs=4, max_seq=4096, kind="e4m3")
+    dec.prefill([[1, 2, 3], ...])                  # prompts of any lengths
+    dec.generate(128)                              # 128 new ids of each sequence
+    dec.hand_over(engine, 0)                       # sequence 0 goes on in the engine's bf16 pools: engine.generate(...)
+
+Drafts come from a sequence's own text: where its last ids stood before, what followed there is proposed, up to `branches` different
+continuations of `depth` ids as a tree behind the last id.  One step runs the tree through the model: `rope_append` puts its rows into the
+caches, `tree_attention` attends over them, `adjust_logits` applies penalties, with the ids drafted in front of each row, and picks.
+The ids along the picks are accepted, one of them always; rows that were accepted from another branch than the first move by a second
+`rope_append`.  The projections between are library products, so the ids are those of undrafted decoding but for near ties, which
+products of other shapes may round differently.
+
+    python -m vdcores_b200.drafted [--layers 32] [--seqs 8] [--prompt 512] [--tokens 128] [--kind e4m3]
+
+decodes with an 8B-shaped model of random weights, with drafts and without, and prints ids a second and ids a step.  (Such a model
+repeats nothing, so hardly a draft is accepted: what is measured is what a step costs.)"""
+from __future__ import annotations
+
+import argparse
+import dataclasses
+import time
+from typing import List, Optional
+
+import torch
+
+from . import isa, ops
+from .decode import LLAMA31_8B, DecodeEngine
+
+D = isa.HEAD_DIM
+
+
+class DraftedDecoder:
+    """repetition, frequency, presence: penalties as in ops.adjust_logits, one number for all sequences; prompt and generated ids count
+    as there.  kind: "bf16" or "e4m3" caches."""
+
+    CHUNK = 256      # prompt rows of a sequence that go through the model at once
+
+    def __init__(self, engine: DecodeEngine, n_seqs: int, max_seq: int, kind: str = "e4m3", branches: int = 2, depth: int = 4,
+                 repetition: Optional[float] = None, frequency: Optional[float] = None, presence: Optional[float] = None):
+        cfg = engine.cfg
+        if cfg.n_experts:
+            raise ValueError("mixtures of experts are not supported here")
+        if branches < 0 or depth < 0 or n_seqs < 1 or max_seq < 1:
+            raise ValueError("branches and depth must not be negative, sequences and max_seq at least 1")
+        self.cfg, self.dev, self.n, self.max_seq = cfg, engine.dev, n_seqs, max_seq
+        self.branches, self.depth = (branches, depth) if branches and depth else (0, 0)
+        self.eng = engine
+        inv = engine.qkv_inv.to(self.dev)
+        self.wqkv = [engine._dense("wqkv", l)[inv] for l in range(cfg.n_layers)]
+        self.wo, self.wgu, self.wd = ([engine._dense(name, l) for l in range(cfg.n_layers)] for name in ("wo", "wgu", "wd"))
+        per = -(-(max_seq + self.branches * self.depth) // isa.KV_PAGE)
+        self.caches = [ops.KVCache.empty(n_seqs * per, cfg.n_kv_heads, kind, self.dev) for _ in range(cfg.n_layers)]
+        self.pages = torch.arange(n_seqs * per, dtype=torch.int32, device=self.dev).view(n_seqs, per)
+        self.rope = engine.rope
+        if self.rope.shape[0] < max_seq:
+            raise ValueError(f"the engine's table has {self.rope.shape[0]} positions, not {max_seq}")
+        # the tree: token 0 is the last id of the text, then the branches, one behind the other
+        parents = [-1] + [0 if i == 0 else b * self.depth + i for b in range(self.branches) for i in range(self.depth)]
+        self.parents = parents
+        self.mask, self.at_depth = ops.tree_mask(parents, self.dev)
+        self.in_front = torch.full((len(parents), self.depth), -1, dtype=torch.int64)      # a token's drafted ancestors and itself
+        for t in range(1, len(parents)):
+            line = []
+            while t > 0 and len(line) <= self.depth:
+                line.append(t)
+                t = parents[t]
+            self.in_front[line[0], :len(line)] = torch.tensor(line[::-1])
+        self.in_front = self.in_front.to(self.dev)
+        self.text: List[List[int]] = [[] for _ in range(n_seqs)]
+        self.prompt_len = [0] * n_seqs
+        self.history = torch.zeros(n_seqs, max_seq, dtype=torch.int32, device=self.dev)
+        every = lambda x: None if x is None else torch.full((n_seqs,), float(x), dtype=torch.float32, device=self.dev)    # noqa: E731
+        self.penalties = dict(repetition=every(repetition), frequency=every(frequency), presence=every(presence))
+        self.steps = 0
+
+    def _i32(self, x):
+        return torch.tensor(x, dtype=torch.int32, device=self.dev)
+
+    def _norm(self, x, w, eps):
+        xf = x.float()
+        return w * (xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)).to(x.dtype)
+
+    def _layers(self, ids, lengths, counts, mask=None, positions=None):
+        """Last hidden states [n, T, hidden] of ids [n, T] behind `lengths` rows of each sequence, and each layer's q, k, v."""
+        cfg, n, T = self.cfg, *ids.shape
+        h = self.eng.embed[ids.long()]
+        rows = []
+        for l in range(cfg.n_layers):
+            qkv = self._norm(h, self.eng.ln1[l], cfg.eps) @ self.wqkv[l].t()
+            q, k, v = (x.unflatten(-1, (-1, D)) for x in qkv.split((cfg.q_width, cfg.kv_width, cfg.kv_width), -1))
+            rows.append((q, k, v))
+            q = self._append(l, q, k, v, lengths, counts, positions)
+            o = ops.tree_attention(q, self.caches[l], self.pages, lengths, mask=mask, counts=counts)
+            h = h + o.flatten(2) @ self.wo[l].t()
+            gu = self._norm(h, self.eng.ln2[l], cfg.eps) @ self.wgu[l].t()
+            h = h + (torch.nn.functional.silu(gu[..., 0::2]) * gu[..., 1::2]) @ self.wd[l].t()
+        return h, rows
+
+    def _append(self, l, q, k, v, lengths, counts, positions):
+        norm = self.eng.qknorm[l] if self.cfg.qk_norm else None
+        return ops.rope_append(q, k, v, self.caches[l], self.pages, lengths, self.rope, positions=positions, counts=counts, qk_norm=norm,
+                               eps=self.cfg.qk_norm_eps)
+
+    @torch.no_grad()
+    def prefill(self, prompts: List[List[int]]):
+        """Takes the prompts' ids (one list a sequence, at least one id each); all but the last go through the model."""
+        if len(prompts) != self.n or any(not 1 <= len(p) <= self.max_seq for p in prompts):
+            raise ValueError(f"{self.n} prompts of 1 to {self.max_seq} ids are needed")
+        self.text = [list(p) for p in prompts]
+        self.prompt_len = [len(p) for p in prompts]
+        self.steps = 0
+        for first in range(0, max(self.prompt_len) - 1, self.CHUNK):
+            part = [p[first:len(p) - 1][:self.CHUNK] for p in prompts]
+            T = max(len(p) for p in part)
+            self._layers(self._i32([p + [0] * (T - len(p)) for p in part]), self._i32([min(first, len(p) - 1) for p in prompts]),
+                         self._i32([len(p) for p in part]))
+        for b, p in enumerate(prompts):
+            self.history[b, :len(p)] = self._i32(p)
+        ops.check()
+
+    def draft(self, text: List[int]) -> List[List[int]]:
+        """Up to `branches` continuations of `depth` ids: what followed the last two ids where they stood before, latest first, then
+        what followed the last one."""
+        found: List[List[int]] = []
+        for same in (2, 1):
+            if len(text) <= same:
+                continue
+            for i in range(len(text) - 1, same - 1, -1):
+                if len(found) == self.branches:
+                    return found
+                if text[i - same:i] == text[-same:]:
+                    new = text[i:i + self.depth]
+                    new += [new[-1]] * (self.depth - len(new))
+                    if all(new[0] != x[0] for x in found):
+                        found.append(new)
+        return found
+
+    @torch.no_grad()
+    def step(self):
+        """One pass through the model: between 1 and 1 + depth ids more of every sequence."""
+        drafts = [self.draft(t) if self.branches else [] for t in self.text]
+        T = 1 + self.depth * max(len(d) for d in drafts)
+        if any(len(t) + self.depth >= self.max_seq for t in self.text):
+            raise RuntimeError("out of cache rows")
+        host = [[t[-1]] + sum(d, []) for t, d in zip(self.text, drafts)]
+        counts = self._i32([len(x) for x in host])
+        ids = self._i32([x + [0] * (T - len(x)) for x in host])
+        lengths = self._i32([len(t) - 1 for t in self.text])
+        h, rows = self._layers(ids, lengths, counts, self.mask[:T, :-(-T // 64)].contiguous(), lengths[:, None] + self.at_depth[:T])
+        logits = self._norm(h, self.eng.norm_w, self.cfg.eps).flatten(0, 1) @ self.eng.lm_head.t()
+        how = {}
+        if any(p is not None for p in self.penalties.values()):
+            of = torch.arange(self.n, dtype=torch.int32, device=self.dev).repeat_interleave(T)
+            how = dict(requests=of, history=self.history, prompt_lens=self._i32(self.prompt_len), history_lens=lengths + 1, **self.penalties)
+            if T > 1:
+                front = self.in_front[:T]
+                how["path"] = torch.where(front >= 0, ids[:, front.clamp(min=0)], -1).flatten(0, 1).contiguous()
+        _, picks = ops.adjust_logits(logits, out=logits, **how)
+        picks = picks.view(self.n, T).tolist()
+
+        taken = []                                       # rows whose ids were accepted
+        for b in range(self.n):
+            line, row = [0], 0
+            while True:
+                want, row = picks[b][row], next((c for c in range(1, len(host[b])) if self.parents[c] == row and host[b][c] == picks[b][row]), None)
+                self.text[b].append(want)
+                if row is None:
+                    break
+                line.append(row)
+            taken.append(line)
+            new = self.text[b][-len(line):]
+            self.history[b, len(self.text[b]) - len(new):len(self.text[b])] = self._i32(new)
+        moved = [len(t) if t != list(range(len(t))) else 0 for t in taken]
+        if any(moved):                                   # the accepted rows one behind the other
+            n = max(moved)
+            at = torch.tensor([(t + [0] * n)[:n] for t in taken], device=self.dev)
+            pick = lambda x: x[torch.arange(self.n, device=self.dev)[:, None], at]    # noqa: E731
+            for l, (q, k, v) in enumerate(rows):
+                self._append(l, pick(q), pick(k), pick(v), lengths, self._i32(moved), None)
+        self.steps += 1
+
+    def generate(self, n_tokens: int) -> List[List[int]]:
+        """At least n_tokens more ids of every sequence; returns the first n_tokens."""
+        start = [len(t) for t in self.text]
+        while min(len(t) - s for t, s in zip(self.text, start)) < n_tokens:
+            self.step()
+        ops.check()
+        return [t[s:s + n_tokens] for t, s in zip(self.text, start)]
+
+    @torch.no_grad()
+    def hand_over(self, engine: DecodeEngine, b: int):
+        """Sequence b's rows into the engine's pools; its next step decodes behind the sequence's last id."""
+        n = len(self.text[b]) - 1
+        k, v = zip(*(ops.read_cache(c, self.pages[b:b + 1], self._i32([n]), n) for c in self.caches))
+        engine.load_kv([x[0] for x in k], [x[0] for x in v])
+        torch.cuda.synchronize(self.dev)                 # (the engine has a stream of its own)
+        engine.set_state(n, self.text[b][-1])
+        torch.cuda.synchronize(self.dev)
+
+
+def main():
+    ap = argparse.ArgumentParser()
+    ap.add_argument("--layers", type=int, default=32)
+    ap.add_argument("--seqs", type=int, default=8)
+    ap.add_argument("--prompt", type=int, default=512)
+    ap.add_argument("--tokens", type=int, default=128)
+    ap.add_argument("--kind", choices=("bf16", "e4m3"), default="e4m3")
+    a = ap.parse_args()
+    cfg = dataclasses.replace(LLAMA31_8B, n_layers=a.layers)
+    max_seq = a.prompt + a.tokens + 64
+    eng = DecodeEngine(cfg, max_seq=max_seq)
+    eng.init_random_weights(seed=0)
+    g = torch.Generator().manual_seed(1)
+    words = torch.randint(0, cfg.vocab, (a.seqs, 32), generator=g)
+    prompts = [words[b][torch.randint(0, 32, (a.prompt,), generator=g)].tolist() for b in range(a.seqs)]
+    for branches, depth in ((0, 0), (2, 4)):
+        dec = DraftedDecoder(eng, a.seqs, max_seq, a.kind, branches, depth)
+        dec.prefill(prompts)
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        dec.generate(a.tokens)
+        torch.cuda.synchronize()
+        dt, made = time.perf_counter() - t0, sum(len(t) for t in dec.text) - sum(dec.prompt_len)
+        print(f"{branches} branches of {depth}: {made / dt:.0f} ids/s, {made / dec.steps / a.seqs:.2f} ids a step and sequence, "
+              f"{1e3 * dt / dec.steps:.2f} ms a step")
+
+
+if __name__ == "__main__":
+    main()
