@@ -17,18 +17,37 @@ from __future__ import annotations
 
 import functools
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import isa, runtime
 
-BF16, F8 = torch.bfloat16, torch.float8_e4m3fn
+BF16, F8, I32, I64, F32 = torch.bfloat16, torch.float8_e4m3fn, torch.int32, torch.int64, torch.float32
 D, PAGE = isa.HEAD_DIM, isa.KV_PAGE
+_FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 # (the public way makes a stream object of it, a microsecond a call)
+_PACK5, _PACK7, _PACK11, _PACK14 = (struct.Struct(f"{n}Q").pack for n in (5, 7, 11, 14))      # pointers at an argument structure's end
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
-_FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+# What a call checks depends on its tensors' shapes, strides, types and devices only; those make a "look" (None for what is not given).
+# The checks run once for a combination of looks and give the fixed part of the C arguments, which is kept: a call then costs half
+# as much of the host's time.  Pointers are looked at anew, and in C.
+def _look(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _looks(names, tensors):
+    try:
+        return [None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors]
+    except (AttributeError, RuntimeError, TypeError):
+        for name, t in zip(names, tensors):
+            if t is not None and not isinstance(t, torch.Tensor):
+                raise ValueError(f"{name} must be a tensor on the GPU") from None
+        raise
 
 
 def _need(ok, what):
@@ -36,49 +55,40 @@ def _need(ok, what):
         raise ValueError(what)
 
 
-def _on_gpu(name, t, dtype, dims):
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.dim() == dims):
+def _on_gpu(name, look, dtype, dims):
+    if look is None or look[3] < 0 or look[2] != dtype or len(look[0]) != dims:
         raise ValueError(f"{name} must be a {dims}-dimensional {dtype} tensor on the GPU")
 
 
-def _stream(t):
-    dev = t.get_device()
+def _same_device(dev, names, looks):
+    for name, look in zip(names, looks):
+        if look is not None and look[3] != dev:
+            raise ValueError(f"{name} is on another device than cuda:{dev}")
+
+
+def _vector(name, look, n, dtype=I32):
+    if look is not None:
+        _on_gpu(name, look, dtype, 1)
+        _need(look[0][0] == n and (n <= 1 or look[1][0] == 1), f"{name} must have {n} values, one behind the other")
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _run(fn, dev, args, *rest):
+    """Enqueues a C call, whose arguments are bytes, on the current stream."""
     if dev != torch.cuda.current_device():
         raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
-    return _raw_stream(dev)
+    runtime.enqueue(fn, dev, args, _raw_stream(dev), *rest)
 
 
-def _same_device(first, *others):
-    dev = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
-
-
-@functools.lru_cache(maxsize=1024)
-def _workspace(device, *sizes):
-    """Bytes of workspace that a tree_attention of these sizes needs."""
-    kind, n_kv, n_pages, B, T, group, max_pages, words = sizes
-    zeros = (0,) * 18
-    return runtime.tree_attention_workspace(runtime.TreeAttention(runtime.Cache(*(0,) * 12, kind, n_kv, n_pages), B, T, group, max_pages, words,
-                                                                  1.0, *zeros))
-
-
-def _vector(name, t, n, dtype=torch.int32):
-    """Address of [n] values, one behind the other."""
-    if t is None:
-        return 0
-    _on_gpu(name, t, dtype, 1)
-    _need(t.shape[0] == n and (n <= 1 or t.stride(0) == 1), f"{name} must have {n} values, one behind the other")
-    return t.data_ptr()
-
-
-def _heads(name, x, n_kv):
+def _heads(name, look, n_kv):
     """(B, T, query heads to a KV head, strides of the four leading dimensions as [B, T, n_kv, group]) of rows [B, T, heads, 128]
     or [B, T, n_kv, group, 128]."""
-    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype == BF16 and x.dim() in (4, 5) and x.shape[-1] == D):
+    if look is None or look[3] < 0 or look[2] != BF16 or len(look[0]) not in (4, 5) or look[0][-1] != D:
         raise ValueError(f"{name} must be [B, T, heads, {D}] or [B, T, n_kv, group, {D}] bf16 on the GPU")
-    size, st = x.shape, x.stride()
+    size, st = look[:2]
     _need(st[-1] == 1, f"{name}: the values of a head must lie one behind the other")
     if len(size) == 5:
         _need(size[2] == n_kv, f"{name} has {size[2]} KV heads, the cache {n_kv}")
@@ -110,15 +120,18 @@ class KVCache:
             strides = (0, 0, 0, 0)
         else:
             for name, t in zip(("k_scale", "v_scale"), scales):
-                _on_gpu(name, t, torch.float32, 3)
+                _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
+                _on_gpu(name, _look(t), F32, 3)
                 _need(t.shape == k.shape[:3] and t.stride(2) == 1, f"{name} must be [pages, heads, {PAGE}], a page's scales one behind the other")
             strides = tuple(4 * t.stride(i) for t in scales for i in (0, 1))
-        _same_device(k, v, k_scale, v_scale)
+        self._device = k.get_device()
+        _same_device(self._device, ("v", "k_scale", "v_scale"), [_look(t) for t in (v, k_scale, v_scale)])
         self.n_pages, self.n_kv_heads = k.shape[:2]
         size = k.element_size()
         ptrs = [t.data_ptr() if t is not None else 0 for t in (k, v, k_scale, v_scale)]
         self._c = runtime.Cache(*ptrs, *(size * t.stride(i) for t in (k, v) for i in (0, 1)), *strides, int(self.kind == "e4m3"),
                                 self.n_kv_heads, self.n_pages)
+        self._raw = bytes(self._c)
 
     @classmethod
     def empty(cls, n_pages: int, n_kv_heads: int, kind: str = "bf16", device="cuda"):
@@ -131,15 +144,22 @@ class KVCache:
                    *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
 
 
-def _tables(cache, pages, lengths, counts=None):
-    """(B, max_pages, row stride and address of pages, addresses of lengths and counts)."""
-    _need(isinstance(cache, KVCache), "cache must be a KVCache")
-    _on_gpu("pages", pages, torch.int32, 2)
-    B, n = pages.shape
-    _need(n >= 1 and (n == 1 or pages.stride(1) == 1), "pages: a sequence's must lie one behind the other, at least one")
-    _same_device(cache.k, pages, lengths, counts)
+def _tables(dev, pages, lengths, counts=None):
+    """(B, max_pages, row stride of pages)."""
+    _on_gpu("pages", pages, I32, 2)
+    B, n = pages[0]
+    _need(n >= 1 and (n == 1 or pages[1][1] == 1), "pages: a sequence's must lie one behind the other, at least one")
     _need(lengths is not None, "lengths are needed")
-    return B, n, pages.stride(0) if B > 1 else 0, pages.data_ptr(), _vector("lengths", lengths, B), _vector("counts", counts, B)
+    _vector("lengths", lengths, B)
+    _vector("counts", counts, B)
+    _same_device(dev, ("pages", "lengths", "counts"), (pages, lengths, counts))
+    return B, n, pages[1][0] if B > 1 else 0
+
+
+def _fixed(cls, values):
+    """Bytes of an argument structure between the cache in front and the pointers at the end."""
+    first = getattr(cls, cls._fields_[1 if cls._fields_[0][0] == "cache" else 0][0]).offset
+    return bytes(cls(*([runtime.Cache()] if first else []), *values))[first:getattr(cls, cls._pointers_[0]).offset]
 
 
 def check():
@@ -215,6 +235,43 @@ def tree_mask(parents, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
     return pack_mask(seen).view(*p.shape, -1).to(device), depth.view(p.shape).to(device)
 
 
+_APPEND = ("q", "k", "v", "pages", "lengths", "table", "positions", "counts", "out")
+
+
+@functools.lru_cache(maxsize=4096)
+def _append_plan(dev, n_kv, layout, eps, norms, *looks):
+    q, k, v, pages, lengths, table, positions, counts, out = looks
+    B, n_pages, pages_b = _tables(dev, pages, lengths, counts)
+    qB, T, group, qs = _heads("q", q, n_kv)
+    _need(qB == B, f"q has {qB} sequences, pages {B}")
+    kv = []
+    for name, x in (("k", k), ("v", v)):
+        _on_gpu(name, x, BF16, 4)
+        _need(x[0] == (B, T, n_kv, D) and x[1][3] == 1, f"{name} must be [{B}, {T}, {n_kv}, {D}], a head's values one behind the other")
+        kv += x[1][:3]
+    _need(out[0] == q[0], "out must have the shape of q")
+    os = _heads("out", out, n_kv)[3]
+    rot = rows = pos_b = pos_t = 0
+    if table is not None:
+        _on_gpu("table", table, F32, 2)
+        rows, rot = table[0]
+        _need(table[1][1] == 1 and (rows == 1 or table[1][0] == rot), "table must be contiguous")
+    if positions is not None:
+        _on_gpu("positions", positions, I32, 2)
+        _need(positions[0] == (B, T), f"positions must be [{B}, {T}]")
+        pos_b, pos_t = positions[1]
+    _need(layout in ("half", "interleaved"), f"unknown layout {layout!r}")
+    if len(norms) == 1:
+        _on_gpu("qk_norm", norms[0], BF16, 1)
+        _need(norms[0][0] == (2 * D,) and norms[0][1] == (1,), "qk_norm must be two bf16 vectors of 128 weights")
+    for i, w in enumerate(norms if len(norms) == 2 else ()):
+        _vector(f"qk_norm[{i}]", w, D, BF16)
+    _same_device(dev, _APPEND + ("qk_norm",) * len(norms), looks + norms)
+    if B == 0 or T == 0:
+        return None
+    return _fixed(runtime.RopeAppend, (B, T, group, rot, layout == "interleaved", rows, n_pages, eps, *qs, *kv, *os, pages_b, pos_b, pos_t))
+
+
 def rope_append(q, k, v, cache: KVCache, pages, lengths, table=None, positions=None, counts=None, layout: str = "half", qk_norm=None,
                 eps: float = 1e-6, out=None) -> torch.Tensor:
     """Rotates q [B, T, heads, 128] (or [B, T, n_kv, group, 128]) and k [B, T, n_kv, 128], and appends k and v to the cache: token t
@@ -228,64 +285,71 @@ def rope_append(q, k, v, cache: KVCache, pages, lengths, table=None, positions=N
 
     bf16 rows, fp32 arithmetic, one rounding at the end.  An e4m3 cache gets e4m3(x / s) with s = the row's largest magnitude / 448;
     a row with an infinity or NaN gets a scale that is one, and reads back as NaN."""
-    n_kv = cache.n_kv_heads
-    B, n_pages, pages_b, p_pages, p_lengths, p_counts = _tables(cache, pages, lengths, counts)
-    qB, T, group, qs = _heads("q", q, n_kv)
-    _need(qB == B, f"q has {qB} sequences, pages {B}")
-    kv = []
-    for name, x in (("k", k), ("v", v)):
-        _on_gpu(name, x, BF16, 4)
-        _need(x.shape == (B, T, n_kv, D) and x.stride(3) == 1, f"{name} must be [{B}, {T}, {n_kv}, {D}], a head's values one behind the other")
-        kv += x.stride()[:3]
-    if out is None:
+    _need(isinstance(cache, KVCache), "cache must be a KVCache")
+    names = _APPEND
+    if out is None and isinstance(q, torch.Tensor):
         out = torch.empty_like(q)
-    else:
-        _need(isinstance(out, torch.Tensor) and out.shape == q.shape, "out must have the shape of q")
-    os = _heads("out", out, n_kv)[3]
-    rot = rows = p_table = p_pos = pos_b = pos_t = p_q = p_k = 0
-    if table is not None:
-        _on_gpu("table", table, torch.float32, 2)
-        rows, rot = table.shape
-        _need(table.is_contiguous(), "table must be contiguous")
-        p_table = table.data_ptr()
-    if positions is not None:
-        _on_gpu("positions", positions, torch.int32, 2)
-        _need(positions.shape == (B, T), f"positions must be [{B}, {T}]")
-        p_pos, (pos_b, pos_t) = positions.data_ptr(), positions.stride()
-    _need(layout in ("half", "interleaved"), f"unknown layout {layout!r}")
+    p_q = p_k = 0
+    norms = ()
     if qk_norm is not None:
         if isinstance(qk_norm, torch.Tensor):
-            _need(qk_norm.dtype == BF16 and qk_norm.is_cuda and qk_norm.is_contiguous() and qk_norm.numel() == 2 * D,
-                  "qk_norm must be two bf16 vectors of 128 weights")
-            p_q = qk_norm.data_ptr()
+            norms, p_q = (_look(qk_norm.flatten() if qk_norm.is_contiguous() else qk_norm),), qk_norm.data_ptr()
             p_k = p_q + 2 * D
-            _same_device(q, qk_norm)
         else:
-            w_q, w_k = qk_norm
-            p_q, p_k = _vector("qk_norm[0]", w_q, D, BF16), _vector("qk_norm[1]", w_k, D, BF16)
-            _same_device(q, w_q, w_k)
-    _same_device(q, k, v, out, cache.k, table, positions)
-    if B == 0 or T == 0:
-        return out
-    runtime.rope_append(runtime.RopeAppend(cache._c, B, T, group, rot, layout == "interleaved", rows, n_pages, eps, *qs, *kv, *os,
-                                           pages_b, pos_b, pos_t, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), p_pages,
-                                           p_lengths, p_counts, p_table, p_pos, p_q, p_k), _stream(q))
+            norms = tuple(_looks(("qk_norm[0]", "qk_norm[1]"), qk_norm))
+            _need(len(norms) == 2 and None not in norms, "qk_norm must be two bf16 vectors of 128 weights")
+            p_q, p_k = (w.data_ptr() for w in qk_norm)
+    tensors = (q, k, v, pages, lengths, table, positions, counts, out)
+    plan = _append_plan(cache._device, cache.n_kv_heads, layout, eps, norms, *_looks(names, tensors))
+    if plan is not None:
+        _run("vdc_rope_append", cache._device, cache._raw + plan + _PACK11(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), pages.data_ptr(), lengths.data_ptr(), _ptr(counts), _ptr(table),
+            _ptr(positions), p_q, p_k))
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _read_plan(dev, n_kv, n, pages, lengths, start):
+    B, n_pages, pages_b = _tables(dev, pages, lengths)
+    _need(n >= 0, "n must not be negative")
+    _vector("start", start, B)
+    _same_device(dev, ("start",), (start,))
+    return B, _fixed(runtime.ReadCache, (B, n, n_pages, 0, pages_b)) if B and n else None
 
 
 def read_cache(cache: KVCache, pages, lengths, n: int, start=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of rows start .. start + n - 1 (start: int32 [B], default 0) of every sequence as dense bf16 tensors
     [B, n, n_kv, 128]; rows at or behind lengths[b] are zeros."""
-    B, n_pages, pages_b, p_pages, p_lengths, _ = _tables(cache, pages, lengths)
-    _need(n >= 0, "n must not be negative")
-    p_start = _vector("start", start, B)
-    _same_device(cache.k, start)
+    _need(isinstance(cache, KVCache), "cache must be a KVCache")
+    B, plan = _read_plan(cache._device, cache.n_kv_heads, n, *_looks(("pages", "lengths", "start"), (pages, lengths, start)))
     k = torch.empty((B, n, cache.n_kv_heads, D), dtype=BF16, device=cache.k.device)
     v = torch.empty_like(k)
-    if B and n:
-        runtime.read_cache(runtime.ReadCache(cache._c, B, n, n_pages, 0, pages_b, p_pages, p_lengths, p_start, k.data_ptr(), v.data_ptr()),
-                           _stream(k))
+    if plan is not None:
+        _run("vdc_read_cache", cache._device, cache._raw + plan + _PACK5(pages.data_ptr(), lengths.data_ptr(), _ptr(start), k.data_ptr(),
+                                                                        v.data_ptr()))
     return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_plan(dev, kind, n_kv, n_pool, scale, q, pages, lengths, mask, counts, out):
+    B, n_pages, pages_b = _tables(dev, pages, lengths, counts)
+    qB, T, group, qs = _heads("q", q, n_kv)
+    _need(qB == B, f"q has {qB} sequences, pages {B}")
+    _need(out[0] == q[0], "out must have the shape of q")
+    os = _heads("out", out, n_kv)[3]
+    words, mask_b, mask_t = -(-T // 64), 0, 0
+    if mask is not None:
+        _need(mask[3] >= 0 and mask[2] == I64 and len(mask[0]) in (2, 3), "mask must be [B, T, words] or [T, words] int64 on the GPU")
+        size, st = mask[:2]
+        _need(size[-2:] == (T, words) and (len(size) == 2 or size[0] == B), f"mask must be [{B}, {T}, {words}] or [{T}, {words}]")
+        _need(words == 1 or st[-1] == 1, "mask: a token's words must lie one behind the other")
+        mask_t, mask_b = st[-2], st[0] if len(size) == 3 else 0
+    _same_device(dev, ("q", "out", "mask"), (q, out, mask))
+    if B == 0 or T == 0:
+        return None, 0
+    values = (B, T, group, n_pages, words, D ** -0.5 if scale is None else scale, *qs, *os, pages_b, mask_b, mask_t)
+    sizes = runtime.TreeAttention(runtime.Cache(*(0,) * 12, kind, n_kv, n_pool), *values)
+    return _fixed(runtime.TreeAttention, values), runtime.tree_attention_workspace(sizes)
 
 
 def tree_attention(q, cache: KVCache, pages, lengths, mask=None, counts=None, scale: Optional[float] = None, out=None) -> torch.Tensor:
@@ -300,36 +364,67 @@ def tree_attention(q, cache: KVCache, pages, lengths, mask=None, counts=None, sc
     out: a tensor like q, not q itself; by default a new one
 
     Scores, softmax and sums are fp32.  A token with nothing to attend to gets zeros."""
-    n_kv = cache.n_kv_heads
-    B, n_pages, pages_b, p_pages, p_lengths, p_counts = _tables(cache, pages, lengths, counts)
-    qB, T, group, qs = _heads("q", q, n_kv)
-    _need(qB == B, f"q has {qB} sequences, pages {B}")
-    if out is None:
+    _need(isinstance(cache, KVCache), "cache must be a KVCache")
+    if out is None and isinstance(q, torch.Tensor):
         out = torch.empty_like(q)
-    else:
-        _need(isinstance(out, torch.Tensor) and out.shape == q.shape, "out must have the shape of q")
-        _need(out.data_ptr() != q.data_ptr(), "out must not be q")
-    os = _heads("out", out, n_kv)[3]
-    words, p_mask, mask_b, mask_t = -(-T // 64), 0, 0, 0
-    if mask is not None:
-        _need(isinstance(mask, torch.Tensor) and mask.is_cuda and mask.dtype == torch.int64 and mask.dim() in (2, 3),
-              "mask must be [B, T, words] or [T, words] int64 on the GPU")
-        size, st = mask.shape, mask.stride()
-        _need(size[-2:] == (T, words) and (len(size) == 2 or size[0] == B), f"mask must be [{B}, {T}, {words}] or [{T}, {words}]")
-        _need(words == 1 or st[-1] == 1, "mask: a token's words must lie one behind the other")
-        p_mask, mask_t, mask_b = mask.data_ptr(), st[-2], st[0] if len(size) == 3 else 0
-    _same_device(q, cache.k, out, mask)
-    if B == 0 or T == 0:
+    elif out is q:
+        raise ValueError("out must not be q")
+    c, dev = cache._c, cache._device
+    plan, nbytes = _attention_plan(dev, c.kind, c.n_kv, c.n_pages, scale, *_looks(
+        ("q", "pages", "lengths", "mask", "counts", "out"), (q, pages, lengths, mask, counts, out)))
+    if plan is None:
         return out
-    a = runtime.TreeAttention(cache._c, B, T, group, n_pages, words, D ** -0.5 if scale is None else scale, *qs, *os, pages_b, mask_b,
-                              mask_t, q.data_ptr(), out.data_ptr(), p_pages, p_lengths, p_counts, p_mask, 0)
-    c = cache._c
-    nbytes = _workspace(q.get_device(), c.kind, n_kv, c.n_pages, B, T, group, n_pages, words)
-    work = q.new_empty(nbytes // 2) if nbytes else None
-    if nbytes:
-        a.work = work.data_ptr()
-    runtime.tree_attention(a, _stream(q))
+    p_q, p_out = q.data_ptr(), out.data_ptr()
+    _need(p_q != p_out, "out must not be q")
+    work = q.new_empty(nbytes // 2)
+    _run("vdc_tree_attention", dev, cache._raw + plan + _PACK7(p_q, p_out, pages.data_ptr(), lengths.data_ptr(), _ptr(counts), _ptr(mask),
+                                                               work.data_ptr()), 0)
     return out
+
+
+_LOGITS = ("logits", "out", "requests", "history", "prompt_lens", "history_lens", "path", "repetition", "frequency", "presence", "bias_ids",
+           "bias", "allowed")
+_LOGIT_TABLES = dict(history=(I32, 2), prompt_lens=(I32, 1), history_lens=(I32, 1), repetition=(F32, 1), frequency=(F32, 1), presence=(F32, 1),
+                     bias_ids=(I32, 2), bias=(F32, 2), path=(I32, 2), allowed=(I32, 2), requests=(I32, 1))
+
+
+@functools.lru_cache(maxsize=4096)
+def _logits_plan(*looks):
+    of = dict(zip(_LOGITS, looks))
+    logits, out, bias, bias_ids, allowed = (of[x] for x in ("logits", "out", "bias", "bias_ids", "allowed"))
+    _need(logits is not None and logits[3] >= 0 and logits[2] in _FLOATS and len(logits[0]) == 2, "logits must be [rows, vocab] fp32, bf16 or f16 on the GPU")
+    rows, vocab = logits[0]
+    _need(vocab >= 1 and (vocab == 1 or logits[1][1] == 1), "a row's logits must lie one behind the other")
+    _need(out[0] == logits[0] and out[2] in (logits[2], F32) and (vocab == 1 or out[1][1] == 1), "out must be like the logits, or fp32")
+    n = None
+    width, step = {}, {}
+    for name, (dtype, dims) in _LOGIT_TABLES.items():
+        look, per_row = of[name], name in ("path", "allowed", "requests")
+        width[name] = step[name] = 0
+        if look is None:
+            continue
+        _on_gpu(name, look, dtype, dims)
+        size, st = look[:2]
+        if dims == 2:
+            _need(size[1] <= 1 or st[1] == 1, f"{name}: a row's values must lie one behind the other")
+            width[name], step[name] = size[1], st[0]
+        else:
+            _need(size[0] <= 1 or st[0] == 1, f"{name}: values must lie one behind the other")
+        if not per_row and n is None:
+            n = size[0]
+        _need(size[0] == (rows if per_row else n), f"{name} has {size[0]} rows, not {rows if per_row else n}")
+    _need((bias_ids is None) == (bias is None), "bias and bias_ids go together")
+    if bias is not None:
+        _need(bias[0] == bias_ids[0] and (n == 1 or step["bias"] == step["bias_ids"]), "bias and bias_ids must have one shape and row stride")
+    _need(of["history"] is not None or (of["prompt_lens"] is None and of["history_lens"] is None), "lengths without a history")
+    _need(allowed is None or width["allowed"] == (vocab + 31) // 32, f"allowed must have {(vocab + 31) // 32} words a row")
+    n = rows if n is None else n
+    _need(of["requests"] is not None or n == rows, f"{n} requests for {rows} rows: requests must say which row is whose")
+    _same_device(logits[3], _LOGITS, looks)
+    if rows == 0:
+        return None
+    return _fixed(runtime.AdjustLogits, (rows, vocab, _FLOATS[logits[2]], _FLOATS[out[2]], n, width["history"], width["path"], width["bias"],
+                                         logits[1][0], out[1][0], step["history"], step["path"], step["bias_ids"], step["allowed"]))
 
 
 def adjust_logits(logits, requests=None, history=None, prompt_lens=None, history_lens=None, path=None, repetition=None, frequency=None,
@@ -350,59 +445,15 @@ def adjust_logits(logits, requests=None, history=None, prompt_lens=None, history
     the bias, then -inf where it is not allowed.  fp32 arithmetic, rounded once; the tokens are chosen before that rounding."""
     one = isinstance(logits, torch.Tensor) and logits.dim() == 1
     if one:
-        logits, out = logits[None], out[None] if out is not None else None
-    _need(isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dtype in _FLOATS and logits.dim() == 2,
-          "logits must be [rows, vocab] fp32, bf16 or f16 on the GPU")
-    rows, vocab = logits.shape
-    _need(vocab >= 1 and (vocab == 1 or logits.stride(1) == 1), "a row's logits must lie one behind the other")
+        logits, out = logits[None], out[None] if isinstance(out, torch.Tensor) else out
+    _need(isinstance(logits, torch.Tensor), "logits must be [rows, vocab] fp32, bf16 or f16 on the GPU")
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-    else:
-        _need(isinstance(out, torch.Tensor) and out.shape == logits.shape and out.dtype in (logits.dtype, torch.float32) and
-              (vocab == 1 or out.stride(1) == 1), "out must be like the logits, or fp32")
-    n = None
-
-    def table(name, t, dtype, dims, per_row=False):
-        """Address and row stride of a table of requests (or rows)."""
-        nonlocal n
-        if t is None:
-            return 0, 0
-        _on_gpu(name, t, dtype, dims)
-        if dims == 2:
-            _need(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: a row's values must lie one behind the other")
-        else:
-            _need(t.shape[0] <= 1 or t.stride(0) == 1, f"{name}: values must lie one behind the other")
-        if not per_row and n is None:
-            n = t.shape[0]
-        _need(t.shape[0] == (rows if per_row else n), f"{name} has {t.shape[0]} rows, not {rows if per_row else n}")
-        return t.data_ptr(), t.stride(0) if dims == 2 else 0
-
-    i32, f32 = torch.int32, torch.float32
-    p_hist, hist_s = table("history", history, i32, 2)
-    p_prompt, _ = table("prompt_lens", prompt_lens, i32, 1)
-    p_lens, _ = table("history_lens", history_lens, i32, 1)
-    p_rep, _ = table("repetition", repetition, f32, 1)
-    p_freq, _ = table("frequency", frequency, f32, 1)
-    p_pres, _ = table("presence", presence, f32, 1)
-    p_ids, bias_s = table("bias_ids", bias_ids, i32, 2)
-    p_bias, bias_s2 = table("bias", bias, f32, 2)
-    p_path, path_s = table("path", path, i32, 2, True)
-    p_allowed, allowed_s = table("allowed", allowed, i32, 2, True)
-    p_req, _ = table("requests", requests, i32, 1, True)
-    _need((bias_ids is None) == (bias is None), "bias and bias_ids go together")
-    if bias is not None:
-        _need(bias.shape == bias_ids.shape and (n == 1 or bias_s == bias_s2), "bias and bias_ids must have one shape and row stride")
-    _need(history is not None or (prompt_lens is None and history_lens is None), "lengths without a history")
-    if allowed is not None:
-        _need(allowed.shape[1] == (vocab + 31) // 32, f"allowed must have {(vocab + 31) // 32} words a row")
-    n = rows if n is None else n
-    _need(requests is not None or n == rows, f"{n} requests for {rows} rows: requests must say which row is whose")
-    _same_device(logits, out, history, prompt_lens, history_lens, path, repetition, frequency, presence, bias_ids, bias, allowed, requests)
-    tokens = logits.new_empty(rows, dtype=i32)
-    if rows:
-        runtime.adjust_logits(runtime.AdjustLogits(
-            rows, vocab, _FLOATS[logits.dtype], _FLOATS[out.dtype], n, history.shape[1] if history is not None else 0,
-            path.shape[1] if path is not None else 0, bias.shape[1] if bias is not None else 0, logits.stride(0), out.stride(0), hist_s,
-            path_s, bias_s, allowed_s, logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), p_req, p_hist, p_prompt, p_lens, p_path, p_rep,
-            p_freq, p_pres, p_ids, p_bias, p_allowed), _stream(logits))
+    plan = _logits_plan(*_looks(_LOGITS, (logits, out, requests, history, prompt_lens, history_lens, path, repetition, frequency, presence,
+                                          bias_ids, bias, allowed)))
+    tokens = logits.new_empty(logits.shape[0], dtype=I32)
+    if plan is not None:
+        _run("vdc_adjust_logits", logits.get_device(), plan + _PACK14(
+            logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), _ptr(requests), _ptr(history), _ptr(prompt_lens), _ptr(history_lens),
+            _ptr(path), _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias_ids), _ptr(bias), _ptr(allowed)))
     return (out[0] if one else out), tokens
