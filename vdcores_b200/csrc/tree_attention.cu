@@ -84,6 +84,15 @@ __device__ __forceinline__ int2 seq_of(const vdc_tree_attention_args& a, const S
 
 __host__ __device__ __forceinline__ int tiles_of(const vdc_tree_attention_args& a) { return (a.T * a.group + kRows - 1) / kRows; }
 
+// Units of few pages are not divided, nor are those of some more where there are two for every SM: what the second kernel and the wait
+// for it cost (4 to 8 us) is more than what the CTAs' shares then differ by.  Divided / whole, us: 6 pages of 8 units 12.3 / 10.7, 16 of
+// 64 26.5 / 18.5, 16 of 512 48.3 / 40.3, 34 of 512 60.3 / 57.4, 32 of 8 18.2 / 16.5, 63 of 8 21 / 28.
+constexpr int kWholePages = 24, kWholePagesOfMany = 64;
+__host__ __device__ __forceinline__ bool whole_units(const vdc_tree_attention_args& a) {
+  return a.max_pages <= kWholePages ||
+         (a.max_pages <= kWholePagesOfMany && (long long)a.B * a.cache.n_kv * tiles_of(a) >= 2 * VDC_MAX_SMS);
+}
+
 // x / y of what mostly fits 32 bits (the long division is much code for a kernel's first microsecond).
 __device__ __forceinline__ long long quotient(long long x, long long y) {
   return ((unsigned long long)x | (unsigned long long)y) >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y);
@@ -137,7 +146,9 @@ __device__ __forceinline__ void find_share(const vdc_tree_attention_args& a, Sha
     base += __shfl_sync(~0u, sum, 31);
   }
   if (lane == 0) {
-    sh.begin = begin;
+    // (a unit that is not divided is its first page's CTA's)
+    const int np = whole_units(a) && begin < end ? pages_of(seq_of(a, sh, first)) : 1;
+    sh.begin = base + (begin - base + np - 1) / np * np;
     sh.end = end;
     sh.first_base = base;
     sh.first_b = first;
@@ -169,7 +180,7 @@ struct Walk {
     p.head = tiles == 1 ? u : u / tiles;
     p.tile = tiles == 1 ? 0 : u % tiles;
     p.p0 = (int)(x - base - (long long)u * p.np);
-    p.p1 = (int)min((long long)p.np, p.p0 + (end - x));
+    p.p1 = whole_units(a) ? p.np : (int)min((long long)p.np, p.p0 + (end - x));
     x += p.p1 - p.p0;
     return true;
   }
@@ -1737,6 +1748,7 @@ extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* 
   const int ctas = ctas_of(a, sms);
   v.run<<<ctas, v.threads, v.bytes, stream>>>(*a, maps[0], maps[1], status, timeout_ns);
   if (cudaError_t e = cudaGetLastError()) return e;
+  if (whole_units(*a)) return cudaSuccess;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a->B * c.n_kv * tiles_of(*a)), (unsigned)(((rows < kRows ? rows : kRows) + kJoinWarps - 1) / kJoinWarps));
   cfg.blockDim = dim3(kJoinWarps * 32);
