@@ -42,9 +42,8 @@ struct Cfg {
   static constexpr float kLift = kF8 ? 11.f : 0.f;      // f16 weights are kept that much larger: 2^15 at most, 2^-25 of the largest with all bits
 };
 constexpr int kSeqs = 512, kWideBufs = 4, kWideBytes = PAGE * D * 2;
-constexpr int kScratchRow = 36;                         // floats of a row's 32 sums on their way between warps
-constexpr int kScratch = kMathWarps * 32 * kScratchRow * 4;
 constexpr int kQRow = 68;                               // words of a query row on its way to tensor memory: 256 bytes, apart for the banks' sake
+constexpr int kScratch = kRows * kQRow * 4;
 
 // columns of tensor memory
 constexpr int kColO = 0, kColS = 256, kColP = 384, kColQ = 448, kCols = 512;
@@ -705,18 +704,25 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       const bool live = r < rows && t < p.live;
       const int n = p.p1 - p.p0;
       bool failed = false;
-      // the tile's rows: half a warp loads one, every copy of it goes from shared memory to its lane
+      // the tile's rows: half a warp loads one (all loads first), and it goes from shared memory to its lane
       {
         const int sub = lane & 15;
         const unsigned half = 0xFFFFu << (lane & 16);
         const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+        constexpr int kEach = kRows / (kMathWarps * 2);
+        uint4 q[kEach];
 #pragma unroll
-        for (int rr = warp * 2 + (lane >> 4); rr < kRows; rr += kMathWarps * 2) {
-          const int qr = p.tile * kRows + rr;
-          uint4 v = make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < kEach; ++k) {
+          const int qr = p.tile * kRows + warp * 2 + (lane >> 4) + k * kMathWarps * 2;
+          q[k] = make_uint4(0, 0, 0, 0);
           if (qr < rows && row_of.token(qr) < p.live)
-            v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + p.b * a.q_b + p.head * a.q_kv +
-                                                     row_of.at(qr, a.q_t, a.q_g)) + sub);
+            q[k] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + p.b * a.q_b + p.head * a.q_kv +
+                                                        row_of.at(qr, a.q_t, a.q_g)) + sub);
+        }
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+          const int rr = warp * 2 + (lane >> 4) + k * kMathWarps * 2;
+          uint4 v = q[k];
           v.x ^= sign; v.y ^= sign; v.z ^= sign; v.w ^= sign;
           uint32_t* to = q_rows + rr * kQRow;
           if constexpr (!kF8) {
@@ -731,6 +737,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
         }
       }
       math_sync();
+      if (tid == 0 && turn > 0) sh.bad[(turn & 1) ^ 1] = 0;      // (everybody is through with the piece in front)
       if (w == 0) {
 #pragma unroll
         for (int j = 0; j < 64; j += 16) {
@@ -870,53 +877,46 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       if (!failed && has) failed = !all_well(spin(&sh.o_done[w], (c & 1) ^ 1, wait), wait, 5, n);
       sh.stats[warp][lane] = make_float2(m, l);
       if (math_any(failed)) break;
-      // ---- the groups' sums meet: statistics first (both look at both), then 32 columns at a time
+      // ---- the groups' sums meet: a thread reaches its row's sums of both, and takes half of the values
       const float2 other = sh.stats[warp ^ 4][lane];
       float mm = fmaxf(m, other.x);
       // a group that saw nothing has no weight; one without a number passes that on
       float ll = l * (m == -INFINITY ? 1.f : exp2_ftz(m - mm)) + other.y * (other.x == -INFINITY ? 1.f : exp2_ftz(other.x - mm));
       if (sh.bad[turn & 1] || !live) mm = -INFINITY, ll = 0.f;
-      const bool whole = p.whole(), none = !has || ll == 0.f || (m == -INFINITY && l == 0.f);
-      const float f = (m == -INFINITY ? 1.f : exp2_ftz(m - mm)) * (whole && ll != 0.f ? 1.f / ll : 1.f);
+      const bool whole = p.whole();
+      const float share = whole && ll != 0.f ? 1.f / ll : 1.f;
+      const bool has_other = n > (w ^ 1);
+      const bool none = !has || ll == 0.f || (m == -INFINITY && l == 0.f), none_other = !has_other || ll == 0.f || (other.x == -INFINITY && other.y == 0.f);
+      const float f = (m == -INFINITY ? 1.f : exp2_ftz(m - mm)) * share, f_other = (other.x == -INFINITY ? 1.f : exp2_ftz(other.x - mm)) * share;
       float* rec = record_of(a, blockIdx.x, p.p1 == p.np);
       const int tile_rows = min(rows - p.tile * kRows, kRows);
-      if (!whole && tid < tile_rows) *reinterpret_cast<float2*>(rec + min(rows, kRows) * D + 2 * tid) = make_float2(mm, ll);
-      __nv_bfloat16* to[kRows / 32];
-#pragma unroll
-      for (int k = 0; k < kRows / 32; ++k) {
-        const int rr = (tid >> 3) + k * 32;
-        to[k] = out_row(a, row_of, p.b, p.head, p.tile * kRows + rr) + (tid & 7) * 4;
-      }
+      const bool exists = tile_row < tile_rows;
+      if (!whole && exists && w == 0) *reinterpret_cast<float2*>(rec + min(rows, kRows) * D + 2 * tile_row) = make_float2(mm, ll);
+      rec += tile_row * D + w * (D / 2);
+      __nv_bfloat16* to = out_row(a, row_of, p.b, p.head, p.tile * kRows + tile_row) + w * (D / 2);
       tc_fence_after();
-      float* mine = scratch + (warp * 32 + lane) * kScratchRow;
-      const float* theirs = scratch + (tid >> 3) * kScratchRow + (tid & 7) * 4;
 #pragma unroll 1
-      for (int col = 0; col < D; col += 32) {
-        uint32_t o[32];
+      for (int col = 0; col < D / 2; col += 16) {
+        uint32_t x[16], y[16];
+        float sum[16];
         __syncwarp();
-        if (has) tmem_load(lanes + kColO + w * D + col, o);
-        if (tile_row < tile_rows) {
+        if (has) tmem_load(lanes + kColO + w * D + w * (D / 2) + col, x);
+        if (has_other) tmem_load(lanes + kColO + (w ^ 1) * D + w * (D / 2) + col, y);
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(mine + j) = none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                        : make_float4(__uint_as_float(o[j]) * f, __uint_as_float(o[j + 1]) * f,
-                                                                      __uint_as_float(o[j + 2]) * f, __uint_as_float(o[j + 3]) * f);
-        }
-        math_sync();
+        for (int j = 0; j < 16; ++j)
+          sum[j] = (none ? 0.f : __uint_as_float(x[j]) * f) + (none_other ? 0.f : __uint_as_float(y[j]) * f_other);
+        if (!exists) continue;
 #pragma unroll
-        for (int k = 0; k < kRows / 32; ++k) {
-          const int rr = (tid >> 3) + k * 32;
-          if (rr < tile_rows) {
-            const float4 x = *reinterpret_cast<const float4*>(theirs + k * 32 * kScratchRow);
-            const float4 y = *reinterpret_cast<const float4*>(theirs + (4 + k) * 32 * kScratchRow);
-            const float4 sum = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-            if (whole) *reinterpret_cast<uint2*>(to[k] + col) = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
-            else *reinterpret_cast<float4*>(rec + rr * D + col + (tid & 7) * 4) = sum;
+        for (int j = 0; j < 16; j += 8) {
+          if (whole) {
+            const float v[8] = {sum[j], sum[j + 1], sum[j + 2], sum[j + 3], sum[j + 4], sum[j + 5], sum[j + 6], sum[j + 7]};
+            *reinterpret_cast<uint4*>(to + col + j) = pack8(v);
+          } else {
+            *reinterpret_cast<float4*>(rec + col + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+            *reinterpret_cast<float4*>(rec + col + j + 4) = make_float4(sum[j + 4], sum[j + 5], sum[j + 6], sum[j + 7]);
           }
         }
-        math_sync();
       }
-      if (tid == 0) sh.bad[turn & 1] = 0;
       tc_fence_before();
     }
     write_zeros(a, sh, row_of, status, kMathWarps * 32);
