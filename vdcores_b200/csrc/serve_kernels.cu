@@ -121,6 +121,8 @@ struct FourPairs {
 template <bool kF8, bool kPairs>
 __global__ void __launch_bounds__(kAppendMaxThreads, 4)
 rope_append(const __grid_constant__ vdc_rope_append_args a, const __grid_constant__ AppendStep step, vdc_status* status) {
+  grid_dep_wait();
+  grid_dep_launch();
   const int t = blockIdx.x, lane = threadIdx.x & 15, half_warp = threadIdx.x >> 4, half_warps = blockDim.x >> 4;
   const unsigned mask = 0xFFFFu << (threadIdx.x & 16);
   const vdc_cache& c = a.cache;
@@ -249,6 +251,8 @@ __device__ __forceinline__ uint4 stored8(const uint8_t* src, float scale) {
 
 template <bool kF8>
 __global__ void __launch_bounds__(kReadThreads) read_cache(const vdc_read_cache_args a, vdc_status* status) {
+  grid_dep_wait();
+  grid_dep_launch();
   const vdc_cache& c = a.cache;
   const int b = blockIdx.y, lane = threadIdx.x & 15;
   const unsigned units = (unsigned)a.n * c.n_kv, unit0 = blockIdx.x * kReadUnits + (threadIdx.x >> 4);
@@ -484,6 +488,8 @@ adjust_logits(const __grid_constant__ vdc_adjust_logits_args a, const __grid_con
 
   for (int i = tid; i < kLogitChunk * (kLogitThreads / 32); i += kLogitThreads) (&sh.best[0][0])[i] = -INFINITY, (&sh.at[0][0])[i] = 0x7FFFFFFF;
   __syncthreads();
+  grid_dep_wait();
+  grid_dep_launch();
   const int most_per = ((a.vocab + 7 + 7) / 8 + parts - 1) / parts;  // groups of a CTA at most, over all rows' alignments
   for (int tile0 = 0; tile0 < most_per; tile0 += plan.tile / 8) {
     int held = -1, held_lead = -1;      // whose list is in shared memory
@@ -750,6 +756,25 @@ extern "C" const char* vdc_rope_append_refuses(const vdc_rope_append_args* a) {
   return nullptr;
 }
 
+// A launch that may begin while the kernel in front ends; all kernels here wait for it before they look at anything.
+template <class... Params, class... Args>
+static cudaError_t launch(void (*run)(Params...), dim3 grid, int threads, int bytes, int cluster, cudaStream_t stream, const Args&... args) {
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)bytes;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, run, args...);
+}
+
 extern "C" cudaError_t vdc_rope_append_launch(const vdc_rope_append_args* a, vdc_status* status, cudaStream_t stream) {
   const dim3 grid((unsigned)a->T, (unsigned)(a->B < 65535 ? a->B : 65535));
   // As many half-warps for a token as the warps that can be resident allow: few tokens wait for one chain of loads, many for what each
@@ -766,8 +791,7 @@ extern "C" cudaError_t vdc_rope_append_launch(const vdc_rope_append_args* a, vdc
   step.o_wrap = (a->o_kv - a->group * a->o_g) / 4;
   const auto run = a->cache.kind ? a->interleaved ? rope_append<true, true> : rope_append<true, false>
                                  : a->interleaved ? rope_append<false, true> : rope_append<false, false>;
-  run<<<grid, threads, 0, stream>>>(*a, step, status);
-  return cudaGetLastError();
+  return launch(run, grid, threads, 0, 1, stream, *a, step, status);
 }
 
 extern "C" const char* vdc_read_cache_refuses(const vdc_read_cache_args* a) {
@@ -780,9 +804,7 @@ extern "C" const char* vdc_read_cache_refuses(const vdc_read_cache_args* a) {
 extern "C" cudaError_t vdc_read_cache_launch(const vdc_read_cache_args* a, vdc_status* status, cudaStream_t stream) {
   const unsigned units = (unsigned)a->n * a->cache.n_kv;
   const dim3 grid((units + kReadUnits - 1) / kReadUnits, (unsigned)a->B);
-  if (a->cache.kind) read_cache<true><<<grid, kReadThreads, 0, stream>>>(*a, status);
-  else read_cache<false><<<grid, kReadThreads, 0, stream>>>(*a, status);
-  return cudaGetLastError();
+  return launch(a->cache.kind ? read_cache<true> : read_cache<false>, grid, kReadThreads, 0, 1, stream, *a, status);
 }
 
 extern "C" const char* vdc_adjust_logits_refuses(const vdc_adjust_logits_args* a) {
@@ -817,18 +839,8 @@ static cudaError_t launch_logits(const vdc_adjust_logits_args* a, int sms, vdc_s
   const int64_t per = (((int64_t)a->vocab + 14) / 8 + plan.parts - 1) / plan.parts * 8;
   plan.tile = (int)(per < tile ? per : tile);
   plan.cap = (int)(text + bias < plan.tile ? text + bias : plan.tile);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((a->rows + plan.chunk - 1) / plan.chunk * plan.parts));
-  cfg.blockDim = dim3(kLogitThreads);
-  cfg.dynamicSmemBytes = plan.bytes(a->n_bias);
-  cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = (unsigned)plan.parts;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, adjust_logits<Tin, Tout>, *a, plan, status);
+  return launch(adjust_logits<Tin, Tout>, dim3((unsigned)((a->rows + plan.chunk - 1) / plan.chunk * plan.parts)), kLogitThreads, plan.bytes(a->n_bias),
+                plan.parts, stream, *a, plan, status);
 }
 
 extern "C" cudaError_t vdc_adjust_logits_launch(const vdc_adjust_logits_args* a, int sms, vdc_status* status, cudaStream_t stream) {

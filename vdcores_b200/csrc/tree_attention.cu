@@ -432,9 +432,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
   const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
   const Waiter wait{&sh.fail, status, timeout_ns, VDC_TREE_ATTENTION_KIND};
 
-  grid_dep_launch();
   if (warp == C::kScoreWarp) tmem_alloc(&sh.tmem, kCols);
-  for (int b = tid; b < min(a.B, kSeqs); b += C::kThreads) sh.seq[b] = seq_load(a, b);
   if (warp == 0) {
     if (lane == 0) {
       for (int i = 0; i < C::kStages; ++i) {
@@ -460,6 +458,9 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
     if (lane < 16) reinterpret_cast<uint32_t*>(sh.poison)[lane] = 0;
     if (lane < 2) sh.bad[lane] = 0;
   }
+  grid_dep_wait();                   // (so far nothing that a kernel in front may still write)
+  grid_dep_launch();
+  for (int b = tid; b < min(a.B, kSeqs); b += C::kThreads) sh.seq[b] = seq_load(a, b);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1029,9 +1030,7 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
   const int rows = a.T * a.group;
   const RowOf row_of(a.group);
 
-  grid_dep_launch();
   if (warp == C::kScoreWarp) tmem_alloc(&sh.tmem, C::kCols);
-  for (int b = tid; b < min(a.B, kSeqs); b += C::kThreads) sh.seq[b] = seq_load(a, b);
   if (warp == C::kLoadWarp && lane == 0) {
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&sh.full[i], 1);
@@ -1051,6 +1050,9 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
     sh.fail = sh.bad[0] = sh.bad[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  grid_dep_wait();                   // (so far nothing that a kernel in front may still write)
+  grid_dep_launch();
+  for (int b = tid; b < min(a.B, kSeqs); b += C::kThreads) sh.seq[b] = seq_load(a, b);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1590,10 +1592,11 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
 
 // Joins the pieces of units that several CTAs shared: a warp per row, lane i the values 4i .. 4i + 3.  Pieces are taken in order,
 // so that the result does not depend on when they came.  What it needs to know of the sequences it looks up before the kernel in front
-// has ended (that one began when everything before it was done).
+// has ended (which let this one begin when everything before was done).
 constexpr int kJoinWarps = 4;
 __global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_constant__ vdc_tree_attention_args a, int ctas) {
   __shared__ long long part[2][kJoinWarps];
+  grid_dep_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rr = blockIdx.y * kJoinWarps + warp;
   const int tiles = tiles_of(a), units = a.cache.n_kv * tiles, b = blockIdx.x / units, u = blockIdx.x - b * units;
   const int rows = a.T * a.group, r = (u % tiles) * kRows + rr, rec_rows = min(rows, kRows);
@@ -1619,18 +1622,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_consta
   } else {
     total = np;
   }
-  if (np == 0 || r >= rows || rr >= kRows) return;
-  total *= units;
-  const long long first = before * units + (long long)u * np;
-  ctas = (int)min((long long)ctas, total);
-  const int c0 = (int)quotient((first + 1) * ctas - 1, total), c1 = (int)quotient((first + np) * ctas - 1, total);
+  int c0 = 0, c1 = 0;
+  if (np > 0 && r < rows && rr < kRows) {
+    total *= units;
+    const long long first = before * units + (long long)u * np;
+    ctas = (int)min((long long)ctas, total);
+    c0 = (int)quotient((first + 1) * ctas - 1, total);
+    c1 = (int)quotient((first + np) * ctas - 1, total);
+  }
+  grid_dep_wait();                       // (all of them: a kernel behind takes this one's end for the end of the one in front, too)
   if (c0 == c1) return;
   __nv_bfloat16* out = out_row(a, RowOf(a.group), b, u / tiles, r) + lane * 4;
   const float* rec0 = record_of(a, c0, false);
   const long long step = record_floats(a);
   auto record = [&](int c) { return rec0 + (2 * (c - c0) - (c == c1 ? 1 : 0)) * step; };
   auto stats = [&](int c) { return __ldcg(reinterpret_cast<const float2*>(record(c) + rec_rows * D + 2 * rr)); };
-  grid_dep_wait();
   float2 st = c0 + lane <= c1 ? stats(c0 + lane) : make_float2(-INFINITY, 0.f);
   float m = st.x;
   for (int c = c0 + 32 + lane; c <= c1; c += 32) m = fmaxf(m, stats(c).x);
@@ -1746,17 +1752,20 @@ extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* 
   }
   const Variant& v = kVariants[c.kind][rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 3 : 4];
   const int ctas = ctas_of(a, sms);
-  v.run<<<ctas, v.threads, v.bytes, stream>>>(*a, maps[0], maps[1], status, timeout_ns);
-  if (cudaError_t e = cudaGetLastError()) return e;
-  if (whole_units(*a)) return cudaSuccess;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(a->B * c.n_kv * tiles_of(*a)), (unsigned)(((rows < kRows ? rows : kRows) + kJoinWarps - 1) / kJoinWarps));
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = stream;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)v.threads);
+  cfg.dynamicSmemBytes = v.bytes;
+  cfg.stream = stream;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
+  if (cudaError_t e = cudaLaunchKernelEx(&cfg, v.run, *a, maps[0], maps[1], status, timeout_ns)) return e;
+  if (whole_units(*a)) return cudaSuccess;
+  cfg.gridDim = dim3((unsigned)(a->B * c.n_kv * tiles_of(*a)), (unsigned)(((rows < kRows ? rows : kRows) + kJoinWarps - 1) / kJoinWarps));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, tree_join, *a, ctas);
 }
