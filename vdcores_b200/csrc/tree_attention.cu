@@ -932,19 +932,20 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
 }
 
 // ------------------------------------------------------------------------- //
-// Up to 64 rows: the keys lie on the lanes.  A step is two pages: S^T = K Q^T (128 keys by the rows), a thread has one key's scores
+// Few rows (up to 32 of bf16, 64 of e4m3): the keys lie on the lanes.  A step is two pages: S^T = K Q^T (128 keys by the rows), a thread has one key's scores
 // and, of e4m3, its scales; O^T += V^T P^T (128 values by the rows) with P in shared memory, written by its key's thread, eight rows
 // of a key in 16 bytes.  The tensor cores then work for the rows that exist and not for 128, a thread needs no other key's scale,
 // the drafted tokens' tests are a thread's own, and two pages pass each role at a time.
 //
 // Two groups of four warps take the steps in turn, with references and sums O^T of their own (a warp reaches 32 of the 128 values
-// only, so that a group has to rescale together); with more than 32 rows they share each step, half of the rows to a group
-// (registers).  A step first asks whether any of the group's scores exceeds its row's reference by too much (one barrier of the
+// only, so that a group has to rescale together); with more than 32 rows (e4m3 only) they share each step, half of the rows to a
+// group (registers).  A step first asks whether any of the group's scores exceeds its row's reference by too much (one barrier of the
 // group); only then, which after the first steps is rare, the maxima are looked for, and the sums rescaled.
 // ------------------------------------------------------------------------- //
 template <bool kF8, int R>
 struct KeysCfg {
   static constexpr bool kSplit = R > 32;                                // the groups share a step's rows
+  static_assert(kF8 || !kSplit, "bf16 values are looked over by the one group that has the step");
   static constexpr int kOwn = kSplit ? R / 2 : R;                       // rows of a thread
   static constexpr int kN = R < 16 ? 16 : R, kSums = kSplit ? 1 : 2;    // columns of S^T and O^T; how many O^T there are
   static constexpr int kCols = (2 + kSums) * kN <= 64 ? 64 : (2 + kSums) * kN <= 128 ? 128 : 256;
@@ -967,7 +968,7 @@ struct KeysCfg {
 constexpr float kNoRef = 1e30f;              // minus the reference of a row that has none yet
 
 struct KeysShared : ShareShared {
-  uint64_t full[8], empty[8], q_full, s_full[2], s_empty[2], p_full[2], o_done[2], v_full[2], v_empty[2], checked;
+  uint64_t full[8], empty[8], q_full, s_full[2], s_empty[2], p_full[2], o_done[2], v_full[2], v_empty[2];
   uint32_t tmem;
   Piece piece[2];                            // the math warps' (this one and the next, live < 0: there is none), and where their walk is
   long long walk_x, walk_base;
@@ -978,7 +979,6 @@ struct KeysShared : ShareShared {
   alignas(16) float ref[2][64];              // of a group's rows: minus the reference
   alignas(16) float factor[2][64];           // what their sums are multiplied by
   float most[kMathWarps][64];                // of a warp's rows: largest score, or sum of weights
-  uint8_t odd[4][128];                       // of a key: a drafted token whose bf16 values are no numbers
   alignas(16) float scales[4][2][128];
 };
 
@@ -1046,7 +1046,6 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
       mbar_init(&sh.v_full[i], 4);
       mbar_init(&sh.v_empty[i], 1);
     }
-    mbar_init(&sh.checked, 4);
     sh.fail = sh.bad[0] = sh.bad[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -1236,7 +1235,7 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
     const int w = warp >> 2, key = tid & 127, r0 = C::kSplit ? w * RT : 0;           // group, the thread's key of a step, its first row
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const uint32_t mine_o = col_o + lanes + (C::kSplit ? 0 : w * C::kN) + r0;        // the group's sums of the warp's 32 values
-    uint32_t g = 0, tails = 0;        // steps of the CTA, and those with drafted tokens
+    uint32_t g = 0;                   // steps of the CTA
     uint64_t l[RT / 2];               // sums of weights of two rows each
     // One thread's walk over the pieces (in shared memory: there are no registers to spare).
     auto step = [&](int turn) {
@@ -1463,7 +1462,7 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
           bool none = false;
           if constexpr (kF8) {
             if (mine >= end) inv = 0.f;
-          } else if (!C::kSplit || w == 0) {
+          } else {
             good &= spin(&sh.o_done[b], ph ^ 1, wait);      // (the sums first, as for the teams that widen)
             good &= spin(&sh.full[val_slot(g)], val_phase(g), wait);
             uint4* v = reinterpret_cast<uint4*>(ring + val_slot(g) * C::kPart + key * 128);
@@ -1480,16 +1479,7 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
               for (int x = 0; x < 16; ++x) v[(x >> 3) * (C::kPart / 32) + (x & 7)] = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
-            if constexpr (C::kSplit) {
-              sh.odd[g & 3][key] = none;
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&sh.checked);
-            }
-          } else {                                // the other group has looked at the values
-            good &= spin(&sh.checked, tails & 1, wait);
-            none = sh.odd[g & 3][key];
           }
-          ++tails;
           see >>= r0;
 #pragma unroll
           for (int r = 0; r < RT; r += 2) {
@@ -1720,7 +1710,12 @@ template <bool kF8, int R>
 constexpr Variant keys() { return {tree_attention_keys<kF8, R>, KeysCfg<kF8, R>::kThreads, KeysCfg<kF8, R>::kBytes}; }
 template <bool kF8>
 constexpr Variant lanes() { return {tree_attention<kF8>, Cfg<kF8>::kThreads, dynamic_bytes<kF8>()}; }
-const Variant kVariants[2][5] = {{keys<false, 8>(), keys<false, 16>(), keys<false, 32>(), keys<false, 64>(), lanes<false>()},
+// By the rows of a KV head (tokens x heads of its group).  Measured on 8 sequences of 2066 .. 4131 rows, 8 heads, us with the kernel that
+// is taken / the next larger one / rows on the lanes:
+//          8 rows               16 rows              32 rows              64 rows
+//   bf16   29.4 / 29.8 / 31.9   30.1 / 31.0 / 32.5   31.8 / 36.0 / 33.7   35.7 with rows on the lanes, 37.3 with keys on them
+//   e4m3   22.6 / 23.4 / 40.0   23.6 / 31.4 / 40.6   32.4 / 36.9 / 41.4   37.8 / 42.3
+const Variant kVariants[2][5] = {{keys<false, 8>(), keys<false, 16>(), keys<false, 32>(), lanes<false>(), lanes<false>()},
                                  {keys<true, 8>(), keys<true, 16>(), keys<true, 32>(), keys<true, 64>(), lanes<true>()}};
 }  // namespace
 
