@@ -156,15 +156,17 @@ int vdc_launch_step(const vdc_step* step, uint64_t stream, uint64_t timeout_ns);
 
 /* ---- Operators for drafted tokens: they serve several sequences whose pages lie in one pool, and take their arguments as
  * device memory described by a struct.  None of them synchronises, allocates or keeps anything between calls, so calls on
- * different streams do not meet.  What they find wrong in device memory (a length, page, position or request outside what the
+ * different streams do not meet.  Each begins while the kernel in front of it in the stream ends, and waits for that end before it
+ * reads or writes anything.  What they find wrong in device memory (a length, page, position or request outside what the
  * struct says) is reported as VDC_ERR_RANGE through vdc_read_status; the row concerned is left out (its outputs are zero, a
  * picked token -1).  Pointers are device addresses, multiples of 16 where not said otherwise; strides of tensors are in
  * elements, those of pages in bytes.  No counterpart in the reference.
  *
  * A cache of one layer: page p and KV head h at k + p * k_page + h * k_head (v alike): VDC_KV_PAGE rows of VDC_HEAD_DIM values,
  * row r's 16-byte pieces at index (piece XOR (r mod 8)).  kind 0: bf16, as the decode engines keep it.  kind 1: e4m3 codes; row r
- * stands for code * scale with the fp32 scale number r at k_scale + p * ks_page + h * ks_head (v_scale alike).  Page strides are
- * multiples of 16. */
+ * stands for code * scale with the fp32 scale number r at k_scale + p * ks_page + h * ks_head (v_scale alike).  A row with a value
+ * that is no number has a scale that is none (so vdc_rope_append writes it); of a drafted token's values, codes that are none under
+ * a scale that is one count as zeros.  Page strides are multiples of 16. */
 typedef struct {
   uint64_t k, v, k_scale, v_scale;
   int64_t k_page, k_head, v_page, v_head, ks_page, ks_head, vs_page, vs_head;
@@ -190,8 +192,8 @@ typedef struct {
 } vdc_rope_append_args;
 int vdc_rope_append(const vdc_rope_append_args* args, uint64_t stream);
 
-/* Rows start[b] .. start[b] + n - 1 (start 0: from row 0) of every sequence to k_out and v_out [B, n, n_kv, 128] bf16, dense;
- * rows at or behind lengths[b] become zeros. */
+/* Rows start[b] .. start[b] + n - 1 (start 0: from row 0) of every sequence to k_out and v_out [B, n, n_kv, 128] bf16, dense (n * n_kv
+ * up to 2^30); rows at or behind lengths[b] become zeros. */
 typedef struct {
   vdc_cache cache;
   int32_t B, n, max_pages, reserved;

@@ -27,10 +27,10 @@ from . import isa, runtime
 BF16, F8, I32, I64, F32 = torch.bfloat16, torch.float8_e4m3fn, torch.int32, torch.int64, torch.float32
 D, PAGE = isa.HEAD_DIM, isa.KV_PAGE
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-# (the public way makes a stream object of it, a microsecond a call)
 _PACK5, _PACK7, _PACK11, _PACK14 = (struct.Struct(f"{n}Q").pack for n in (5, 7, 11, 14))      # pointers at an argument structure's end
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
-    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+# (the public ways make a stream object, and look whether CUDA is up: a microsecond and a half a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 # What a call checks depends on its tensors' shapes, strides, types and devices only; those make a "look" (None for what is not given).
@@ -72,13 +72,9 @@ def _vector(name, look, n, dtype=I32):
         _need(look[0][0] == n and (n <= 1 or look[1][0] == 1), f"{name} must have {n} values, one behind the other")
 
 
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
 def _run(fn, dev, args, *rest):
     """Enqueues a C call, whose arguments are bytes, on the current stream."""
-    if dev != torch.cuda.current_device():
+    if dev != _current_device():
         raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     runtime.enqueue(fn, dev, args, _raw_stream(dev), *rest)
 
@@ -249,6 +245,7 @@ def _append_plan(dev, n_kv, layout, eps, norms, *looks):
         _on_gpu(name, x, BF16, 4)
         _need(x[0] == (B, T, n_kv, D) and x[1][3] == 1, f"{name} must be [{B}, {T}, {n_kv}, {D}], a head's values one behind the other")
         kv += x[1][:3]
+    out = q if out is None else out          # (a new one, contiguous as q is)
     _need(out[0] == q[0], "out must have the shape of q")
     os = _heads("out", out, n_kv)[3]
     rot = rows = pos_b = pos_t = 0
@@ -286,9 +283,10 @@ def rope_append(q, k, v, cache: KVCache, pages, lengths, table=None, positions=N
     bf16 rows, fp32 arithmetic, one rounding at the end.  An e4m3 cache gets e4m3(x / s) with s = the row's largest magnitude / 448;
     a row with an infinity or NaN gets a scale that is one, and reads back as NaN."""
     _need(isinstance(cache, KVCache), "cache must be a KVCache")
-    names = _APPEND
+    given = out
     if out is None and isinstance(q, torch.Tensor):
         out = torch.empty_like(q)
+        given = None if q.is_contiguous() else out
     p_q = p_k = 0
     norms = ()
     if qk_norm is not None:
@@ -299,12 +297,13 @@ def rope_append(q, k, v, cache: KVCache, pages, lengths, table=None, positions=N
             norms = tuple(_looks(("qk_norm[0]", "qk_norm[1]"), qk_norm))
             _need(len(norms) == 2 and None not in norms, "qk_norm must be two bf16 vectors of 128 weights")
             p_q, p_k = (w.data_ptr() for w in qk_norm)
-    tensors = (q, k, v, pages, lengths, table, positions, counts, out)
-    plan = _append_plan(cache._device, cache.n_kv_heads, layout, eps, norms, *_looks(names, tensors))
+    plan = _append_plan(cache._device, cache.n_kv_heads, layout, eps, norms,
+                        *_looks(_APPEND, (q, k, v, pages, lengths, table, positions, counts, given)))
     if plan is not None:
         _run("vdc_rope_append", cache._device, cache._raw + plan + _PACK11(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), pages.data_ptr(), lengths.data_ptr(), _ptr(counts), _ptr(table),
-            _ptr(positions), p_q, p_k))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), pages.data_ptr(), lengths.data_ptr(),
+            0 if counts is None else counts.data_ptr(), 0 if table is None else table.data_ptr(),
+            0 if positions is None else positions.data_ptr(), p_q, p_k))
     return out
 
 
@@ -322,11 +321,11 @@ def read_cache(cache: KVCache, pages, lengths, n: int, start=None) -> Tuple[torc
     [B, n, n_kv, 128]; rows at or behind lengths[b] are zeros."""
     _need(isinstance(cache, KVCache), "cache must be a KVCache")
     B, plan = _read_plan(cache._device, cache.n_kv_heads, n, *_looks(("pages", "lengths", "start"), (pages, lengths, start)))
-    k = torch.empty((B, n, cache.n_kv_heads, D), dtype=BF16, device=cache.k.device)
+    k = lengths.new_empty((B, n, cache.n_kv_heads, D), dtype=BF16)
     v = torch.empty_like(k)
     if plan is not None:
-        _run("vdc_read_cache", cache._device, cache._raw + plan + _PACK5(pages.data_ptr(), lengths.data_ptr(), _ptr(start), k.data_ptr(),
-                                                                        v.data_ptr()))
+        _run("vdc_read_cache", cache._device, cache._raw + plan + _PACK5(pages.data_ptr(), lengths.data_ptr(), 0 if start is None else start.data_ptr(),
+                                                                        k.data_ptr(), v.data_ptr()))
     return k, v
 
 
@@ -335,6 +334,7 @@ def _attention_plan(dev, kind, n_kv, n_pool, scale, q, pages, lengths, mask, cou
     B, n_pages, pages_b = _tables(dev, pages, lengths, counts)
     qB, T, group, qs = _heads("q", q, n_kv)
     _need(qB == B, f"q has {qB} sequences, pages {B}")
+    out = q if out is None else out          # (a new one, contiguous as q is)
     _need(out[0] == q[0], "out must have the shape of q")
     os = _heads("out", out, n_kv)[3]
     words, mask_b, mask_t = -(-T // 64), 0, 0
@@ -365,20 +365,23 @@ def tree_attention(q, cache: KVCache, pages, lengths, mask=None, counts=None, sc
 
     Scores, softmax and sums are fp32.  A token with nothing to attend to gets zeros."""
     _need(isinstance(cache, KVCache), "cache must be a KVCache")
+    given = out
     if out is None and isinstance(q, torch.Tensor):
         out = torch.empty_like(q)
+        given = None if q.is_contiguous() else out
     elif out is q:
         raise ValueError("out must not be q")
     c, dev = cache._c, cache._device
     plan, nbytes = _attention_plan(dev, c.kind, c.n_kv, c.n_pages, scale, *_looks(
-        ("q", "pages", "lengths", "mask", "counts", "out"), (q, pages, lengths, mask, counts, out)))
+        ("q", "pages", "lengths", "mask", "counts", "out"), (q, pages, lengths, mask, counts, given)))
     if plan is None:
         return out
     p_q, p_out = q.data_ptr(), out.data_ptr()
     _need(p_q != p_out, "out must not be q")
     work = q.new_empty(nbytes // 2)
-    _run("vdc_tree_attention", dev, cache._raw + plan + _PACK7(p_q, p_out, pages.data_ptr(), lengths.data_ptr(), _ptr(counts), _ptr(mask),
-                                                               work.data_ptr()), 0)
+    _run("vdc_tree_attention", dev, cache._raw + plan + _PACK7(
+        p_q, p_out, pages.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr(),
+        0 if mask is None else mask.data_ptr(), work.data_ptr()), 0)
     return out
 
 
@@ -453,7 +456,7 @@ def adjust_logits(logits, requests=None, history=None, prompt_lens=None, history
                                           bias_ids, bias, allowed)))
     tokens = logits.new_empty(logits.shape[0], dtype=I32)
     if plan is not None:
+        tables = (requests, history, prompt_lens, history_lens, path, repetition, frequency, presence, bias_ids, bias, allowed)
         _run("vdc_adjust_logits", logits.get_device(), plan + _PACK14(
-            logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), _ptr(requests), _ptr(history), _ptr(prompt_lens), _ptr(history_lens),
-            _ptr(path), _ptr(repetition), _ptr(frequency), _ptr(presence), _ptr(bias_ids), _ptr(bias), _ptr(allowed)))
+            logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), *[0 if t is None else t.data_ptr() for t in tables]))
     return (out[0] if one else out), tokens
