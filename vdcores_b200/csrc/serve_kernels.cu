@@ -34,8 +34,8 @@ __device__ __forceinline__ int page_of(const vdc_cache& c, const int* pages, int
 // crosses lanes, and the token's cosines and sines stay in registers over its heads.  Query rows are loaded four at a time and ahead
 // of the page table, whose chain of loads is what a token would otherwise wait for.  Products and sums are rounded one by one (no
 // contraction), so that the codes of a row do not depend on how the compiler pairs them.
-// 8192 tokens, 32 query and 2 x 4 cache heads, norms, e4m3: 44.5 us (bytes alone: 25); two thirds of the issue slots, the rest waits for
-// loads.  One token: 4.3 us.
+// 8192 tokens, 32 query and 2 x 4 cache heads, norms, e4m3: 42.5 us (bytes alone: 25); two thirds of the issue slots, the rest waits for
+// loads.  One token: 3.4 us.
 // ------------------------------------------------------------------------- //
 constexpr int kAppendMaxThreads = 256, kAppendRows = 4;
 
@@ -228,7 +228,7 @@ rope_append(const __grid_constant__ vdc_rope_append_args a, const __grid_constan
 
 // ------------------------------------------------------------------------- //
 // read_cache: a half-warp per row of one head, keys and values, two rows at a time so that more loads are on their way; rows are bytes
-// in and bytes out, so memory is the bound.  16 sequences of up to 4131 e4m3 rows of 8 heads: 65.6 us, 88 % of a plain copy's rate.
+// in and bytes out, so memory is the bound.  16 sequences of up to 4131 e4m3 rows of 8 heads: 63.5 us, 90 % of a plain copy's rate.
 // ------------------------------------------------------------------------- //
 constexpr int kReadThreads = 256, kReadRows = 2, kReadUnits = kReadThreads / 16 * kReadRows;
 
@@ -296,6 +296,8 @@ __global__ void __launch_bounds__(kReadThreads) read_cache(const vdc_read_cache_
 // Then rows stream through: logits come to shared memory several groups of eight ahead, are masked two at a time, written, and
 // compared; a listed one takes a turn by itself.
 // (Gathering the listed ones' logits afterwards, one to a thread, took as long as the rows themselves.)
+// 512 rows of 151936 bf16 logits, texts of 2048 .. 4096, 32 biases, masks: 80 us, 4.0 TB/s; two thirds of the issue slots, half of that for
+// the listed tokens.  One row of 128256: 12.4 us, of which the list takes 4.
 // ------------------------------------------------------------------------- //
 constexpr int kLogitThreads = 512, kLogitChunk = 8, kLogitMaxBias = 4096, kLogitMaxPath = 64;
 constexpr int kLogitTile = 262144, kLogitMaxNamed = 12288, kLogitSmallTile = 16384;      // tokens of a tile with so many listed ones at most, with more
