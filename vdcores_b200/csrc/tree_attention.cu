@@ -21,7 +21,7 @@
 //
 // Measured on one B200, calls back to back: 8 tokens over 131000 e4m3 rows 74 us (277 MB, 3.7 TB/s; steps alone 0.9 of the copy rate),
 // 64 tokens over 1056 .. 2112 e4m3 rows 57 us (215 MB, 3.8 TB/s), one token over 333 bf16 rows 9 us, 4 trees of 63 tokens with 8 heads a
-// group over 1025 .. 2050 bf16 rows 32 us.  Long sequences are bound by memory; short ones by a CTA's start, its steps in series (a wait
+// group over 1025 .. 2050 bf16 rows 29 us.  Long sequences are bound by memory; short ones by a CTA's start, its steps in series (a wait
 // for the scores, tensor memory, the group's barrier, weights, shared memory) and what joins the pieces.
 #include "mk_stage.cuh"
 
@@ -399,7 +399,7 @@ __device__ __forceinline__ bool names_no_page(const vdc_tree_attention_args& a, 
 }
 
 // The workspace: two records for each CTA, of a piece that reaches its unit's end and of one that does not: sums [rows][128] and
-// (reference, sum of weights) [rows], a multiple of 16 bytes.
+// (reference, sum of weights) [rows], a multiple of 16 bytes.  With rows on the lanes the sums are [32][rows][4], as the lanes write them.
 __host__ __device__ __forceinline__ long long record_floats(const vdc_tree_attention_args& a) {
   const int rows = a.T * a.group;
   return ((long long)(rows < kRows ? rows : kRows) * (D + 2) + 3) & ~3ll;
@@ -899,7 +899,7 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
       const int tile_rows = min(rows - p.tile * kRows, kRows);
       const bool exists = tile_row < tile_rows;
       if (!whole && exists && w == 0) *reinterpret_cast<float2*>(rec + min(rows, kRows) * D + 2 * tile_row) = make_float2(mm, ll);
-      rec += tile_row * D + w * (D / 2);
+      float4* mine = reinterpret_cast<float4*>(rec) + w * (D / 8) * min(rows, kRows) + tile_row;
       __nv_bfloat16* to = out_row(a, row_of, p.b, p.head, p.tile * kRows + tile_row) + w * (D / 2);
       tc_fence_after();
 #pragma unroll 1
@@ -919,8 +919,8 @@ tree_attention(const __grid_constant__ vdc_tree_attention_args a, const __grid_c
             const float v[8] = {sum[j], sum[j + 1], sum[j + 2], sum[j + 3], sum[j + 4], sum[j + 5], sum[j + 6], sum[j + 7]};
             *reinterpret_cast<uint4*>(to + col + j) = pack8(v);
           } else {
-            *reinterpret_cast<float4*>(rec + col + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
-            *reinterpret_cast<float4*>(rec + col + j + 4) = make_float4(sum[j + 4], sum[j + 5], sum[j + 6], sum[j + 7]);
+            mine[(col + j) / 4 * min(rows, kRows)] = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+            mine[((col + j) / 4 + 1) * min(rows, kRows)] = make_float4(sum[j + 4], sum[j + 5], sum[j + 6], sum[j + 7]);
           }
         }
       }
@@ -1586,15 +1586,16 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
   }
 }
 
-// Joins the pieces of units that several CTAs shared: a warp per row, lane i the values 4i .. 4i + 3; 4 to 8 us, bound by its two loads in
-// series (statistics, then sums).  Pieces are taken in order,
-// so that the result does not depend on when they came.  What it needs to know of the sequences it looks up before the kernel in front
-// has ended (which let this one begin when everything before was done).
+// Joins the pieces of units that several CTAs shared.  Records of keys on the lanes (rows of 128 sums): a warp per row, lane i the values
+// 4i .. 4i + 3.  Records of rows on the lanes (32 times four sums of every row): a thread per row, a block the same four values.  Pieces are
+// taken in order, so that the result does not depend on when they came.  What it needs to know of the sequences it looks up before the
+// kernel in front has ended (which let this one begin when everything before was done).  Some 4 us, bound by its loads in series.
 constexpr int kJoinWarps = 4;
+template <bool kLanes>
 __global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_constant__ vdc_tree_attention_args a, int ctas) {
   __shared__ long long part[2][kJoinWarps];
   grid_dep_launch();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rr = blockIdx.y * kJoinWarps + warp;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rr = kLanes ? threadIdx.x : blockIdx.y * kJoinWarps + warp;
   const int tiles = tiles_of(a), units = a.cache.n_kv * tiles, b = blockIdx.x / units, u = blockIdx.x - b * units;
   const int rows = a.T * a.group, r = (u % tiles) * kRows + rr, rec_rows = min(rows, kRows);
   // pages of all sequences and of those in front of this one
@@ -1629,11 +1630,39 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_consta
   }
   grid_dep_wait();                       // (all of them: a kernel behind takes this one's end for the end of the one in front, too)
   if (c0 == c1) return;
-  __nv_bfloat16* out = out_row(a, RowOf(a.group), b, u / tiles, r) + lane * 4;
+  __nv_bfloat16* out = out_row(a, RowOf(a.group), b, u / tiles, r) + (kLanes ? blockIdx.y : lane) * 4;
   const float* rec0 = record_of(a, c0, false);
   const long long step = record_floats(a);
   auto record = [&](int c) { return rec0 + (2 * (c - c0) - (c == c1 ? 1 : 0)) * step; };
   auto stats = [&](int c) { return __ldcg(reinterpret_cast<const float2*>(record(c) + rec_rows * D + 2 * rr)); };
+  if constexpr (kLanes) {
+    float m = -INFINITY, l = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = c0; c <= c1; c += 4) {
+      float2 st[4];
+      float4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool is = c + j <= c1;
+        st[j] = is ? stats(c + j) : make_float2(-INFINITY, 0.f);
+        x[j] = is ? __ldcg(reinterpret_cast<const float4*>(record(c + j)) + blockIdx.y * rec_rows + rr) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      const float was = m;
+      m = fmaxf(m, fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)));
+      auto take = [&](float ref) { return ref == -INFINITY ? 1.f : exp2_ftz(ref - m); };      // no reference: nothing, or no number
+      const float f0 = take(was);
+      l *= f0; sum.x *= f0; sum.y *= f0; sum.z *= f0; sum.w *= f0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = take(st[j].x);
+        l += st[j].y * f;
+        sum.x += x[j].x * f; sum.y += x[j].y * f; sum.z += x[j].z * f; sum.w += x[j].w * f;
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+    return;
+  }
   float2 st = c0 + lane <= c1 ? stats(c0 + lane) : make_float2(-INFINITY, 0.f);
   float m = st.x;
   for (int c = c0 + 32 + lane; c <= c1; c += 32) m = fmaxf(m, stats(c).x);
@@ -1712,11 +1741,12 @@ namespace {
 struct Variant {
   void (*run)(const vdc_tree_attention_args, const CUtensorMap, const CUtensorMap, vdc_status*, uint64_t);
   int threads, bytes;
+  bool on_lanes;      // the rows
 };
 template <bool kF8, int R>
-constexpr Variant keys() { return {tree_attention_keys<kF8, R>, KeysCfg<kF8, R>::kThreads, KeysCfg<kF8, R>::kBytes}; }
+constexpr Variant keys() { return {tree_attention_keys<kF8, R>, KeysCfg<kF8, R>::kThreads, KeysCfg<kF8, R>::kBytes, false}; }
 template <bool kF8>
-constexpr Variant lanes() { return {tree_attention<kF8>, Cfg<kF8>::kThreads, dynamic_bytes<kF8>()}; }
+constexpr Variant lanes() { return {tree_attention<kF8>, Cfg<kF8>::kThreads, dynamic_bytes<kF8>(), true}; }
 // By the rows of a KV head (tokens x heads of its group).  Measured on 8 sequences of 2066 .. 4131 rows, 8 heads, us with the kernel that
 // is taken / the next larger one / rows on the lanes:
 //          8 rows               16 rows              32 rows              64 rows
@@ -1766,8 +1796,8 @@ extern "C" cudaError_t vdc_tree_attention_launch(const vdc_tree_attention_args* 
   cfg.numAttrs = 1;
   if (cudaError_t e = cudaLaunchKernelEx(&cfg, v.run, *a, maps[0], maps[1], status, timeout_ns)) return e;
   if (whole_units(*a)) return cudaSuccess;
-  cfg.gridDim = dim3((unsigned)(a->B * c.n_kv * tiles_of(*a)), (unsigned)(((rows < kRows ? rows : kRows) + kJoinWarps - 1) / kJoinWarps));
+  cfg.gridDim = dim3((unsigned)(a->B * c.n_kv * tiles_of(*a)), v.on_lanes ? D / 4u : (unsigned)((rows + kJoinWarps - 1) / kJoinWarps));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, tree_join, *a, ctas);
+  return cudaLaunchKernelEx(&cfg, v.on_lanes ? tree_join<true> : tree_join<false>, *a, ctas);
 }
