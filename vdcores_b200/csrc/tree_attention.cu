@@ -19,10 +19,12 @@
 // memory, in two passes of the 8-bit tensor cores.  V is widened to f16 (exact) by two more teams of four warps; P is f16 as well (its
 // 11 bits are three more than the bf16 weights of bf16 caches have).
 //
-// Measured on one B200, calls back to back: 8 tokens over 131000 e4m3 rows 74 us (277 MB, 3.7 TB/s; steps alone 0.9 of the copy rate),
+// Measured on one B200, calls back to back: 8 tokens over 131000 e4m3 rows 77 us (277 MB, 3.6 TB/s; steps alone 0.9 of the copy rate),
 // 64 tokens over 1056 .. 2112 e4m3 rows 57 us (215 MB, 3.8 TB/s), one token over 333 bf16 rows 9 us, 4 trees of 63 tokens with 8 heads a
 // group over 1025 .. 2050 bf16 rows 29 us.  Long sequences are bound by memory; short ones by a CTA's start, its steps in series (a wait
 // for the scores, tensor memory, the group's barrier, weights, shared memory) and what joins the pieces.
+#include <type_traits>
+
 #include "mk_stage.cuh"
 
 namespace vdc {
@@ -121,6 +123,69 @@ struct Piece {
   __device__ __forceinline__ bool whole() const { return p0 == 0 && p1 == np; }
 };
 
+// Pages of a piece, where each CTA gets one piece of one unit at most: a second piece costs a CTA as much as seven pages do, so this is
+// the better way where its longest piece has few pages more than an even share has, and shares are short (long ones are bound by memory,
+// which does not wait for a CTA's second piece).  0: even shares.  Even shares / one piece each, us: one token over 4000 bf16 rows, 8
+// heads 19.4 / 15.8; 8 tokens over 16000 e4m3 rows 27.7 / 25.3; 8 trees of 16, 128 rows a head, over 1500 .. 3000 26.3 / 19.4; 40 tokens
+// over 30000, three units, 40 / 32; but 8 tokens over 131000 74 / 78, and 16 over 4000 .. 8000, the longest piece 37 pages more, 47 / 54.
+// A warp; `np` gives a sequence's pages.
+constexpr int kMinPiece = 4, kMaxShare = 48, kMaxMore = 7, kFewSeqs = (VDC_MAX_SMS + 31) / 32;
+template <class Pages>
+__device__ __forceinline__ int piece_pages(const vdc_tree_attention_args& a, Pages np, long long total, int ctas, int lane) {
+  const long long units = (long long)a.cache.n_kv * tiles_of(a);
+  if (whole_units(a) || a.B * units > ctas || total > (long long)kMaxShare * ctas) return 0;
+  int pages[kFewSeqs];
+#pragma unroll
+  for (int i = 0; i < kFewSeqs; ++i) pages[i] = 32 * i < a.B && lane + 32 * i < a.B ? np(lane + 32 * i) : 0;
+  const int share = max(kMinPiece, (int)((uint32_t)(total + ctas - 1) / (uint32_t)ctas));
+  auto fits = [&](int most) {
+    const float each = __frcp_rn((float)most);      // (few pages: the quotient's error is far below half of 1 / most)
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kFewSeqs; ++i)
+      if (32 * i < a.B) n += (int)(((float)(pages[i] + most - 1) + 0.5f) * each);
+    return (int)__reduce_add_sync(~0u, n) * units <= ctas;
+  };
+  if (!fits(share + kMaxMore)) return 0;
+  int less = 0;                                    // the fewest that do (more of them fit, too)
+#pragma unroll
+  for (int step = 4; step > 0; step >>= 1)
+    if (fits(share + kMaxMore - less - step)) less += step;
+  return share + kMaxMore - less;
+}
+
+// One warp: this CTA's piece, where it gets one.
+__device__ __forceinline__ bool share_one_piece(const vdc_tree_attention_args& a, ShareShared& sh, long long total, int lane) {
+  const int units = a.cache.n_kv * tiles_of(a), most = piece_pages(a, [&](int b) { return pages_of(seq_of(a, sh, b)); }, total, gridDim.x, lane);
+  if (most == 0) return false;
+  long long base = 0;                            // pages and pieces of the sequences in front
+  int pieces = 0;
+  if (lane == 0) sh.begin = sh.end = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int np = b0 + lane < a.B ? pages_of(seq_of(a, sh, b0 + lane)) : 0, k = (np + most - 1) / most;      // (32 sequences: 32 bits)
+    int sum = k;
+    long long pages = np;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int below = __shfl_up_sync(~0u, sum, o);
+      const long long below_pages = __shfl_up_sync(~0u, pages, o);
+      if (lane >= o) sum += below, pages += below_pages;
+    }
+    const int at = (int)blockIdx.x - pieces - (sum - k) * units;      // among the pieces of the lane's sequence
+    if (at >= 0 && at < k * units) {
+      const int u = at / k, j = at - u * k;
+      const long long p0 = quotient((long long)j * np, k), p1 = quotient((long long)(j + 1) * np, k);
+      sh.first_b = b0 + lane;
+      sh.first_base = base + (pages - np) * units;
+      sh.begin = sh.first_base + (long long)u * np + p0;
+      sh.end = sh.begin + p1 - p0;
+    }
+    pieces += __shfl_sync(~0u, sum, 31) * units;
+    base += __shfl_sync(~0u, pages, 31) * units;
+  }
+  return true;
+}
+
 // One warp: this CTA's share of all units' pages, and the sequence it begins in.
 __device__ __forceinline__ void find_share(const vdc_tree_attention_args& a, ShareShared& sh, int lane) {
   const long long units = (long long)a.cache.n_kv * tiles_of(a);
@@ -129,6 +194,7 @@ __device__ __forceinline__ void find_share(const vdc_tree_attention_args& a, Sha
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(~0u, total, o);
   total *= units;
+  if (share_one_piece(a, sh, total, lane)) return;
   const long long ctas = min((long long)gridDim.x, max(total, 1ll)), me = min((long long)blockIdx.x, ctas);    // a page each at least
   const long long begin = quotient(total * me, ctas), end = quotient(total * min(me + 1, ctas), ctas);
   long long base = 0;
@@ -1621,12 +1687,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_consta
     total = np;
   }
   int c0 = 0, c1 = 0;
-  if (np > 0 && r < rows && rr < kRows) {
+  if (const int most = piece_pages(a, [&](int i) { return pages_of(seq_load(a, i)); }, total * units, ctas, lane)) {
+    int pieces = 0;
+    for (int i = lane; i < b; i += 32) pieces += (pages_of(seq_load(a, i)) + most - 1) / most;
+    const int k = (np + most - 1) / most;
+    c0 = __reduce_add_sync(~0u, pieces) * units + u * k;
+    c1 = np > 0 && r < rows && rr < kRows ? c0 + k - 1 : c0;
+  } else if (np > 0 && r < rows && rr < kRows) {
     total *= units;
     const long long first = before * units + (long long)u * np;
-    ctas = (int)min((long long)ctas, total);
-    c0 = (int)quotient((first + 1) * ctas - 1, total);
-    c1 = (int)quotient((first + np) * ctas - 1, total);
+    const int n = (int)min((long long)ctas, total);
+    c0 = (int)quotient((first + 1) * n - 1, total);
+    c1 = (int)quotient((first + np) * n - 1, total);
   }
   grid_dep_wait();                       // (all of them: a kernel behind takes this one's end for the end of the one in front, too)
   if (c0 == c1) return;
@@ -1638,26 +1710,33 @@ __global__ void __launch_bounds__(kJoinWarps * 32) tree_join(const __grid_consta
   if constexpr (kLanes) {
     float m = -INFINITY, l = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = c0; c <= c1; c += 4) {
-      float2 st[4];
-      float4 x[4];
+    auto take = [&](auto at_once, int c) {
+      constexpr int kAtOnce = decltype(at_once)::value;
+      float2 st[kAtOnce];
+      float4 x[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < kAtOnce; ++j) {
         const bool is = c + j <= c1;
         st[j] = is ? stats(c + j) : make_float2(-INFINITY, 0.f);
         x[j] = is ? __ldcg(reinterpret_cast<const float4*>(record(c + j)) + blockIdx.y * rec_rows + rr) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       const float was = m;
-      m = fmaxf(m, fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)));
-      auto take = [&](float ref) { return ref == -INFINITY ? 1.f : exp2_ftz(ref - m); };      // no reference: nothing, or no number
-      const float f0 = take(was);
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) m = fmaxf(m, st[j].x);
+      auto factor = [&](float ref) { return ref == -INFINITY ? 1.f : exp2_ftz(ref - m); };      // no reference: nothing, or no number
+      const float f0 = factor(was);
       l *= f0; sum.x *= f0; sum.y *= f0; sum.z *= f0; sum.w *= f0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float f = take(st[j].x);
+      for (int j = 0; j < kAtOnce; ++j) {
+        const float f = factor(st[j].x);
         l += st[j].y * f;
         sum.x += x[j].x * f; sum.y += x[j].y * f; sum.z += x[j].z * f; sum.w += x[j].w * f;
       }
+    };
+    if (c1 - c0 < 4) {
+      take(std::integral_constant<int, 4>{}, c0);
+    } else {
+      for (int c = c0; c <= c1; c += 8) take(std::integral_constant<int, 8>{}, c);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
