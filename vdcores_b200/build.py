@@ -1,5 +1,6 @@
 """Builds libvdcores_b200.so in-tree with nvcc for sm_100a:  python -m vdcores_b200.build"""
 import os
+import shutil
 import subprocess
 import sys
 
@@ -12,6 +13,7 @@ SOURCES = [os.path.join(HERE, "csrc", f) for f in ("megakernel.cu", "stage_kerne
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-shared",
          "-Xcompiler", "-fPIC", "-DVDC_NO_STREAMER"]
 OBJ_DIR = os.path.join(HERE, "build")
+BINDING, BINDING_SOURCE = os.path.join(HERE, "_binding.so"), os.path.join(HERE, "csrc", "binding.cpp")
 
 
 def needs_build() -> bool:
@@ -19,18 +21,19 @@ def needs_build() -> bool:
         return True
     t = os.path.getmtime(LIB)
     csrc = os.path.join(HERE, "csrc")
-    deps = [os.path.join(csrc, f) for f in os.listdir(csrc)] + [os.path.join(HERE, "..", "include", "vdcores.h")]
+    deps = [os.path.join(csrc, f) for f in os.listdir(csrc) if f != "binding.cpp"] + [os.path.join(HERE, "..", "include", "vdcores.h")]
     return any(os.path.getmtime(d) > t for d in deps)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """One object per source (compiled side by side, kept while neither it nor a header changes), then the library."""
+    build_binding(force)
     if not (force or needs_build()):
         return LIB
     nvcc = os.environ.get("NVCC", "nvcc")
     os.makedirs(OBJ_DIR, exist_ok=True)
     csrc = os.path.join(HERE, "csrc")
-    headers = [os.path.join(csrc, f) for f in os.listdir(csrc) if not f.endswith(".cu")]
+    headers = [os.path.join(csrc, f) for f in os.listdir(csrc) if not f.endswith((".cu", ".cpp"))]
     headers += [os.path.join(HERE, "..", "include", "vdcores.h"), os.path.abspath(__file__)]
     objs, running = [], []
     for src in SOURCES:
@@ -44,6 +47,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
         raise subprocess.CalledProcessError(1, failed[0])
     subprocess.check_call([nvcc, *FLAGS, "-o", LIB, *objs])
     return LIB
+
+
+def build_binding(force: bool = False) -> str:
+    """The calls of ops.py as an extension module against this interpreter's PyTorch (host code only)."""
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(BINDING_SOURCE), os.path.getmtime(os.path.abspath(__file__))):
+        return BINDING
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    nvcc = shutil.which(os.environ.get("NVCC", "nvcc"))
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include") if nvcc else "/usr/local/cuda/include"
+    include = [sysconfig.get_paths()["include"], os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda]
+    subprocess.check_call([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+                           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in include), "-o", BINDING,
+                           BINDING_SOURCE, f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"])
+    return BINDING
 
 
 def build_trace(define: str) -> str:

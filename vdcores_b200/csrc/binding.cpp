@@ -1,0 +1,255 @@
+// Calls of the drafted-token operators without Python's share of the time: what a call's checks depend on (shapes, strides, types and
+// devices) is read from the tensors here and looked up among the combinations that have passed them; only a new combination goes
+// through the checks in ops.py, which give the fixed part of the C arguments.  Per call there remain the outputs' allocation, the
+// pointers, and the C entry.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cstring>
+#include <string>
+#include <unordered_map>
+#include <vector>
+
+namespace {
+
+struct Plan {
+  std::string fixed;      // bytes of the arguments behind the cache, up to the pointers; empty: there is nothing to run
+  long long work;         // bytes of workspace
+  PyObject* extras;       // equal to the call's, held
+};
+
+// Where a pointer comes from: a tensor's place among the arguments (an absent one is 0), an allocation, or a place whose tensor also
+// holds what an absent one behind it would (the second half of 256 weights of two bytes).
+constexpr int kWork = 100, kTokens = 101, kFirst = 102, kSecond = 103, kSecondHalf = 200;
+enum Makes { kOutLike, kRowsOut, kLogitsOut };
+
+struct Site {
+  PyObject_HEAD
+  vectorcallfunc call;
+  int (*one)(const void*, uint64_t);
+  int (*timed)(const void*, uint64_t, uint64_t);
+  PyObject *plan, *failed;            // ops.py: the checks of a new combination; what to raise for a status
+  int makes, out, n_tensors;          // what is made, and where `out` stands among the tensors
+  std::vector<int>* pointers;
+  std::unordered_multimap<std::string, Plan>* plans;
+};
+
+void look(std::string& key, const at::Tensor& t) {
+  const auto size = t.sizes(), stride = t.strides();
+  const int64_t head = (int64_t)t.scalar_type() | (int64_t)t.device().type() << 16 | (int64_t)(uint8_t)t.device().index() << 32 | (int64_t)size.size() << 48;
+  key.append(reinterpret_cast<const char*>(&head), 8);
+  key.append(reinterpret_cast<const char*>(size.data()), 8 * size.size());
+  key.append(reinterpret_cast<const char*>(stride.data()), 8 * stride.size());
+}
+
+// run(cache bytes, extras, tensors ...): the outputs
+PyObject* site_call(PyObject* self, PyObject* const* args, size_t nargsf, PyObject* names) {
+  Site& s = *reinterpret_cast<Site*>(self);
+  const Py_ssize_t n = PyVectorcall_NARGS(nargsf);
+  if (n != s.n_tensors + 2 || (names && PyTuple_GET_SIZE(names)) || !PyBytes_Check(args[0]) || !PyTuple_Check(args[1])) {
+    PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
+    return nullptr;
+  }
+  HANDLE_TH_ERRORS
+  PyObject* const* in = args + 2;
+  const Py_hash_t hash = PyObject_Hash(args[1]);
+  if (hash == -1) return nullptr;
+  std::string key;
+  key.reserve(512);
+  key.append(reinterpret_cast<const char*>(&hash), sizeof hash);
+  at::Tensor made[2];
+  std::vector<const at::Tensor*> t(s.n_tensors, nullptr);
+  bool known = true;      // tensors, or absent
+  for (int i = 0; i < s.n_tensors; ++i) {
+    if (in[i] == Py_None) {
+      key.push_back(0);
+    } else if (THPVariable_Check(in[i])) {
+      const at::Tensor& x = THPVariable_Unpack(in[i]);
+      if (x.layout() != at::kStrided) {
+        known = false;
+        break;
+      }
+      t[i] = &x;
+      look(key, x);
+    } else {
+      known = false;
+      break;
+    }
+  }
+  Plan* p = nullptr;
+  if (known) {
+    const auto range = s.plans->equal_range(key);
+    for (auto it = range.first; it != range.second; ++it) {
+      const int same = PyObject_RichCompareBool(it->second.extras, args[1], Py_EQ);
+      if (same < 0) return nullptr;
+      if (same) {
+        p = &it->second;
+        break;
+      }
+    }
+  }
+  Plan fresh;
+  if (!p) {
+    PyObject* tuple = PyTuple_New(s.n_tensors);
+    if (!tuple) return nullptr;
+    for (int i = 0; i < s.n_tensors; ++i) {
+      Py_INCREF(in[i]);
+      PyTuple_SET_ITEM(tuple, i, in[i]);
+    }
+    PyObject* got = PyObject_CallFunctionObjArgs(s.plan, args[1], tuple, nullptr);      // (fixed or None, bytes of workspace), or raises
+    Py_DECREF(tuple);
+    if (!got) return nullptr;
+    PyObject* fixed;
+    long long work;
+    if (!PyArg_ParseTuple(got, "OL", &fixed, &work)) {
+      Py_DECREF(got);
+      return nullptr;
+    }
+    if (fixed != Py_None) fresh.fixed.assign(PyBytes_AS_STRING(fixed), (size_t)PyBytes_GET_SIZE(fixed));
+    fresh.work = work;
+    Py_DECREF(got);
+    if (!known) {
+      PyErr_SetString(PyExc_ValueError, "arguments must be dense tensors on the GPU");
+      return nullptr;
+    }
+    if (s.plans->size() >= 16384) {
+      for (auto& old : *s.plans) Py_DECREF(old.second.extras);
+      s.plans->clear();
+    }
+    Py_INCREF(args[1]);
+    fresh.extras = args[1];
+    p = &s.plans->emplace(key, std::move(fresh))->second;
+  }
+  const std::string fixed = p->fixed;      // (the table may change while an allocation runs)
+  const long long work_bytes = p->work;
+  const bool nothing = fixed.empty();
+
+  at::Tensor work, out;
+  if (s.makes == kRowsOut) {                // [B, n, heads, 128] from the extras (n, heads)
+    const long long rows = PyLong_AsLongLong(PyTuple_GET_ITEM(args[1], 1)), heads = PyLong_AsLongLong(PyTuple_GET_ITEM(args[1], 2));
+    made[0] = at::empty({t[0]->size(0), rows, heads, 128}, t[1]->options().dtype(at::kBFloat16));
+    made[1] = at::empty_like(made[0]);
+  } else {
+    if (!t[s.out])
+      out = s.makes == kLogitsOut ? at::empty_like(*t[0], t[0]->options(), at::MemoryFormat::Contiguous) : at::empty_like(*t[0]);
+    else
+      out = *t[s.out];
+    if (s.makes == kLogitsOut) made[1] = at::empty({t[0]->size(0)}, t[0]->options().dtype(at::kInt));
+    if (work_bytes) work = at::empty({work_bytes / 2}, t[0]->options());
+  }
+  if (!nothing) {
+    const int dev = t[0]->device().index();
+    if (dev != c10::cuda::current_device()) {
+      PyErr_Format(PyExc_ValueError, "the tensors are on cuda:%d, the current device is cuda:%d", dev, (int)c10::cuda::current_device());
+      return nullptr;
+    }
+    if (s.makes == kOutLike && s.timed && out.data_ptr() == t[0]->data_ptr()) {
+      PyErr_SetString(PyExc_ValueError, "out must not be q");
+      return nullptr;
+    }
+    const size_t raw = (size_t)PyBytes_GET_SIZE(args[0]), bytes = raw + fixed.size() + 8 * s.pointers->size();
+    alignas(16) char c[1024];
+    if (bytes > sizeof c) {
+      PyErr_SetString(PyExc_RuntimeError, "argument structure too long");
+      return nullptr;
+    }
+    std::memcpy(c, PyBytes_AS_STRING(args[0]), raw);
+    std::memcpy(c + raw, fixed.data(), fixed.size());
+    char* to = c + raw + fixed.size();
+    for (const int from : *s.pointers) {
+      uint64_t v = 0;
+      auto at = [](const at::Tensor& x) { return (uint64_t)(uintptr_t)x.data_ptr(); };
+      if (from == kWork) v = work.defined() ? at(work) : 0;
+      else if (from == kTokens || from == kSecond) v = at(made[1]);
+      else if (from == kFirst) v = at(made[0]);
+      else if (from >= kSecondHalf) v = t[from - kSecondHalf] ? at(*t[from - kSecondHalf]) : t[from - kSecondHalf - 1] ? at(*t[from - kSecondHalf - 1]) + 256 : 0;
+      else if (from == s.out && s.makes != kRowsOut) v = at(out);
+      else if (t[from]) v = at(*t[from]);
+      std::memcpy(to, &v, 8);
+      to += 8;
+    }
+    const uint64_t stream = (uint64_t)(uintptr_t)c10::cuda::getCurrentCUDAStream(dev).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = s.timed ? s.timed(c, stream, 0) : s.one(c, stream);
+    Py_END_ALLOW_THREADS
+    if (rc != 0) {
+      PyObject* r = PyObject_CallFunction(s.failed, "i", rc);
+      Py_XDECREF(r);
+      if (!PyErr_Occurred()) PyErr_Format(PyExc_RuntimeError, "status %d", rc);
+      return nullptr;
+    }
+  }
+  if (s.makes == kOutLike) {
+    if (t[s.out]) {
+      Py_INCREF(in[s.out]);
+      return in[s.out];
+    }
+    return THPVariable_Wrap(std::move(out));
+  }
+  PyObject *a, *b = THPVariable_Wrap(std::move(made[1]));
+  if (s.makes == kLogitsOut && t[s.out]) {
+    a = in[s.out];
+    Py_INCREF(a);
+  } else {
+    a = THPVariable_Wrap(s.makes == kRowsOut ? std::move(made[0]) : std::move(out));
+  }
+  if (!a || !b) {
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    return nullptr;
+  }
+  PyObject* both = PyTuple_Pack(2, a, b);
+  Py_DECREF(a);
+  Py_DECREF(b);
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+PyTypeObject SiteType = {PyVarObject_HEAD_INIT(nullptr, 0)};
+
+// site(entry's address, timed, plan, failed, makes, out, tensors, pointers): lives as long as the process
+PyObject* make_site(PyObject*, PyObject* args) {
+  unsigned long long entry;
+  int timed, makes, out, n;
+  PyObject *plan, *failed, *pointers;
+  if (!PyArg_ParseTuple(args, "KpOOiiiO!", &entry, &timed, &plan, &failed, &makes, &out, &n, &PyTuple_Type, &pointers)) return nullptr;
+  Site* s = PyObject_New(Site, &SiteType);
+  if (!s) return nullptr;
+  s->call = site_call;
+  s->one = timed ? nullptr : reinterpret_cast<int (*)(const void*, uint64_t)>((uintptr_t)entry);
+  s->timed = timed ? reinterpret_cast<int (*)(const void*, uint64_t, uint64_t)>((uintptr_t)entry) : nullptr;
+  Py_INCREF(plan);
+  Py_INCREF(failed);
+  s->plan = plan;
+  s->failed = failed;
+  s->makes = makes;
+  s->out = out;
+  s->n_tensors = n;
+  s->pointers = new std::vector<int>();
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(pointers); ++i) s->pointers->push_back((int)PyLong_AsLong(PyTuple_GET_ITEM(pointers, i)));
+  s->plans = new std::unordered_multimap<std::string, Plan>();
+  Py_INCREF(s);                               // (never freed: the tables belong to the process)
+  return reinterpret_cast<PyObject*>(s);
+}
+
+PyMethodDef methods[] = {{"site", make_site, METH_VARARGS, "A C entry with its checks and its table of combinations."}, {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", "Calls of the drafted-token operators.", -1, methods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__binding() {
+  SiteType.tp_name = "vdcores_b200._binding.Site";
+  SiteType.tp_basicsize = sizeof(Site);
+  SiteType.tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_HAVE_VECTORCALL;
+  SiteType.tp_vectorcall_offset = offsetof(Site, call);
+  SiteType.tp_call = PyVectorcall_Call;
+  if (PyType_Ready(&SiteType) < 0) return nullptr;
+  return PyModule_Create(&module);
+}

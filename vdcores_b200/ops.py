@@ -15,27 +15,27 @@ holds.  Heads have 128 values and a page 64 rows, as everywhere in the framework
 """
 from __future__ import annotations
 
-import functools
+import ctypes
 import math
-import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import isa, runtime
 
+try:
+    from . import _binding
+except ImportError as e:
+    raise ImportError("vdcores_b200/_binding.so is missing or does not fit this PyTorch: build it with `python -m vdcores_b200.build`") from e
+
 BF16, F8, I32, I64, F32 = torch.bfloat16, torch.float8_e4m3fn, torch.int32, torch.int64, torch.float32
 D, PAGE = isa.HEAD_DIM, isa.KV_PAGE
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_PACK5, _PACK7, _PACK11, _PACK14 = (struct.Struct(f"{n}Q").pack for n in (5, 7, 11, 14))      # pointers at an argument structure's end
-# (the public ways make a stream object, and look whether CUDA is up: a microsecond and a half a call)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 # What a call checks depends on its tensors' shapes, strides, types and devices only; those make a "look" (None for what is not given).
-# The checks run once for a combination of looks and give the fixed part of the C arguments, which is kept: a call then costs half
-# as much of the host's time.  Pointers are looked at anew, and in C.
+# The checks below run once for a combination of looks and give the fixed part of the C arguments, which csrc/binding.cpp keeps with the
+# combination: a call then costs a third of the host's time.  Pointers are looked at anew, and in C.
 def _look(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
@@ -72,11 +72,24 @@ def _vector(name, look, n, dtype=I32):
         _need(look[0][0] == n and (n <= 1 or look[1][0] == 1), f"{name} must have {n} values, one behind the other")
 
 
-def _run(fn, dev, args, *rest):
-    """Enqueues a C call, whose arguments are bytes, on the current stream."""
-    if dev != _current_device():
+def _here(dev):
+    """The tensors' device has to be the current one."""
+    if dev != torch.cuda.current_device():
         raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
-    runtime.enqueue(fn, dev, args, _raw_stream(dev), *rest)
+    runtime.init()
+
+
+def _failed(rc):
+    raise runtime.VdcError(rc, runtime.last_error())
+
+
+def _site(entry, plan, makes, out, names, pointers, timed=False):
+    """The entry as binding.cpp calls it: plan(extras, tensors) checks a new combination; pointers are places among `names`, or what
+    the call makes itself."""
+    made = dict(work=100, tokens=101, first=102, second=103)
+    places = tuple(made[x] if x in made else 200 + names.index(x[1:]) if x[0] == "+" else names.index(x) for x in pointers)
+    address = ctypes.cast(getattr(runtime._lib, entry), ctypes.c_void_p).value
+    return _binding.site(address, timed, plan, _failed, makes, names.index(out) if out else -1, len(names), places)
 
 
 def _heads(name, look, n_kv):
@@ -231,12 +244,13 @@ def tree_mask(parents, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
     return pack_mask(seen).view(*p.shape, -1).to(device), depth.view(p.shape).to(device)
 
 
-_APPEND = ("q", "k", "v", "pages", "lengths", "table", "positions", "counts", "out")
+_APPEND = ("q", "k", "v", "pages", "lengths", "table", "positions", "counts", "out", "w_q", "w_k")
 
 
-@functools.lru_cache(maxsize=4096)
-def _append_plan(dev, n_kv, layout, eps, norms, *looks):
-    q, k, v, pages, lengths, table, positions, counts, out = looks
+def _append_plan(extras, tensors):
+    dev, n_kv, layout, eps = extras
+    looks = _looks(_APPEND, tensors)
+    q, k, v, pages, lengths, table, positions, counts, out, w_q, w_k = looks
     B, n_pages, pages_b = _tables(dev, pages, lengths, counts)
     qB, T, group, qs = _heads("q", q, n_kv)
     _need(qB == B, f"q has {qB} sequences, pages {B}")
@@ -245,7 +259,7 @@ def _append_plan(dev, n_kv, layout, eps, norms, *looks):
         _on_gpu(name, x, BF16, 4)
         _need(x[0] == (B, T, n_kv, D) and x[1][3] == 1, f"{name} must be [{B}, {T}, {n_kv}, {D}], a head's values one behind the other")
         kv += x[1][:3]
-    out = q if out is None else out          # (a new one, contiguous as q is)
+    out = _look(torch.empty_like(tensors[0])) if out is None else out
     _need(out[0] == q[0], "out must have the shape of q")
     os = _heads("out", out, n_kv)[3]
     rot = rows = pos_b = pos_t = 0
@@ -258,15 +272,22 @@ def _append_plan(dev, n_kv, layout, eps, norms, *looks):
         _need(positions[0] == (B, T), f"positions must be [{B}, {T}]")
         pos_b, pos_t = positions[1]
     _need(layout in ("half", "interleaved"), f"unknown layout {layout!r}")
-    if len(norms) == 1:
-        _on_gpu("qk_norm", norms[0], BF16, 1)
-        _need(norms[0][0] == (2 * D,) and norms[0][1] == (1,), "qk_norm must be two bf16 vectors of 128 weights")
-    for i, w in enumerate(norms if len(norms) == 2 else ()):
-        _vector(f"qk_norm[{i}]", w, D, BF16)
-    _same_device(dev, _APPEND + ("qk_norm",) * len(norms), looks + norms)
+    if w_q is not None and w_k is None:
+        _need(w_q[2] == BF16 and w_q[3] >= 0 and math.prod(w_q[0]) == 2 * D and tensors[9].is_contiguous(),
+              "qk_norm must be two bf16 vectors of 128 weights")
+    else:
+        _need((w_q is None) == (w_k is None), "qk_norm must be two bf16 vectors of 128 weights")
+        _vector("qk_norm[0]", w_q, D, BF16)
+        _vector("qk_norm[1]", w_k, D, BF16)
+    _same_device(dev, _APPEND, looks)
+    _here(dev)
     if B == 0 or T == 0:
-        return None
-    return _fixed(runtime.RopeAppend, (B, T, group, rot, layout == "interleaved", rows, n_pages, eps, *qs, *kv, *os, pages_b, pos_b, pos_t))
+        return None, 0
+    return _fixed(runtime.RopeAppend, (B, T, group, rot, layout == "interleaved", rows, n_pages, eps, *qs, *kv, *os, pages_b, pos_b, pos_t)), 0
+
+
+_append = _site("vdc_rope_append", _append_plan, 0, "out", _APPEND, ("q", "k", "v", "out", "pages", "lengths", "counts", "table", "positions",
+                                                                     "w_q", "+w_k"))
 
 
 def rope_append(q, k, v, cache: KVCache, pages, lengths, table=None, positions=None, counts=None, layout: str = "half", qk_norm=None,
@@ -283,58 +304,44 @@ def rope_append(q, k, v, cache: KVCache, pages, lengths, table=None, positions=N
     bf16 rows, fp32 arithmetic, one rounding at the end.  An e4m3 cache gets e4m3(x / s) with s = the row's largest magnitude / 448;
     a row with an infinity or NaN gets a scale that is one, and reads back as NaN."""
     _need(isinstance(cache, KVCache), "cache must be a KVCache")
-    given = out
-    if out is None and isinstance(q, torch.Tensor):
-        out = torch.empty_like(q)
-        given = None if q.is_contiguous() else out
-    p_q = p_k = 0
-    norms = ()
-    if qk_norm is not None:
-        if isinstance(qk_norm, torch.Tensor):
-            norms, p_q = (_look(qk_norm.flatten() if qk_norm.is_contiguous() else qk_norm),), qk_norm.data_ptr()
-            p_k = p_q + 2 * D
-        else:
-            norms = tuple(_looks(("qk_norm[0]", "qk_norm[1]"), qk_norm))
-            _need(len(norms) == 2 and None not in norms, "qk_norm must be two bf16 vectors of 128 weights")
-            p_q, p_k = (w.data_ptr() for w in qk_norm)
-    plan = _append_plan(cache._device, cache.n_kv_heads, layout, eps, norms,
-                        *_looks(_APPEND, (q, k, v, pages, lengths, table, positions, counts, given)))
-    if plan is not None:
-        _run("vdc_rope_append", cache._device, cache._raw + plan + _PACK11(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), pages.data_ptr(), lengths.data_ptr(),
-            0 if counts is None else counts.data_ptr(), 0 if table is None else table.data_ptr(),
-            0 if positions is None else positions.data_ptr(), p_q, p_k))
-    return out
+    w_q, w_k = (qk_norm, None) if qk_norm is None or isinstance(qk_norm, torch.Tensor) else qk_norm
+    return _append(cache._raw, (cache._device, cache.n_kv_heads, layout, eps), q, k, v, pages, lengths, table, positions, counts, out, w_q, w_k)
 
 
-@functools.lru_cache(maxsize=4096)
-def _read_plan(dev, n_kv, n, pages, lengths, start):
+_READ = ("pages", "lengths", "start")
+
+
+def _read_plan(extras, tensors):
+    dev, n, n_kv = extras
+    pages, lengths, start = _looks(_READ, tensors)
     B, n_pages, pages_b = _tables(dev, pages, lengths)
-    _need(n >= 0, "n must not be negative")
+    _need(isinstance(n, int) and n >= 0, "n must be a number of rows, not negative")
     _vector("start", start, B)
     _same_device(dev, ("start",), (start,))
-    return B, _fixed(runtime.ReadCache, (B, n, n_pages, 0, pages_b)) if B and n else None
+    _here(dev)
+    return _fixed(runtime.ReadCache, (B, n, n_pages, 0, pages_b)) if B and n else None, 0
+
+
+_read = _site("vdc_read_cache", _read_plan, 1, None, _READ, ("pages", "lengths", "start", "first", "second"))
 
 
 def read_cache(cache: KVCache, pages, lengths, n: int, start=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of rows start .. start + n - 1 (start: int32 [B], default 0) of every sequence as dense bf16 tensors
     [B, n, n_kv, 128]; rows at or behind lengths[b] are zeros."""
     _need(isinstance(cache, KVCache), "cache must be a KVCache")
-    B, plan = _read_plan(cache._device, cache.n_kv_heads, n, *_looks(("pages", "lengths", "start"), (pages, lengths, start)))
-    k = lengths.new_empty((B, n, cache.n_kv_heads, D), dtype=BF16)
-    v = torch.empty_like(k)
-    if plan is not None:
-        _run("vdc_read_cache", cache._device, cache._raw + plan + _PACK5(pages.data_ptr(), lengths.data_ptr(), 0 if start is None else start.data_ptr(),
-                                                                        k.data_ptr(), v.data_ptr()))
-    return k, v
+    return _read(cache._raw, (cache._device, n, cache.n_kv_heads), pages, lengths, start)
 
 
-@functools.lru_cache(maxsize=4096)
-def _attention_plan(dev, kind, n_kv, n_pool, scale, q, pages, lengths, mask, counts, out):
+_ATTEND = ("q", "pages", "lengths", "mask", "counts", "out")
+
+
+def _attention_plan(extras, tensors):
+    dev, kind, n_kv, n_pool, scale = extras
+    q, pages, lengths, mask, counts, out = _looks(_ATTEND, tensors)
     B, n_pages, pages_b = _tables(dev, pages, lengths, counts)
     qB, T, group, qs = _heads("q", q, n_kv)
     _need(qB == B, f"q has {qB} sequences, pages {B}")
-    out = q if out is None else out          # (a new one, contiguous as q is)
+    out = _look(torch.empty_like(tensors[0])) if out is None else out
     _need(out[0] == q[0], "out must have the shape of q")
     os = _heads("out", out, n_kv)[3]
     words, mask_b, mask_t = -(-T // 64), 0, 0
@@ -345,11 +352,15 @@ def _attention_plan(dev, kind, n_kv, n_pool, scale, q, pages, lengths, mask, cou
         _need(words == 1 or st[-1] == 1, "mask: a token's words must lie one behind the other")
         mask_t, mask_b = st[-2], st[0] if len(size) == 3 else 0
     _same_device(dev, ("q", "out", "mask"), (q, out, mask))
+    _here(dev)
     if B == 0 or T == 0:
         return None, 0
     values = (B, T, group, n_pages, words, D ** -0.5 if scale is None else scale, *qs, *os, pages_b, mask_b, mask_t)
     sizes = runtime.TreeAttention(runtime.Cache(*(0,) * 12, kind, n_kv, n_pool), *values)
     return _fixed(runtime.TreeAttention, values), runtime.tree_attention_workspace(sizes)
+
+
+_attend = _site("vdc_tree_attention", _attention_plan, 0, "out", _ATTEND, ("q", "out", "pages", "lengths", "counts", "mask", "work"), timed=True)
 
 
 def tree_attention(q, cache: KVCache, pages, lengths, mask=None, counts=None, scale: Optional[float] = None, out=None) -> torch.Tensor:
@@ -365,24 +376,8 @@ def tree_attention(q, cache: KVCache, pages, lengths, mask=None, counts=None, sc
 
     Scores, softmax and sums are fp32.  A token with nothing to attend to gets zeros."""
     _need(isinstance(cache, KVCache), "cache must be a KVCache")
-    given = out
-    if out is None and isinstance(q, torch.Tensor):
-        out = torch.empty_like(q)
-        given = None if q.is_contiguous() else out
-    elif out is q:
-        raise ValueError("out must not be q")
-    c, dev = cache._c, cache._device
-    plan, nbytes = _attention_plan(dev, c.kind, c.n_kv, c.n_pages, scale, *_looks(
-        ("q", "pages", "lengths", "mask", "counts", "out"), (q, pages, lengths, mask, counts, given)))
-    if plan is None:
-        return out
-    p_q, p_out = q.data_ptr(), out.data_ptr()
-    _need(p_q != p_out, "out must not be q")
-    work = q.new_empty(nbytes // 2)
-    _run("vdc_tree_attention", dev, cache._raw + plan + _PACK7(
-        p_q, p_out, pages.data_ptr(), lengths.data_ptr(), 0 if counts is None else counts.data_ptr(),
-        0 if mask is None else mask.data_ptr(), work.data_ptr()), 0)
-    return out
+    c = cache._c
+    return _attend(cache._raw, (cache._device, c.kind, c.n_kv, c.n_pages, scale), q, pages, lengths, mask, counts, out)
 
 
 _LOGITS = ("logits", "out", "requests", "history", "prompt_lens", "history_lens", "path", "repetition", "frequency", "presence", "bias_ids",
@@ -391,13 +386,14 @@ _LOGIT_TABLES = dict(history=(I32, 2), prompt_lens=(I32, 1), history_lens=(I32, 
                      bias_ids=(I32, 2), bias=(F32, 2), path=(I32, 2), allowed=(I32, 2), requests=(I32, 1))
 
 
-@functools.lru_cache(maxsize=4096)
-def _logits_plan(*looks):
+def _logits_plan(extras, tensors):
+    looks = _looks(_LOGITS, tensors)
     of = dict(zip(_LOGITS, looks))
     logits, out, bias, bias_ids, allowed = (of[x] for x in ("logits", "out", "bias", "bias_ids", "allowed"))
     _need(logits is not None and logits[3] >= 0 and logits[2] in _FLOATS and len(logits[0]) == 2, "logits must be [rows, vocab] fp32, bf16 or f16 on the GPU")
     rows, vocab = logits[0]
     _need(vocab >= 1 and (vocab == 1 or logits[1][1] == 1), "a row's logits must lie one behind the other")
+    out = (logits[0], (vocab, 1), *logits[2:]) if out is None else out
     _need(out[0] == logits[0] and out[2] in (logits[2], F32) and (vocab == 1 or out[1][1] == 1), "out must be like the logits, or fp32")
     n = None
     width, step = {}, {}
@@ -424,10 +420,14 @@ def _logits_plan(*looks):
     n = rows if n is None else n
     _need(of["requests"] is not None or n == rows, f"{n} requests for {rows} rows: requests must say which row is whose")
     _same_device(logits[3], _LOGITS, looks)
+    _here(logits[3])
     if rows == 0:
-        return None
+        return None, 0
     return _fixed(runtime.AdjustLogits, (rows, vocab, _FLOATS[logits[2]], _FLOATS[out[2]], n, width["history"], width["path"], width["bias"],
-                                         logits[1][0], out[1][0], step["history"], step["path"], step["bias_ids"], step["allowed"]))
+                                         logits[1][0], out[1][0], step["history"], step["path"], step["bias_ids"], step["allowed"])), 0
+
+
+_adjust = _site("vdc_adjust_logits", _logits_plan, 2, "out", _LOGITS, ("logits", "out", "tokens") + _LOGITS[2:])
 
 
 def adjust_logits(logits, requests=None, history=None, prompt_lens=None, history_lens=None, path=None, repetition=None, frequency=None,
@@ -449,14 +449,6 @@ def adjust_logits(logits, requests=None, history=None, prompt_lens=None, history
     one = isinstance(logits, torch.Tensor) and logits.dim() == 1
     if one:
         logits, out = logits[None], out[None] if isinstance(out, torch.Tensor) else out
-    _need(isinstance(logits, torch.Tensor), "logits must be [rows, vocab] fp32, bf16 or f16 on the GPU")
-    if out is None:
-        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-    plan = _logits_plan(*_looks(_LOGITS, (logits, out, requests, history, prompt_lens, history_lens, path, repetition, frequency, presence,
-                                          bias_ids, bias, allowed)))
-    tokens = logits.new_empty(logits.shape[0], dtype=I32)
-    if plan is not None:
-        tables = (requests, history, prompt_lens, history_lens, path, repetition, frequency, presence, bias_ids, bias, allowed)
-        _run("vdc_adjust_logits", logits.get_device(), plan + _PACK14(
-            logits.data_ptr(), out.data_ptr(), tokens.data_ptr(), *[0 if t is None else t.data_ptr() for t in tables]))
+    out, tokens = _adjust(b"", (), logits, out, requests, history, prompt_lens, history_lens, path, repetition, frequency, presence, bias_ids,
+                          bias, allowed)
     return (out[0] if one else out), tokens

@@ -95,9 +95,6 @@ _lib.vdc_read_cache.argtypes = [ctypes.POINTER(ReadCache), _u64]
 _lib.vdc_tree_attention_workspace.argtypes = [ctypes.POINTER(TreeAttention), ctypes.POINTER(_u64)]
 _lib.vdc_tree_attention.argtypes = [ctypes.POINTER(TreeAttention), _u64, _u64]
 _lib.vdc_adjust_logits.argtypes = [ctypes.POINTER(AdjustLogits), _u64]
-# the same entries for structures that are bytes already
-_from_bytes = {n: ctypes.CFUNCTYPE(_i32, ctypes.c_char_p, *[_u64] * (2 if n == "vdc_tree_attention" else 1))((n, _lib))
-               for n in ("vdc_rope_append", "vdc_read_cache", "vdc_tree_attention", "vdc_adjust_logits")}
 _lib.vdc_wide_tiles.argtypes = [_i32] * 6 + [ctypes.POINTER(_i32)]
 _lib.vdc_read_status.argtypes = [_u64, ctypes.POINTER(Status), _i32]
 _lib.vdc_build_tma_desc.argtypes = [_vp, _vp, _i32, _i32, ctypes.POINTER(_u64), ctypes.POINTER(_u64),
@@ -263,15 +260,6 @@ def launch_step(step, stream=0, timeout_ns=0):
     """Enqueues one token of a model at batch 1; no synchronisation."""
     init()
     _check(_lib.vdc_launch_step(ctypes.byref(step), int(stream), int(timeout_ns)))
-
-
-def enqueue(name, device, args, *rest):
-    """Calls the entry `name` of the operators below with an argument structure given as bytes; `device` is the current one."""
-    if device not in _initialised:
-        init()
-    rc = _from_bytes[name](args, *rest)
-    if rc != 0:
-        raise VdcError(rc, last_error())
 
 
 def rope_append(args, stream=0):
