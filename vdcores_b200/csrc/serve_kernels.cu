@@ -519,12 +519,8 @@ adjust_logits(const __grid_constant__ vdc_adjust_logits_args a, const __grid_con
           return g1 > g0 && (unsigned)token < (unsigned)a.vocab && k < (unsigned)(g1 - g0) * 8 ? (int)k : -1;
         };
         auto enter = [&](int k) { atomicOr(is_listed + (k >> 5), 1u << (k & 31)); };
-        int n_hist = 0, n_prompt = 0;
         const int* hist = reinterpret_cast<const int*>(a.history) + req * a.history_s;
-        if (seen_matters && a.history) {
-          n_hist = a.history_lens ? max(0, min(a.L, __ldg(reinterpret_cast<const int*>(a.history_lens) + req))) : a.L;
-          n_prompt = a.prompt_lens ? max(0, min(n_hist, __ldg(reinterpret_cast<const int*>(a.prompt_lens) + req))) : 0;
-        }
+        const bool has_text = seen_matters && a.history;
         // all loads first: text, paths, biases
         constexpr int kBatch = 8;
         int k[kBatch];
@@ -542,12 +538,17 @@ adjust_logits(const __grid_constant__ vdc_adjust_logits_args a, const __grid_con
         }
         auto fetch_text = [&](int i0) {
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j) k[j] = n_hist ? __ldg(hist + min(i0 + j * kLogitThreads, n_hist - 1)) : -1;
+          for (int j = 0; j < kBatch; ++j) k[j] = has_text && i0 + j * kLogitThreads < a.L ? __ldg(hist + i0 + j * kLogitThreads) : -1;
         };
         fetch_text(tid);                         // (the first ones are on their way while the table is cleared)
+        int n_hist = 0, n_prompt = 0;
+        if (has_text) {
+          n_hist = a.history_lens ? max(0, min(a.L, __ldg(reinterpret_cast<const int*>(a.history_lens) + req))) : a.L;
+          n_prompt = a.prompt_lens ? max(0, min(n_hist, __ldg(reinterpret_cast<const int*>(a.prompt_lens) + req))) : 0;
+        }
         const int n_words = (g1 - g0 + 3) / 4;
         for (int i = tid; i < n_words; i += kLogitThreads) is_listed[i] = 0;
-        for (int i = tid; i < plan.cap; i += kLogitThreads) list[i] = LogitEntry{0, 0.f};
+        for (int i = tid; i < min(plan.cap, n_hist + n_paths + n_bias); i += kLogitThreads) list[i] = LogitEntry{0, 0.f};
         __syncthreads();
         for (int i0 = tid; i0 < n_hist; i0 += kLogitThreads * kBatch) {
           if (i0 != tid) fetch_text(i0);
