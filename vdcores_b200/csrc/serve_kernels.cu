@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kReadThreads) read_cache(const vdc_read_cache_
 // compared; a listed one takes a turn by itself.
 // (Gathering the listed ones' logits afterwards, one to a thread, took as long as the rows themselves.)
 // 512 rows of 151936 bf16 logits, texts of 2048 .. 4096, 32 biases, masks: 80 us, 4.0 TB/s; two thirds of the issue slots, half of that for
-// the listed tokens.  One row of 128256: 12.4 us, of which the list takes 4.
+// the listed tokens.  One row of 128256: 12.1 us, of which the list takes 3.
 // ------------------------------------------------------------------------- //
 constexpr int kLogitThreads = 512, kLogitChunk = 8, kLogitMaxBias = 4096, kLogitMaxPath = 64;
 constexpr int kLogitTile = 262144, kLogitMaxNamed = 12288, kLogitSmallTile = 16384;      // tokens of a tile with so many listed ones at most, with more
