@@ -149,6 +149,7 @@ PyObject* site_call(PyObject* self, PyObject* const* args, size_t nargsf, PyObje
       PyErr_Format(PyExc_ValueError, "the tensors are on cuda:%d, the current device is cuda:%d", dev, (int)c10::cuda::current_device());
       return nullptr;
     }
+    // (attention reads all of q while others write; its entry is the one with a limit for waits)
     if (s.makes == kOutLike && s.timed && out.data_ptr() == t[0]->data_ptr()) {
       PyErr_SetString(PyExc_ValueError, "out must not be q");
       return nullptr;
