@@ -19,7 +19,7 @@
 // memory, in two passes of the 8-bit tensor cores.  V is widened to f16 (exact) by two more teams of four warps; P is f16 as well (its
 // 11 bits are three more than the bf16 weights of bf16 caches have).
 //
-// Measured on one B200, calls back to back: 8 tokens over 131000 e4m3 rows 77 us (277 MB, 3.6 TB/s; steps alone 0.9 of the copy rate),
+// Measured on one B200, calls back to back: 8 tokens over 131000 e4m3 rows 75.5 us (277 MB, 3.7 TB/s; steps alone 0.9 of the copy rate),
 // 64 tokens over 1056 .. 2112 e4m3 rows 57 us (215 MB, 3.8 TB/s), one token over 333 bf16 rows 9 us, 4 trees of 63 tokens with 8 heads a
 // group over 1025 .. 2050 bf16 rows 29 us.  Long sequences are bound by memory; short ones by a CTA's start, its steps in series (a wait
 // for the scores, tensor memory, the group's barrier, weights, shared memory) and what joins the pieces.
@@ -1033,7 +1033,8 @@ struct KeysCfg {
   static constexpr int kLoadWarp = kMathWarps + (kF8 ? 8 : 0), kScoreWarp = kLoadWarp + 1, kSumWarp = kLoadWarp + 2;
   static constexpr int kThreads = kF8 ? 640 : 384, kMathRegs = kF8 ? (R <= 16 ? 104 : R <= 32 ? 120 : 128) : 208, kOtherRegs = kF8 ? (R <= 16 ? 88 : R <= 32 ? 80 : 72) : 88;
   static_assert(kMathWarps * 32 * kMathRegs + (kThreads - kMathWarps * 32) * kOtherRegs <= kThreads * (kF8 ? 96 : 168), "registers of a launch");
-  static constexpr int kCodes = R <= 16 ? 8 : 4;                        // pieces of codes that a thread widens at a time
+  static constexpr int kCodes = 4;                                      // pieces of codes that a thread widens at a time: the roles share the
+                                                                        // instruction cache (eight: 55.5 -> 57 us at 64 sequences)
   // powers of two by which a score may exceed its reference, and by which f16 weights are kept larger (2^15 at most)
   static constexpr float kSlack = kF8 ? 4.f : 8.f, kLift = kF8 ? 11.f : 0.f;
 };
@@ -1263,7 +1264,7 @@ tree_attention_keys(const __grid_constant__ vdc_tree_attention_args a, const __g
           ok = all_well(good, wait, 3, i);
           if (!ok) break;
           const int left = end - i * PAGE, own = p.ctx - i * PAGE;
-#pragma unroll
+#pragma unroll 1
           for (int j0 = 0; j0 < 8; j0 += C::kCodes) {
             uint4 code[C::kCodes];
 #pragma unroll
