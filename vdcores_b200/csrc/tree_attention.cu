@@ -449,16 +449,10 @@ template <int kThreads>
 __device__ __forceinline__ bool names_no_page(const vdc_tree_attention_args& a, const Piece& p, int tid, vdc_status* status) {
   bool found = false;
   int which = 0;
-  for (int i0 = tid; i0 < p.np; i0 += kThreads * 8) {
-    int id[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) id[j] = i0 + kThreads * j < p.np ? __ldg(reinterpret_cast<const int*>(a.pages) + p.b * a.pages_b + i0 + kThreads * j) : 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (id[j] < 0 || id[j] >= a.cache.n_pages) {
-        found = true;
-        which = id[j];
-      }
+#pragma unroll 4
+  for (int i = tid; i < p.np; i += kThreads) {
+    const int id = __ldg(reinterpret_cast<const int*>(a.pages) + p.b * a.pages_b + i);
+    if (id < 0 || id >= a.cache.n_pages) found = true, which = id;
   }
   if (found) report(status, VDC_ERR_RANGE, VDC_TREE_ATTENTION_KIND, 1, p.b, which);
   return found;
